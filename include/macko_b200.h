@@ -436,6 +436,62 @@ int macko_decode_rope_attention(const void *qkv, const void *cos_table, const vo
 int macko_decode_silu_mul(const void *gate_up, void *out, int64_t n, void *stream);
 int macko_decode_argmax(const void *values, int64_t n, int64_t *index, void *stream);
 
+/*
+ * A key/value cache in 8 bits, in pages, for several sequences (the reference has none). Keys and values of a page and head
+ * are codes times one scale: value = code * scale. Page j of sequence i is page_table[i * table_stride + j]; it holds the
+ * sequence's tokens j * page_size .. j * page_size + page_size - 1. lengths[i] counts the tokens of sequence i, the rows of the
+ * call included: rows query_start[i] .. query_start[i + 1] - 1 of the call are its last ones, at positions lengths[i] - n .. lengths[i] - 1
+ * (query_start NULL: one row per sequence, rows == sequences). page_table, lengths and query_start are read on the device, so a
+ * captured call can be replayed after they have been rewritten. Nothing outside the buffers is touched whatever they hold: a page
+ * number outside 0 .. pages - 1 is a page that is not there (its tokens are not written, and nobody sees them); a row at a
+ * negative position (a sequence shorter than its rows: length 0 is a sequence that is not served) or behind the last page that
+ * the table can name is not appended, and rows that belong to no sequence give zeros.
+ */
+#define MACKO_KV_INT8 0 /* codes are int8, -127 .. 127 */
+#define MACKO_KV_E4M3 1 /* codes are 8-bit floating point, 4 bits of exponent and 3 of fraction, at most 448 */
+#define MACKO_FP16 0
+#define MACKO_BF16 1
+
+typedef struct macko_kv_cache {
+    void *k, *v;                             /* [pages][kv_heads][page_size][head_dim] codes, 16-byte aligned */
+    float *k_scale, *v_scale;                /* [pages][kv_heads], greater than zero */
+    int64_t k_page_stride, v_page_stride;    /* bytes between pages, multiples of 16 */
+    int64_t k_scale_stride, v_scale_stride;  /* floats between pages */
+    int64_t pages;
+    int32_t kv_heads, page_size, head_dim, code; /* page_size 16, 32, 64 or 128; head_dim 64, 128 or 256; MACKO_KV_* */
+} macko_kv_cache;
+
+typedef struct macko_kv_rows {
+    const int32_t *page_table; /* [sequences][table_width] */
+    const int32_t *lengths;    /* [sequences] */
+    const int32_t *query_start; /* [sequences + 1], not decreasing, or NULL */
+    int64_t table_stride, table_width, sequences, rows;
+} macko_kv_rows;
+
+/*
+ * macko_cache_rope_append: qkv holds `rows` rows of (heads + 2 * kv_heads) * head_dim values (q, then k, then v), row_stride
+ *   elements apart (16-byte aligned rows). q and k are rotated at their row's position (rotate-half, fp16 tables
+ *   [>= table_width * page_size][head_dim] with both halves equal); the rotated q, rounded once, goes to q [rows][heads][head_dim],
+ *   k and v into the cache. The scale of a page and head is the smallest power of two, not below 2^-64, with which the call's
+ *   rows on that page fit the codes, or the scale that the page has if that is larger and the page held tokens of the sequence
+ *   before; those are moved to the new scale where it grows. A value that is not finite makes the scale of its page and head NaN,
+ *   for good: whoever attends to that page gets NaN. Slots behind the last token keep their bytes. A page must be written for
+ *   one sequence only in one call, and calls that write one page must not overlap.
+ * macko_cache_attention: out[row][head] = sum over the tokens t at or before the row's position of softmax(scale * q . k_t) v_t, in
+ *   out [rows][heads][head_dim]; head h reads key head h / (heads / kv_heads). A row that sees nothing gives zeros. q: rows
+ *   q_row_stride and heads q_head_stride elements apart, both multiples of 8, 16-byte aligned. `workspace`: scratch of this call
+ *   alone of macko_cache_attention_workspace_bytes(...) bytes, 16-byte aligned (the size depends on the arguments that it
+ *   takes and on the current device; negative: they are out of range).
+ * Both launch with programmatic stream serialization, like the products.
+ */
+int macko_cache_rope_append(const macko_kv_cache *cache, const macko_kv_rows *batch, const void *qkv, int64_t row_stride, int32_t type,
+                            const void *cos_table, const void *sin_table, void *q, int32_t heads, void *stream);
+int64_t macko_cache_attention_workspace_bytes(int64_t sequences, int64_t rows, int64_t table_width, int32_t heads, int32_t kv_heads,
+                                              int32_t page_size, int32_t head_dim, int32_t one_row_each);
+int macko_cache_attention(const macko_kv_cache *cache, const macko_kv_rows *batch, const void *q, int64_t q_row_stride,
+                          int64_t q_head_stride, int32_t type, void *out, int32_t heads, float scale, void *workspace,
+                          int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -145,6 +145,17 @@ def _argmax_fake(values):
     return values.new_empty((1,), dtype=torch.int64)
 
 
+@torch.library.register_fake("macko_spmv::rope_append")
+def _rope_append_fake(qkv, cos_table, sin_table, k_cache, v_cache, k_scale, v_scale, page_table, lengths, query_start=None):
+    _, kv_heads, _, head_dim = k_cache.shape
+    return qkv.new_empty((qkv.shape[0], qkv.shape[1] // head_dim - 2 * kv_heads, head_dim))
+
+
+@torch.library.register_fake("macko_spmv::paged_attention")
+def _paged_attention_fake(q, k_cache, v_cache, k_scale, v_scale, page_table, lengths, query_start=None, scale=None):
+    return q.new_empty(q.shape)
+
+
 def move_to_device(compressed, device):
     """Move the three buffers of a compressed matrix (src/macko_spmv/__init__.py:110-117)."""
     return (
@@ -442,5 +453,7 @@ def multiply_batched(compressed_M, V):
     return torch.ops.macko_spmv.multiply_batched.default(*compressed_M[:5], V)
 
 
-__all__ = ["compress", "multiply", "multiply_batched", "decompress", "move_to_device", "freeze", "rows_are_even", "FrozenMatrix",
+from .kv_cache import KVCache, new_cache, paged_attention, rope_append  # noqa: E402  (needs the loaded operators)
+
+__all__ = ["KVCache", "new_cache", "rope_append", "paged_attention", "compress", "multiply", "multiply_batched", "decompress", "move_to_device", "freeze", "rows_are_even", "FrozenMatrix",
            "native_library_paths", "native_version", "LIB_NAME"]

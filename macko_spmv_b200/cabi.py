@@ -42,6 +42,28 @@ class PlanInfo(ctypes.Structure):
     ]
 
 
+class KVCache(ctypes.Structure):
+    """``macko_kv_cache``: a paged key/value cache in 8 bits."""
+
+    _fields_ = [
+        ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp),
+        ("k_page_stride", _i64), ("v_page_stride", _i64), ("k_scale_stride", _i64), ("v_scale_stride", _i64), ("pages", _i64),
+        ("kv_heads", _i32), ("page_size", _i32), ("head_dim", _i32), ("code", _i32),
+    ]
+
+
+class KVRows(ctypes.Structure):
+    """``macko_kv_rows``: which rows of a call belong to which sequence, and where those lie in the cache."""
+
+    _fields_ = [
+        ("page_table", _vp), ("lengths", _vp), ("query_start", _vp),
+        ("table_stride", _i64), ("table_width", _i64), ("sequences", _i64), ("rows", _i64),
+    ]
+
+
+KV_INT8, KV_E4M3 = 0, 1
+FP16, BF16 = 0, 1
+
 SIGNATURES = {
     "macko_version": (_int, []),
     "macko_status_string": (ctypes.c_char_p, [_int]),
@@ -82,6 +104,9 @@ SIGNATURES = {
     "macko_decode_rope_attention": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp]),
     "macko_decode_silu_mul": (_int, [_vp, _vp, _i64, _vp]),
     "macko_decode_argmax": (_int, [_vp, _i64, _vp, _vp]),
+    "macko_cache_rope_append": (_int, [ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp]),
+    "macko_cache_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32]),
+    "macko_cache_attention": (_int, [ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), _vp, _i64, _i64, _i32, _vp, _i32, _f, _vp, _i64, _vp]),
 }
 
 

@@ -17,6 +17,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace macko {
 namespace {
@@ -407,32 +408,6 @@ rope_attention_kernel(const __half *__restrict__ qkv, const __half *__restrict__
     if (csize > 1) cluster_barrier();   // the other CTAs' shared memory stays until the first one has read it
 }
 
-template <typename T> struct Same { using type = T; };
-
-// `cluster` > 1: thread-block clusters of that many CTAs along x (the grid is a multiple of it).
-template <typename... Args>
-int launch_pdl(const char *what, void (*kernel)(Args...), dim3 grid, dim3 block, int cluster, cudaStream_t stream,
-               typename Same<Args>::type... args)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    if (e == cudaSuccess) e = cudaGetLastError();
-    if (e != cudaSuccess) return fail(MACKO_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
-    return MACKO_OK;
-}
-
 }  // namespace
 }  // namespace macko
 
@@ -448,7 +423,7 @@ static int add_rmsnorm_checked(void *x, const void *pending, int n_pending, int6
         (n_pending > 0 && pending_stride < n))
         return fail(MACKO_ERR_INVALID_ARGUMENT, "add_rmsnorm: n=%lld n_pending=%d stride=%lld or a null pointer",
                     (long long)n, n_pending, (long long)pending_stride);
-    return launch_pdl("add_rmsnorm", add_rmsnorm_kernel, dim3(1), dim3(kNormThreads), 1, static_cast<cudaStream_t>(stream),
+    return launch_pdl("add_rmsnorm", add_rmsnorm_kernel, dim3(1), dim3(kNormThreads), 1, 0, static_cast<cudaStream_t>(stream),
                       static_cast<__half *>(x), static_cast<const __half *>(pending), n_pending, (long long)pending_stride,
                       static_cast<const __half *>(weight), static_cast<__half *>(out), (int)n, eps,
                       reinterpret_cast<unsigned *>(peer_flags), world, (unsigned)(spin_limit == 0 ? (1u << 23) : spin_limit));
@@ -474,7 +449,7 @@ int macko_decode_silu_mul(const void *gate_up, void *out, int64_t n, void *strea
     if (!gate_up || !out || n <= 0 || n > (1 << 28))
         return fail(MACKO_ERR_INVALID_ARGUMENT, "silu_mul: n=%lld or a null pointer", (long long)n);
     const int ctas = (int)((n / 8 + 255) / 256) > 0 ? (int)((n / 8 + 255) / 256) : 1;
-    return launch_pdl("silu_mul", silu_mul_kernel, dim3(ctas > 296 ? 296 : ctas), dim3(256), 1, static_cast<cudaStream_t>(stream),
+    return launch_pdl("silu_mul", silu_mul_kernel, dim3(ctas > 296 ? 296 : ctas), dim3(256), 1, 0, static_cast<cudaStream_t>(stream),
                       static_cast<const __half *>(gate_up), static_cast<__half *>(out), (int)n);
 }
 
@@ -482,7 +457,7 @@ int macko_decode_argmax(const void *values, int64_t n, int64_t *index, void *str
 {
     if (!values || !index || n <= 0 || n > (1 << 30))
         return fail(MACKO_ERR_INVALID_ARGUMENT, "argmax: n=%lld or a null pointer", (long long)n);
-    return launch_pdl("argmax", argmax_kernel, dim3(1), dim3(1024), 1, static_cast<cudaStream_t>(stream),
+    return launch_pdl("argmax", argmax_kernel, dim3(1), dim3(1024), 1, 0, static_cast<cudaStream_t>(stream),
                       static_cast<const __half *>(values), (int)n, reinterpret_cast<long long *>(index));
 }
 
@@ -505,7 +480,7 @@ int macko_decode_rope_attention(const void *qkv, const void *cos_table, const vo
     while (cluster > 1 && (long long)heads * cluster > dev->sm_count) cluster >>= 1;
     const dim3 grid((unsigned)(heads * cluster)), block(kAttnWarps * 32);
 #define MACKO_ATTN(V)                                                                                                   \
-    return launch_pdl("rope_attention", rope_attention_kernel<V>, grid, block, cluster, s, static_cast<const __half *>(qkv), \
+    return launch_pdl("rope_attention", rope_attention_kernel<V>, grid, block, cluster, 0, s, static_cast<const __half *>(qkv), \
                       static_cast<const __half *>(cos_table), static_cast<const __half *>(sin_table),                    \
                       reinterpret_cast<const long long *>(position), static_cast<__half *>(k_cache),                     \
                       static_cast<__half *>(v_cache), static_cast<__half *>(out), heads, max_len, scale)

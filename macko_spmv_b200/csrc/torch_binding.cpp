@@ -14,6 +14,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <cmath>
+#include <optional>
 #include <tuple>
 
 #include "macko_b200.h"
@@ -483,6 +485,124 @@ at::Tensor argmax_cuda(const at::Tensor &values)
     return out;
 }
 
+// ---- the paged 8-bit cache (macko_cache_*) ---------------------------------------------------------------
+
+// The stride of dimension 0, whatever PyTorch says about it where there is one entry or none.
+int64_t outer_stride(const at::Tensor &t)
+{
+    int64_t inner = 1;
+    for (int64_t d = 1; d < t.dim(); ++d) inner *= t.size(d);
+    return t.size(0) > 1 ? t.stride(0) : inner;
+}
+
+bool inner_contiguous(const at::Tensor &t)
+{
+    int64_t inner = 1;
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+        if (t.size(d) != 1 && t.stride(d) != inner) return false;
+        inner *= t.size(d);
+    }
+    return true;
+}
+
+macko_kv_cache checked_cache(const at::Tensor &x, const at::Tensor &k, const at::Tensor &v, const at::Tensor &ks, const at::Tensor &vs)
+{
+    for (const at::Tensor *t : {&k, &v, &ks, &vs}) TORCH_CHECK(t->is_cuda() && t->device() == x.device(), "the cache must be on the device of the rows");
+    TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(), "k and v of the cache must be [pages, kv_heads, page_size, head_dim]");
+    TORCH_CHECK((k.dtype() == at::kChar || k.dtype() == at::kFloat8_e4m3fn) && v.dtype() == k.dtype(), "the cache holds torch.int8 or torch.float8_e4m3fn");
+    TORCH_CHECK(ks.dim() == 2 && ks.size(0) == k.size(0) && ks.size(1) == k.size(1) && vs.sizes() == ks.sizes() && ks.dtype() == at::kFloat &&
+                    vs.dtype() == at::kFloat,
+                "the scales of the cache must be torch.float32 [pages, kv_heads]");
+    TORCH_CHECK(inner_contiguous(k) && inner_contiguous(v) && inner_contiguous(ks) && inner_contiguous(vs), "every page of the cache must be contiguous");
+    TORCH_CHECK(k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX && k.size(3) <= INT32_MAX, "cache too large");
+    return {k.data_ptr(), v.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), outer_stride(k), outer_stride(v), outer_stride(ks),
+            outer_stride(vs), k.size(0), (int32_t)k.size(1), (int32_t)k.size(2), (int32_t)k.size(3),
+            k.dtype() == at::kChar ? MACKO_KV_INT8 : MACKO_KV_E4M3};
+}
+
+macko_kv_rows checked_rows(const at::Tensor &x, const at::Tensor &table, const at::Tensor &lengths, const std::optional<at::Tensor> &start)
+{
+    TORCH_CHECK(table.is_cuda() && lengths.is_cuda() && table.device() == x.device() && lengths.device() == x.device(),
+                "page_table and lengths must be on the device of the rows");
+    TORCH_CHECK(table.dtype() == at::kInt && lengths.dtype() == at::kInt, "page_table and lengths must be torch.int32");
+    TORCH_CHECK(table.dim() == 2 && lengths.dim() == 1 && table.size(0) == lengths.size(0), "page_table must be [sequences, pages] and lengths [sequences]");
+    TORCH_CHECK(inner_contiguous(table) && lengths.is_contiguous(), "page_table and lengths must be contiguous");
+    if (start.has_value()) {
+        TORCH_CHECK(start->is_cuda() && start->device() == x.device() && start->dtype() == at::kInt && start->dim() == 1 &&
+                        start->size(0) == lengths.size(0) + 1 && start->is_contiguous(),
+                    "query_start must be torch.int32 [sequences + 1] on the device of the rows");
+    } else {
+        TORCH_CHECK(x.size(0) == lengths.size(0), "without query_start every sequence has one row");
+    }
+    return {table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), start.has_value() ? start->data_ptr<int32_t>() : nullptr,
+            outer_stride(table), table.size(1), lengths.size(0), x.size(0)};
+}
+
+int32_t checked_type(const at::Tensor &x, const char *name)
+{
+    TORCH_CHECK(x.is_cuda() && (x.dtype() == at::kHalf || x.dtype() == at::kBFloat16), name, " must be a CUDA tensor of torch.half or torch.bfloat16");
+    return x.dtype() == at::kHalf ? MACKO_FP16 : MACKO_BF16;
+}
+
+}  // namespace
+
+namespace macko_torch {
+
+at::Tensor rope_append_cuda(const at::Tensor &qkv, const at::Tensor &cos_table, const at::Tensor &sin_table, at::Tensor k_cache,
+                            at::Tensor v_cache, at::Tensor k_scale, at::Tensor v_scale, const at::Tensor &page_table,
+                            const at::Tensor &lengths, const std::optional<at::Tensor> &query_start)
+{
+    const int32_t type = checked_type(qkv, "qkv");
+    TORCH_CHECK(qkv.dim() == 2 && inner_contiguous(qkv), "qkv must be [rows, (heads + 2 kv_heads) head_dim] with contiguous rows");
+    const macko_kv_cache cache = checked_cache(qkv, k_cache, v_cache, k_scale, v_scale);
+    const macko_kv_rows rows = checked_rows(qkv, page_table, lengths, query_start);
+    const int64_t hd = cache.head_dim, hkv = cache.kv_heads, heads = hd > 0 ? qkv.size(1) / hd - 2 * hkv : 0;
+    TORCH_CHECK(heads > 0 && heads <= INT32_MAX && (heads + 2 * hkv) * hd == qkv.size(1), "qkv must hold q, k and v of ", hkv, " key heads of ", hd);
+    check_half_vec(cos_table, "cos_table");
+    check_half_vec(sin_table, "sin_table");
+    TORCH_CHECK(cos_table.device() == qkv.device() && sin_table.device() == qkv.device(), "tensors on different devices");
+    TORCH_CHECK(cos_table.dim() == 2 && cos_table.size(1) == hd && cos_table.size(0) >= rows.table_width * cache.page_size &&
+                    sin_table.sizes() == cos_table.sizes(),
+                "cos/sin tables must be [>= positions of the page table, head_dim]");
+    const c10::cuda::CUDAGuard guard(qkv.device());
+    at::Tensor q = at::empty({qkv.size(0), heads, hd}, qkv.options());
+    check_status(macko_cache_rope_append(&cache, &rows, qkv.data_ptr(), outer_stride(qkv), type, cos_table.data_ptr(), sin_table.data_ptr(),
+                                         q.data_ptr(), (int32_t)heads, c10::cuda::getCurrentCUDAStream()),
+                 "macko_cache_rope_append");
+    return q;
+}
+
+at::Tensor paged_attention_cuda(const at::Tensor &q, const at::Tensor &k_cache, const at::Tensor &v_cache, const at::Tensor &k_scale,
+                                const at::Tensor &v_scale, const at::Tensor &page_table, const at::Tensor &lengths,
+                                const std::optional<at::Tensor> &query_start, std::optional<double> scale)
+{
+    const int32_t type = checked_type(q, "q");
+    const macko_kv_cache cache = checked_cache(q, k_cache, v_cache, k_scale, v_scale);
+    const macko_kv_rows rows = checked_rows(q, page_table, lengths, query_start);
+    const int64_t hd = cache.head_dim;
+    TORCH_CHECK(q.dim() == 3 && q.size(2) == hd && q.size(1) <= INT32_MAX, "q must be [rows, heads, ", hd, "]");
+    TORCH_CHECK(q.size(2) == 1 || q.stride(2) == 1, "the last dimension of q must be contiguous");
+    const int64_t heads = q.size(1), head_stride = heads > 1 ? q.stride(1) : hd, row_stride = q.size(0) > 1 ? q.stride(0) : heads * head_stride;
+    const c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor out = at::empty({q.size(0), heads, hd}, q.options());
+    const int64_t bytes = macko_cache_attention_workspace_bytes(rows.sequences, rows.rows, rows.table_width, (int32_t)heads, cache.kv_heads,
+                                                                cache.page_size, cache.head_dim, rows.query_start == nullptr);
+    TORCH_CHECK(bytes >= 0, "macko_cache_attention_workspace_bytes: ", macko_last_error());
+    const at::Tensor workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+    check_status(macko_cache_attention(&cache, &rows, q.data_ptr(), row_stride, head_stride, type, out.data_ptr(), (int32_t)heads,
+                                       (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)hd)), workspace.data_ptr(), bytes,
+                                       c10::cuda::getCurrentCUDAStream()),
+                 "macko_cache_attention");
+    return out;
+}
+
+}  // namespace macko_torch
+
+namespace {
+
+using macko_torch::paged_attention_cuda;
+using macko_torch::rope_append_cuda;
+
 }  // namespace
 
 TORCH_LIBRARY(macko_spmv, m)
@@ -510,6 +630,10 @@ TORCH_LIBRARY(macko_spmv, m)
           "Tensor(b!) v_cache) -> Tensor");
     m.def("silu_mul(Tensor gate_up) -> Tensor");
     m.def("argmax(Tensor values) -> Tensor");
+    m.def("rope_append(Tensor qkv, Tensor cos_table, Tensor sin_table, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, "
+          "Tensor(d!) v_scale, Tensor page_table, Tensor lengths, Tensor? query_start=None) -> Tensor");
+    m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor page_table, Tensor lengths, "
+          "Tensor? query_start=None, float? scale=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(macko_spmv, CUDA, m)
@@ -530,4 +654,6 @@ TORCH_LIBRARY_IMPL(macko_spmv, CUDA, m)
     m.impl("rope_attention", &rope_attention_cuda);
     m.impl("silu_mul", &silu_mul_cuda);
     m.impl("argmax", &argmax_cuda);
+    m.impl("rope_append", &rope_append_cuda);
+    m.impl("paged_attention", &paged_attention_cuda);
 }
