@@ -56,7 +56,7 @@ def _nvcc() -> str:
 
 
 def build_core(force: bool = False, verbose: bool = False) -> str:
-    headers = [os.path.join(CSRC, h) for h in ("common.cuh", "plan.cuh", "unit.cuh", "windows.cuh", "kv_cache.cuh", "launch.cuh")] + [os.path.join(INCLUDE, "macko_b200.h")]
+    headers = [os.path.join(CSRC, h) for h in ("common.cuh", "plan.cuh", "unit.cuh", "windows.cuh", "kv_cache.cuh", "launch.cuh", "attention_work.cuh")] + [os.path.join(INCLUDE, "macko_b200.h")]
     sources = [os.path.join(CSRC, s) for s in CUDA_SOURCES]
     if not force and _newer(LIB_CORE, sources + headers + [__file__]):
         return LIB_CORE

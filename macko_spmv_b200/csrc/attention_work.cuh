@@ -1,0 +1,199 @@
+// How attention over the paged cache is cut into work for a fixed number of CTAs, and how the pieces are put together again.
+//
+// A unit is one head of the cache and the rows of one sequence that meet it together: `queries` consecutive rows of the call with `heads`
+// heads each (a group of more heads than a unit holds is cut into `parts`). It walks the tokens in tiles of `tile`. Units of a sequence
+// are ordered by (head, part), then by rows; block b of the rows ends at position begin + (b + 1) * queries - 1 and takes
+// ceil((begin + (b + 1) * queries) / tile) tiles. All tiles of the call in this order are numbered; CTA c takes numbers
+// [c * share, (c + 1) * share). So every CTA has the same work whatever the lengths are, a unit lies in consecutive CTAs, and a
+// CTA has at most two units that are not its own alone: the one that began before it and the one that goes on after it. Their
+// partial results (maximum, sum, weighted values, fp32) go to scratch memory, and a second small kernel puts them together.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace macko {
+
+struct WorkShape {
+    int queries, heads, parts;   // rows and heads of a unit, parts of a head group
+    int tile;                    // tokens
+    int group, kv_heads;         // heads per cache head, cache heads
+    int ctas, least_share;
+};
+
+// Rows of a unit that goes on in the CTAs behind: what the second kernel needs. pieces 0: nothing.
+struct SplitUnit {
+    int first_row, rows, head, pieces;   // rows = queries * heads, packed query by query
+    int heads, unused[3];
+};
+
+// sum of floor((a * i + b) / m) for i = 0 .. n - 1
+__host__ __device__ inline long long floor_sum(unsigned long long n, unsigned long long m, unsigned long long a, unsigned long long b)
+{
+    unsigned long long sum = 0;
+    while (n > 0) {
+        if (a >= m) {
+            sum += (n - 1) * n / 2 * (a / m);
+            a %= m;
+        }
+        if (b >= m) {
+            sum += n * (b / m);
+            b %= m;
+        }
+        const unsigned long long last = a * n + b;
+        if (last < m) break;
+        n = last / m;
+        b = last % m;
+        const unsigned long long t = m;
+        m = a;
+        a = t;
+    }
+    return (long long)sum;
+}
+
+// Tiles of the first `blocks` row blocks of a sequence whose rows begin at position `begin`, for one (head, part).
+__host__ __device__ inline long long tiles_before(const WorkShape &w, int begin, int blocks)
+{
+    if (blocks == 0) return 0;
+    if (blocks == 1) return ((long long)begin + w.queries + w.tile - 1) / w.tile;
+    return floor_sum(blocks, w.tile, w.queries, (unsigned long long)begin + w.queries + w.tile - 1);
+}
+
+#ifdef __CUDACC__
+
+// One sequence's place in the numbering.
+struct SequenceWork {
+    Sequence rows;
+    int begin, blocks;       // begin: first position, kept inside 0 .. capacity for counting
+    long long per_head, total;
+};
+
+__device__ __forceinline__ SequenceWork sequence_work(const WorkShape &w, const RowsView &r, int i)
+{
+    SequenceWork s;
+    s.rows = sequence_at(r, i);
+    s.begin = min(max(s.rows.begin(), 0), r.capacity);
+    s.blocks = (s.rows.count + w.queries - 1) / w.queries;
+    s.per_head = tiles_before(w, s.begin, s.blocks);
+    s.total = s.per_head * (w.kv_heads * w.parts);
+    return s;
+}
+
+// A run of tiles of one unit, as one CTA walks it.
+struct Piece {
+    int sequence, block, kv_head, part;
+    int first_tile, tiles;   // tiles [first_tile, + tiles) of the unit
+    bool begins, ends;       // whether the unit begins and ends with it
+    int pieces;              // CTAs that share the unit, counted where it begins
+};
+
+// Walks the pieces of CTA `cta`. Every thread of the block calls both functions with the same arguments; `shared`: 40 words.
+struct WorkWalk {
+    long long at, end, share;
+    long long base;          // number of the current sequence's first tile
+    int sequence;
+    SequenceWork s;
+
+    __device__ void start(const WorkShape &w, const RowsView &r, int cta, long long *shared)
+    {
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (blockDim.x + 31) >> 5;
+        // the total, then the sequence with this CTA's first tile
+        long long total = 0, first_own = 0;
+        for (int i = tid; i < r.sequences; i += blockDim.x) {
+            const long long own = sequence_work(w, r, i).total;
+            if (i == tid) first_own = own;
+            total += own;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (lane == 0) shared[warp] = total;
+        if (tid == 0) shared[32] = r.sequences;
+        __syncthreads();
+        total = 0;
+        for (int v = 0; v < warps; ++v) total += shared[v];
+        share = max((total + w.ctas - 1) / w.ctas, (long long)w.least_share);
+        at = share * cta;
+        end = min(at + share, total);
+        sequence = r.sequences;
+        base = 0;
+        __syncthreads();
+        if (at >= end) return;
+        long long before = 0;
+        for (int first = 0; first < r.sequences; first += blockDim.x) {
+            const long long own = first == 0 ? first_own : first + tid < r.sequences ? sequence_work(w, r, first + tid).total : 0;
+            long long sum = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            if (lane == 31) shared[warp] = sum;
+            __syncthreads();
+            long long all = 0;
+            for (int v = 0; v < warps; ++v) {
+                if (v < warp) sum += shared[v];
+                all += shared[v];
+            }
+            const long long lo = before + sum - own;
+            if (at >= lo && at < lo + own) {
+                shared[32] = first + tid;
+                shared[33] = lo;
+            }
+            before += all;
+            __syncthreads();
+            if (at < before) break;
+        }
+        sequence = (int)shared[32];
+        if (sequence >= r.sequences) {   // the lengths have changed under the call: nothing outside the arrays is read for that
+            at = end;
+            return;
+        }
+        base = shared[33];
+        s = sequence_work(w, r, sequence);
+    }
+
+    // The next piece, or false.
+    __device__ bool next(const WorkShape &w, const RowsView &r, Piece &p)
+    {
+        if (at >= end) return false;
+        while (at >= base + s.total) {
+            base += s.total;
+            if (++sequence >= r.sequences) return false;
+            s = sequence_work(w, r, sequence);
+        }
+        const long long local = at - base;
+        const int head_part = (int)(local / s.per_head);
+        const long long rest = local - head_part * s.per_head;
+        int block = 0;
+        long long before = 0;
+        if (s.blocks > 1) {
+            int lo = 0, hi = s.blocks;   // tiles_before(lo) <= rest < tiles_before(hi)
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                const long long t = tiles_before(w, s.begin, mid);
+                if (t <= rest) {
+                    lo = mid;
+                    before = t;
+                } else {
+                    hi = mid;
+                }
+            }
+            block = lo;
+        }
+        const int of_unit = (int)(((long long)s.begin + (long long)(block + 1) * w.queries + w.tile - 1) / w.tile);
+        p.sequence = sequence;
+        p.block = block;
+        p.kv_head = head_part / w.parts;
+        p.part = head_part % w.parts;
+        p.first_tile = (int)(rest - before);
+        p.tiles = (int)min((long long)(of_unit - p.first_tile), end - at);
+        p.begins = p.first_tile == 0;
+        p.ends = p.first_tile + p.tiles == of_unit;
+        p.pieces = p.begins ? (int)((at + of_unit - 1) / share - at / share) + 1 : 0;
+        at += p.tiles;
+        return true;
+    }
+};
+
+#endif  // __CUDACC__
+
+}  // namespace macko

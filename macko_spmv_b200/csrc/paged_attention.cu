@@ -1,97 +1,533 @@
-// Attention over the paged 8-bit cache.
+// Attention over the paged 8-bit cache, for a few rows per sequence and head of the cache: decoding and drafted tokens.
+//
+//   x(t) = scale * (q . k_t) * k_scale(page) * log2 e + log2 v_scale(page)        k_t, v_t: codes
+//   out  = sum 2^(x(t) - m) v_t  /  sum 2^(x(t) - m) / v_scale(page),             m = max x(t)
+//
+// The scale of the values is part of the exponent, so the weights that meet the codes are at most 1 whatever the scales are, and
+// rounding them to fp16 (2^-11 of themselves) is the one rounding on the way; sums, maxima and the accumulators are fp32. Products of
+// codes with fp16 are exact in the tensor core. bfloat16 rows of q become fp16 under a power of two of their own.
+//
+// Bound by HBM: a code is used for 2 to 16 rows. A warp takes 16 or 32 tokens at a time from the cache straight into registers, in the
+// layout that mma.m16n8k16 wants: tokens (for S^T = K Q^T) and dimensions (for O^T = V^T P^T) are its 16 rows, the call's rows its 8 columns, so that
+// one step costs half of what it would the other way round. Which dimensions are "k = 2t, 2t + 1" is free as long as K and Q agree, so a
+// lane loads 16 consecutive bytes of a token; bytes of two tokens are interleaved for V. The next K is asked for when this one has been
+// converted, and V alike, so a warp has its 8 KB in flight all the time.
 #include <climits>
 
-#include "kv_cache.cuh"
+#include "attention_work.cuh"
 #include "launch.cuh"
 
 namespace macko {
 namespace {
 
+constexpr int kWarps = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+
 struct AttentionArgs {
     CacheView cache;
     RowsView rows;
+    WorkShape work;
     const uint16_t *q;
     uint16_t *out;
+    SplitUnit *split;        // [ctas], or null: one unit per CTA, nothing is split
+    float *partial;          // [ctas][2][unit rows][head_dim + 2]
     long long q_row_stride, q_head_stride;
-    int heads;
-    float scale;
+    int heads, unit_rows;
+    float scale;             // times log2 e
 };
 
-// One warp per row and head: lane l holds dimensions l * D / 32 ..., tokens one after another with a running maximum.
-template <bool BF16, bool E4M3, int D>
-__global__ void __launch_bounds__(128)
-attention_kernel(const AttentionArgs a)
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    constexpr int V = D / 32;   // dimensions of a lane: 2, 4 or 8
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// BYTES consecutive codes.
+template <int BYTES> struct Codes { uint32_t w[BYTES / 4]; };
+
+template <int BYTES>
+__device__ __forceinline__ Codes<BYTES> load_codes(const uint8_t *p, bool there)
+{
+    Codes<BYTES> c;
+    if (BYTES == 8) {
+        uint2 v = make_uint2(0u, 0u);
+        if (there) v = __ldcg(reinterpret_cast<const uint2 *>(p));
+        c.w[0] = v.x;
+        c.w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (there) v = __ldcg(reinterpret_cast<const uint4 *>(p) + i);
+            c.w[4 * i] = v.x;
+            c.w[4 * i + 1] = v.y;
+            c.w[4 * i + 2] = v.z;
+            c.w[4 * i + 3] = v.w;
+        }
+    }
+    return c;
+}
+
+// Row ρ of a unit is row ρ / heads of its rows and head ρ % heads of its heads.
+struct UnitRows {
+    int first_row, queries, heads, head;   // first row of the call, rows, heads, first head
+    int begin;                             // position of the first row
+    __device__ __forceinline__ int rows() const { return queries * heads; }
+};
+
+__device__ __forceinline__ UnitRows unit_rows(const AttentionArgs &a, const SequenceWork &s, const Piece &p)
+{
+    UnitRows u;
+    const WorkShape &w = a.work;
+    u.first_row = s.rows.first + p.block * w.queries;
+    u.queries = min(w.queries, s.rows.count - p.block * w.queries);
+    u.heads = min(w.heads, w.group - p.part * w.heads);
+    u.head = p.kv_head * w.group + p.part * w.heads;
+    u.begin = s.rows.begin() + p.block * w.queries;
+    return u;
+}
+
+template <bool BF16, bool E4M3, int D, int RB>
+__global__ void __launch_bounds__(kWarps * 32, RB == 8 && D <= 128 ? 3 : 2)
+few_rows_kernel(const AttentionArgs a)
+{
+    constexpr int NB = RB / 8;              // blocks of 8 rows
+    constexpr int MT = D == 256 ? 1 : 2;    // blocks of 16 tokens that a warp takes at a time
+    constexpr int kTile = kWarps * 16 * MT;
+    constexpr int KC = D / 64;              // 16-byte chunks of a key that a lane holds
+    constexpr int VB = D / 8;               // bytes of a value that a lane holds
+    constexpr int DT = D / 16;              // blocks of 16 dimensions
+    __shared__ long long found[40];
+    extern __shared__ __align__(16) float merge[];   // [warps][RB][D], then maxima and sums [warps][RB]
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const RowsView &r = a.rows;
     const CacheView &c = a.cache;
-    const int lane = threadIdx.x & 31;
-    const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (id >= (long long)r.rows * a.heads) return;
-    const int row = (int)(id / a.heads), head = (int)(id % a.heads), kv_head = head / (a.heads / c.kv_heads);
-    int seq = row;
-    if (r.start != nullptr) {
-        seq = 0;
-        for (int i = 1 + lane; i <= r.sequences; i += 32) seq += __ldg(r.start + i) <= row;
-        seq = __reduce_add_sync(0xffffffffu, seq);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int page_mask = (1 << c.page_log2) - 1;
+
+    WorkWalk walk;
+    Piece piece;
+    bool more;
+    if (a.split != nullptr) {
+        if (tid == 0) a.split[blockIdx.x].pieces = 0;
+        walk.start(a.work, r, blockIdx.x, found);
+        more = walk.next(a.work, r, piece);
+    } else {
+        // one unit per CTA: sequences of one row each
+        const int per_sequence = a.work.kv_heads * a.work.parts, of = blockIdx.x % per_sequence;
+        walk.at = walk.end = 0;
+        walk.s.rows = sequence_at(r, blockIdx.x / per_sequence);
+        const int seen = min(max(walk.s.rows.length, 0), r.capacity);
+        piece = Piece{(int)(blockIdx.x / per_sequence), 0, of / a.work.parts, of % a.work.parts, 0, (seen + kTile - 1) / kTile, true, true, 1};
+        more = true;
     }
-    int seen = 0;
-    if (seq < r.sequences) {
-        const Sequence s = sequence_at(r, seq);
-        if (row >= s.first && row < s.first + s.count) seen = max(0, min(s.begin() + row - s.first + 1, r.capacity));
-    }
-    float q[V], acc[V];
+    while (more) {
+        const UnitRows u = unit_rows(a, walk.s, piece);
+        const int n_rows = u.rows();
+
+        // q as the B operand: row g of every block of 8, dimensions 64 c + 16 t + 4 i + 0..3 for step 4 c + i
+        uint32_t q[NB][D / 16][2];
+        float factor[NB][2];     // scale of rows 2t and 2t + 1
+        int limit[NB][2];        // tokens that they see
 #pragma unroll
-    for (int j = 0; j < V; j += 2) {
-        const float2 t = unpack2<BF16>(*reinterpret_cast<const uint32_t *>(a.q + row * a.q_row_stride + head * a.q_head_stride + lane * V + j));
-        q[j] = t.x * a.scale;
-        q[j + 1] = t.y * a.scale;
-        acc[j] = acc[j + 1] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int t = 0; t < seen; ++t) {
-        const int page = page_at(c, r, seq, t);
-        if (page < 0) continue;
-        const long long at = (((long long)kv_head << c.page_log2) + (t & ((1 << c.page_log2) - 1))) * D + lane * V;
-        const uint8_t *kp = c.k + page * c.k_stride + at, *vp = c.v + page * c.v_stride + at;
-        const float ks = c.k_scale[page * c.k_scale_stride + kv_head], vs = value_scale(c.v_scale[page * c.v_scale_stride + kv_head]);
-        float s = 0.f, v[V];
+        for (int nb = 0; nb < NB; ++nb) {
+            const int row = nb * 8 + g;
+            const int query = row / u.heads, head = u.head + row % u.heads;
+            const bool there = row < n_rows;
+            const uint16_t *qp = a.q + (long long)(u.first_row + query) * a.q_row_stride + (long long)head * a.q_head_stride + 16 * t;
 #pragma unroll
-        for (int j = 0; j < V; j += 2) {
-            uint32_t lo, hi;
-            codes_to_half<E4M3>(*reinterpret_cast<const uint16_t *>(kp + j), lo, hi);
-            const float2 k2 = unpack2<false>(lo);
-            s += q[j] * k2.x + q[j + 1] * k2.y;
-            codes_to_half<E4M3>(*reinterpret_cast<const uint16_t *>(vp + j), lo, hi);
-            const float2 v2 = unpack2<false>(lo);
-            v[j] = v2.x * vs;
-            v[j + 1] = v2.y * vs;
+            for (int ch = 0; ch < KC; ++ch) {
+                uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+                if (there) {
+                    lo = __ldcg(reinterpret_cast<const uint4 *>(qp + 64 * ch));
+                    hi = __ldcg(reinterpret_cast<const uint4 *>(qp + 64 * ch) + 1);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    q[nb][4 * ch + j / 2][j & 1] = (&lo.x)[j];
+                    q[nb][4 * ch + 2 + j / 2][j & 1] = (&hi.x)[j];
+                }
+            }
+            float own = 1.f;
+            if (BF16) {
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const float2 f = unpack2<true>((&q[nb][0][0])[i]);
+                    most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                // the largest to 2^14 .. 2^15; the exponent stays inside what fp32 can give back
+                const int e = most > 0.f && most < INFINITY ? min(max((int)(__float_as_uint(most) >> 23) - 127 - 14, -112), 113) : 0;
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                own = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const float2 f = unpack2<true>((&q[nb][0][0])[i]);
+                    (&q[nb][0][0])[i] = pack2<false>(f.x * down, f.y * down);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                factor[nb][i] = __shfl_sync(0xffffffffu, own, 4 * (2 * t + i)) * a.scale;
+                const int other = nb * 8 + 2 * t + i;
+                limit[nb][i] = other < n_rows ? min(u.begin + other / u.heads + 1, r.capacity) : 0;
+            }
         }
+        const int all_see = min(u.begin + 1, r.capacity);                       // tokens before this are seen by every row
+        const int end = max(0, min(u.begin + u.queries, r.capacity));           // and none from here on by any
+
+        float m[NB][2], l[NB][2], o[DT][NB][4];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s *= ks;
-        const float big = fmaxf(m, s), keep = m == -INFINITY ? 0.f : __expf(m - big), p = __expf(s - big);
-        m = big;
-        l = l * keep + p;
+        for (int nb = 0; nb < NB; ++nb) {
+            m[nb][0] = m[nb][1] = -INFINITY;
+            l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] = acc[j] * keep + p * v[j];
+            for (int d = 0; d < DT; ++d) o[d][nb][0] = o[d][nb][1] = o[d][nb][2] = o[d][nb][3] = 0.f;
+        }
+
+        const int stop = min(end, (piece.first_tile + piece.tiles) * kTile);
+        const int first = piece.first_tile * kTile + warp * 16 * MT;
+        const long long head_at = ((long long)piece.kv_head << c.page_log2) * D;
+        int page_of_lane = -1;
+        float ks_of_lane = 0.f, vs_of_lane = 1.f;
+        Codes<16> kc[MT][2][KC];
+        Codes<VB> vc[MT][4];
+        // pages and scales of the warp's next 32 blocks of 16 tokens, one per lane
+        auto fetch_pages = [&](int from) {
+            const int token = from + (lane / MT) * kTile + (lane % MT) * 16;
+            page_of_lane = token < end ? page_at(c, r, piece.sequence, token) : -1;
+            ks_of_lane = 0.f;
+            vs_of_lane = 1.f;
+            if (page_of_lane >= 0) {
+                ks_of_lane = __ldcg(c.k_scale + page_of_lane * c.k_scale_stride + piece.kv_head);
+                vs_of_lane = value_scale(__ldcg(c.v_scale + page_of_lane * c.v_scale_stride + piece.kv_head));
+            }
+        };
+        auto load_k = [&](int token, int index, int mt) {
+            const int page = __shfl_sync(0xffffffffu, page_of_lane, index * MT + mt);
+            const uint8_t *base = c.k + page * c.k_stride + head_at + (long long)((token + mt * 16) & page_mask) * D + 16 * t;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int ch = 0; ch < KC; ++ch)
+                    kc[mt][h][ch] = load_codes<16>(base + (g + 8 * h) * D + 64 * ch, page >= 0 && token + mt * 16 + g + 8 * h < end);
+        };
+        auto load_v = [&](int token, int index, int mt) {
+            const int page = __shfl_sync(0xffffffffu, page_of_lane, index * MT + mt);
+            const uint8_t *base = c.v + page * c.v_stride + head_at + (long long)((token + mt * 16) & page_mask) * D + VB * g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 2 * t + (i & 1) + 8 * (i >> 1);
+                vc[mt][i] = load_codes<VB>(base + row * D, page >= 0 && token + mt * 16 + row < end);
+            }
+        };
+        constexpr int kPerFetch = 32 / MT;
+        int index = 0;
+        if (first < stop) {
+            fetch_pages(first);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) load_k(first, 0, mt);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) load_v(first, 0, mt);
+        }
+        for (int token = first; token < stop; token += kTile) {
+            float x[MT][NB][4], inverse[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) x[mt][nb][0] = x[mt][nb][1] = x[mt][nb][2] = x[mt][nb][3] = 0.f;
+#pragma unroll
+                for (int ch = 0; ch < KC; ++ch)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t a0, a1, a2, a3;
+                        codes_to_half<E4M3>(kc[mt][0][ch].w[i], a0, a2);
+                        codes_to_half<E4M3>(kc[mt][1][ch].w[i], a1, a3);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) mma(x[mt][nb], a0, a1, a2, a3, q[nb][4 * ch + i][0], q[nb][4 * ch + i][1]);
+                    }
+            }
+            // what the softmax needs of this slice's pages, before the next ones may take their place
+            float k_scale[MT], shift[MT];
+            bool there[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float vs = __shfl_sync(0xffffffffu, vs_of_lane, index * MT + mt);
+                k_scale[mt] = __shfl_sync(0xffffffffu, ks_of_lane, index * MT + mt);
+                there[mt] = __shfl_sync(0xffffffffu, page_of_lane, index * MT + mt) >= 0;
+                shift[mt] = __log2f(vs);
+                inverse[mt] = 1.f / vs;
+            }
+            const int next = token + kTile;
+            const bool go_on = next < stop;
+            if (++index == kPerFetch && go_on) {
+                index = 0;
+                fetch_pages(next);
+            }
+            if (go_on) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) load_k(next, index, mt);
+            }
+
+            float top[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) top[nb][0] = top[nb][1] = -INFINITY;
+            const bool whole = token + 16 * MT <= all_see;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float &v = x[mt][nb][i];
+                        v = v * (k_scale[mt] * factor[nb][i & 1]) + shift[mt];
+                        if (!there[mt] || (!whole && token + mt * 16 + g + 8 * (i >> 1) >= limit[nb][i & 1])) v = -INFINITY;
+                        top[nb][i & 1] = fmaxf(top[nb][i & 1], v);
+                    }
+            }
+            bool grown = false;
+            float keep[NB][2], base[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float &v = top[nb][i];
+#pragma unroll
+                    for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
+                    v = fmaxf(v, m[nb][i]);
+                    base[nb][i] = v == -INFINITY ? 0.f : v;
+                    keep[nb][i] = exp2_fast(m[nb][i] - base[nb][i]);
+                    grown |= v != m[nb][i];
+                    m[nb][i] = v;
+                }
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    l[nb][0] *= keep[nb][0];
+                    l[nb][1] *= keep[nb][1];
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[d][nb][i] *= keep[nb][i & 1];
+                }
+            }
+            uint32_t p[MT][NB][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[mt][nb][i] = exp2_fast(x[mt][nb][i] - base[nb][i & 1]);
+                    // a masked block of tokens may have any scale: it adds nothing
+                    if (there[mt]) {
+                        l[nb][0] += (x[mt][nb][0] + x[mt][nb][2]) * inverse[mt];
+                        l[nb][1] += (x[mt][nb][1] + x[mt][nb][3]) * inverse[mt];
+                    }
+                    p[mt][nb][0] = transpose8x8(pack2<false>(x[mt][nb][0], x[mt][nb][1]));
+                    p[mt][nb][1] = transpose8x8(pack2<false>(x[mt][nb][2], x[mt][nb][3]));
+                }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int w = 0; w < VB / 4; ++w) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t select = half ? 0x7362u : 0x5140u;
+                        uint32_t a0, a1, a2, a3;
+                        codes_to_half<E4M3>(__byte_perm(vc[mt][0].w[w], vc[mt][1].w[w], select), a0, a1);
+                        codes_to_half<E4M3>(__byte_perm(vc[mt][2].w[w], vc[mt][3].w[w], select), a2, a3);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) mma(o[2 * w + half][nb], a0, a1, a2, a3, p[mt][nb][0], p[mt][nb][1]);
+                    }
+                }
+            if (go_on) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) load_v(next, index, mt);
+            }
+        }
+
+        // the warps' results together: rows 2t, 2t + 1 of every block, dimensions g * D / 8 + 2 d + (0, 1)
+        float *maxima = merge + kWarps * RB * D, *sums = maxima + kWarps * RB;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float v = l[nb][i];
+#pragma unroll
+                for (int s = 4; s < 32; s <<= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+                const int row = nb * 8 + 2 * t + i;
+                if (g == 0) {
+                    maxima[warp * RB + row] = m[nb][i];
+                    sums[warp * RB + row] = v;
+                }
+                float2 *to = reinterpret_cast<float2 *>(merge + (warp * RB + row) * D + g * VB);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) to[d] = make_float2(o[d][nb][i], o[d][nb][2 + i]);
+            }
+        __syncthreads();
+        const bool alone = piece.begins && piece.ends;
+        float *partial = alone ? nullptr : a.partial + ((long long)blockIdx.x * 2 + (piece.begins ? 1 : 0)) * RB * (D + 2);
+        for (int i = tid; i < n_rows * (D / 4); i += kWarps * 32) {
+            const int row = i / (D / 4), d = 4 * (i % (D / 4));
+            float most = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) most = fmaxf(most, maxima[w * RB + row]);
+            const float base = most == -INFINITY ? 0.f : most;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = exp2_fast(maxima[w * RB + row] - base);
+                const float4 x = *reinterpret_cast<const float4 *>(merge + (w * RB + row) * D + d);
+                sum += f * sums[w * RB + row];
+                v.x += f * x.x;
+                v.y += f * x.y;
+                v.z += f * x.z;
+                v.w += f * x.w;
+            }
+            if (alone) {
+                const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+                const uint2 packed = make_uint2(pack2<BF16>(v.x * inverse, v.y * inverse), pack2<BF16>(v.z * inverse, v.w * inverse));
+                const long long to = ((long long)(u.first_row + row / u.heads) * a.heads + u.head + row % u.heads) * D + d;
+                *reinterpret_cast<uint2 *>(a.out + to) = packed;
+            } else {
+                *reinterpret_cast<float4 *>(partial + row * D + d) = v;
+                if (d == 0) {
+                    partial[RB * D + row] = most;
+                    partial[RB * D + RB + row] = sum;
+                }
+            }
+        }
+        if (!alone && piece.begins && tid == 0)
+            a.split[blockIdx.x] = SplitUnit{u.first_row, n_rows, u.head, piece.pieces, u.heads, {0, 0, 0}};
+        __syncthreads();
+        more = walk.next(a.work, r, piece);
     }
-    const float inverse = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int j = 0; j < V; j += 2)
-        *reinterpret_cast<uint32_t *>(a.out + id * D + lane * V + j) = pack2<BF16>(acc[j] * inverse, acc[j + 1] * inverse);
+
+    // rows of no sequence: those before the first and behind the last one's
+    if (r.start != nullptr) {
+        const int lo = r.sequences > 0 ? min(max(__ldcg(r.start), 0), r.rows) : r.rows;
+        const int hi = r.sequences > 0 ? min(max(__ldcg(r.start + r.sequences), lo), r.rows) : r.rows;
+        const long long per_row = (long long)a.heads * D / 8;
+        for (long long i = (long long)blockIdx.x * blockDim.x + tid; i < (lo + r.rows - hi) * per_row; i += (long long)gridDim.x * blockDim.x) {
+            const long long row = i / per_row, at = row < lo ? row : row - lo + hi;
+            reinterpret_cast<uint4 *>(a.out)[at * per_row + i % per_row] = make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
 }
 
-template <bool BF16, bool E4M3>
-int launch_attention(const AttentionArgs &a, cudaStream_t s)
+// Units that lie in several CTAs: one block per CTA with whose share such a unit begins, and gridDim.y blocks for its rows. A
+// row's pieces are spread over the block's warps that are left for it.
+template <bool BF16, int D>
+__global__ void __launch_bounds__(256)
+join_kernel(const AttentionArgs a)
 {
-    const dim3 grid((unsigned)(((long long)a.rows.rows * a.heads + 3) / 4));
-    switch (a.cache.head_dim) {
-    case 64: return launch_pdl("paged_attention", attention_kernel<BF16, E4M3, 64>, grid, dim3(128), 1, 0, s, a);
-    case 128: return launch_pdl("paged_attention", attention_kernel<BF16, E4M3, 128>, grid, dim3(128), 1, 0, s, a);
-    default: return launch_pdl("paged_attention", attention_kernel<BF16, E4M3, 256>, grid, dim3(128), 1, 0, s, a);
+    constexpr int V = D / 32;   // dimensions of a lane: 2, 4 or 8
+    __shared__ float parts[8][D + 2];
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 *at = reinterpret_cast<const int4 *>(a.split + blockIdx.x);
+    const int4 s = __ldcg(at);   // first row, rows, head, pieces
+    const int pieces = s.w;
+    if (pieces == 0) return;
+    const int unit_heads = __ldcg(at + 1).x;
+    const int rows_here = a.unit_rows / gridDim.y;                 // rows of this block: a power of two, or all of them
+    const int warps_of_row = rows_here >= 8 ? 1 : 8 / rows_here, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int stride = a.unit_rows * (D + 2);
+    for (int base = 0; base < rows_here; base += 8 / warps_of_row) {
+        const int row = blockIdx.y * rows_here + base + warp / warps_of_row, member = warp % warps_of_row;
+        float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = 0.f;
+        if (row < s.y) {
+            constexpr int U = 4;
+            for (int p0 = member; p0 < pieces; p0 += U * warps_of_row) {
+                float pm[U], pl[U], po[U][V];
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const int p = p0 + i * warps_of_row;
+                    pm[i] = -INFINITY;
+                    pl[i] = 0.f;
+                    if (p < pieces) {
+                        // the first piece is the second result of its CTA, the others are the first of theirs
+                        const float *from = a.partial + ((long long)(blockIdx.x + p) * 2 + (p == 0)) * stride;
+                        pm[i] = __ldcg(from + a.unit_rows * D + row);
+                        pl[i] = __ldcg(from + a.unit_rows * D + a.unit_rows + row);
+#pragma unroll
+                        for (int j = 0; j < V; j += 2) {
+                            const float2 x = __ldcg(reinterpret_cast<const float2 *>(from + row * D + lane * V + j));
+                            po[i][j] = x.x;
+                            po[i][j + 1] = x.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) po[i][j] = 0.f;
+                    }
+                }
+                float most = m;
+#pragma unroll
+                for (int i = 0; i < U; ++i) most = fmaxf(most, pm[i]);
+                const float base2 = most == -INFINITY ? 0.f : most, keep = exp2_fast(m - base2);
+                m = most;
+                l *= keep;
+#pragma unroll
+                for (int j = 0; j < V; ++j) o[j] *= keep;
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const float f = exp2_fast(pm[i] - base2);
+                    l += f * pl[i];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o[j] += f * po[i][j];
+                }
+            }
+        }
+        if (warps_of_row > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < V; ++j) parts[warp][lane * V + j] = o[j];
+            if (lane == 0) {
+                parts[warp][D] = m;
+                parts[warp][D + 1] = l;
+            }
+            __syncthreads();
+            if (member == 0) {
+                float most = m;
+                for (int w = 1; w < warps_of_row; ++w) most = fmaxf(most, parts[warp + w][D]);
+                const float base2 = most == -INFINITY ? 0.f : most, keep = exp2_fast(m - base2);
+                l *= keep;
+#pragma unroll
+                for (int j = 0; j < V; ++j) o[j] *= keep;
+                for (int w = 1; w < warps_of_row; ++w) {
+                    const float f = exp2_fast(parts[warp + w][D] - base2);
+                    l += f * parts[warp + w][D + 1];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o[j] += f * parts[warp + w][lane * V + j];
+                }
+            }
+        }
+        if (member == 0 && row < s.y) {
+            const float inverse = l == 0.f ? 0.f : 1.f / l;
+            uint16_t *to = a.out + ((long long)(s.x + row / unit_heads) * a.heads + s.z + row % unit_heads) * D + lane * V;
+#pragma unroll
+            for (int j = 0; j < V; j += 2) *reinterpret_cast<uint32_t *>(to + j) = pack2<BF16>(o[j] * inverse, o[j + 1] * inverse);
+        }
     }
 }
 
@@ -103,6 +539,78 @@ int check_sizes(const macko_kv_cache *cache, const macko_kv_rows *batch, int hea
         return fail(MACKO_ERR_INVALID_ARGUMENT, "paged_attention: %d heads for %d key heads", heads, cache->kv_heads);
     if (a->rows.rows > INT_MAX / heads) return fail(MACKO_ERR_SIZE_OVERFLOW, "paged_attention: %d rows of %d heads", a->rows.rows, heads);
     return MACKO_OK;
+}
+
+// Which launch runs, and what it keeps in the workspace: host arithmetic on sizes alone.
+struct Launch {
+    WorkShape work;
+    int unit_rows;      // 8 or 16
+    int ctas, smem;
+    bool split;
+    int join_rows;      // blocks per split unit
+    int64_t split_bytes, partial_bytes;
+};
+
+int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
+{
+    const int group = heads / a.cache.kv_heads, d = a.cache.head_dim;
+    const bool one_each = a.rows.start == nullptr;
+    // rows that a head of the cache meets in a sequence, as far as the host knows: on average
+    const int64_t mean = one_each ? group : ((int64_t)a.rows.rows * group + a.rows.sequences - 1) / (a.rows.sequences > 0 ? a.rows.sequences : 1);
+    const int rows = mean <= 8 ? 8 : 16;
+    l->unit_rows = rows;
+    l->work.heads = group < rows ? group : rows;
+    l->work.parts = (group + l->work.heads - 1) / l->work.heads;
+    l->work.queries = one_each ? 1 : rows / l->work.heads;
+    l->work.tile = kWarps * 16 * (d == 256 ? 1 : 2);
+    l->work.group = group;
+    l->work.kv_heads = a.cache.kv_heads;
+    l->work.least_share = 4;
+    l->smem = (kWarps * rows * d + 2 * kWarps * rows) * 4;
+    const int64_t units = (int64_t)a.rows.sequences * a.cache.kv_heads * l->work.parts;
+    l->split = !(one_each && a.rows.capacity <= 512);
+    l->ctas = l->split ? sm_count * (rows == 8 && d <= 128 ? 3 : 2) : 0;
+    if (!l->split) {
+        if (units > INT_MAX) return fail(MACKO_ERR_SIZE_OVERFLOW, "paged_attention: too many sequences and heads");
+        l->ctas = (int)units;
+    }
+    l->work.ctas = l->ctas;
+    l->join_rows = units < l->ctas / 4 ? rows : rows / 8;
+    l->split_bytes = l->split ? (int64_t)l->ctas * sizeof(SplitUnit) : 0;
+    l->partial_bytes = l->split ? (int64_t)l->ctas * 2 * rows * (d + 2) * 4 : 0;
+    return MACKO_OK;
+}
+
+template <bool BF16, bool E4M3, int D, int RB>
+int launch_few(const AttentionArgs &a, const Launch &l, cudaStream_t s)
+{
+    static bool raised[kMaxDevices];   // dynamic shared memory above 48 KB is allowed per kernel and device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && l.smem > 40 * 1024 && (dev >= kMaxDevices || !raised[dev])) {
+        e = cudaFuncSetAttribute(few_rows_kernel<BF16, E4M3, D, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, l.smem);
+        if (e == cudaSuccess && dev < kMaxDevices) raised[dev] = true;
+    }
+    if (e != cudaSuccess) return fail(MACKO_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
+    if (int st = launch_pdl("paged_attention", few_rows_kernel<BF16, E4M3, D, RB>, dim3(l.ctas), dim3(kWarps * 32), 1, l.smem, s, a)) return st;
+    if (!l.split) return MACKO_OK;
+    return launch_pdl("paged_attention", join_kernel<BF16, D>, dim3(l.ctas, l.join_rows), dim3(256), 1, 0, s, a);
+}
+
+template <bool BF16, bool E4M3, int D>
+int launch_rows(const AttentionArgs &a, const Launch &l, cudaStream_t s)
+{
+    return l.unit_rows == 8 ? launch_few<BF16, E4M3, D, 8>(a, l, s) : launch_few<BF16, E4M3, D, 16>(a, l, s);
+}
+
+template <bool BF16, bool E4M3>
+int launch_attention(const AttentionArgs &a, const Launch &l, cudaStream_t s)
+{
+    switch (a.cache.head_dim) {
+    case 64: return launch_rows<BF16, E4M3, 64>(a, l, s);
+    case 128: return launch_rows<BF16, E4M3, 128>(a, l, s);
+    default: return launch_rows<BF16, E4M3, 256>(a, l, s);
+    }
 }
 
 }  // namespace
@@ -121,8 +629,12 @@ int64_t macko_cache_attention_workspace_bytes(int64_t sequences, int64_t rows, i
     const macko_kv_rows batch = {reinterpret_cast<const int32_t *>(16), reinterpret_cast<const int32_t *>(16),
                                  one_row_each ? nullptr : reinterpret_cast<const int32_t *>(16), table_width, table_width, sequences, rows};
     AttentionArgs a = {};
+    const DeviceInfo *dev = nullptr;
+    Launch l;
     if (check_sizes(&cache, &batch, heads, &a)) return -1;
-    return 0;
+    if (rows == 0) return 0;
+    if (current_device_info(&dev) || plan_launch(a, heads, dev->sm_count, &l)) return -1;
+    return l.split_bytes + l.partial_bytes;
 }
 
 int macko_cache_attention(const macko_kv_cache *cache, const macko_kv_rows *batch, const void *q, int64_t q_row_stride,
@@ -134,18 +646,29 @@ int macko_cache_attention(const macko_kv_cache *cache, const macko_kv_rows *batc
     if (type != MACKO_FP16 && type != MACKO_BF16) return fail(MACKO_ERR_INVALID_ARGUMENT, "paged_attention: unknown type %d", type);
     if (a.rows.rows == 0) return MACKO_OK;
     if (!q || !out) return fail(MACKO_ERR_INVALID_ARGUMENT, "paged_attention: null pointer");
-    if (!aligned(q, 16) || !aligned(out, 16) || q_row_stride % 8 || q_head_stride % 8)
-        return fail(MACKO_ERR_MISALIGNED, "paged_attention: rows and heads of q and out must be 16-byte aligned");
+    if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16) || q_row_stride % 8 || q_head_stride % 8)
+        return fail(MACKO_ERR_MISALIGNED, "paged_attention: rows and heads of q, out and the workspace must be 16-byte aligned");
+    const DeviceInfo *dev = nullptr;
+    if (int st = current_device_info(&dev)) return st;
+    Launch l;
+    if (int st = plan_launch(a, heads, dev->sm_count, &l)) return st;
+    if (workspace_bytes < l.split_bytes + l.partial_bytes || (!workspace && l.split))
+        return fail(MACKO_ERR_WORKSPACE, "paged_attention: %lld bytes of workspace, %lld needed", (long long)workspace_bytes,
+                    (long long)(l.split_bytes + l.partial_bytes));
+    a.work = l.work;
     a.q = static_cast<const uint16_t *>(q);
     a.out = static_cast<uint16_t *>(out);
+    a.split = l.split ? static_cast<SplitUnit *>(workspace) : nullptr;
+    a.partial = l.split ? reinterpret_cast<float *>(static_cast<char *>(workspace) + l.split_bytes) : nullptr;
     a.q_row_stride = q_row_stride;
     a.q_head_stride = q_head_stride;
     a.heads = heads;
-    a.scale = scale;
+    a.unit_rows = l.unit_rows;
+    a.scale = scale * kLog2e;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e4m3 = cache->code == MACKO_KV_E4M3;
-    if (type == MACKO_BF16) return e4m3 ? launch_attention<true, true>(a, s) : launch_attention<true, false>(a, s);
-    return e4m3 ? launch_attention<false, true>(a, s) : launch_attention<false, false>(a, s);
+    if (type == MACKO_BF16) return e4m3 ? launch_attention<true, true>(a, l, s) : launch_attention<true, false>(a, l, s);
+    return e4m3 ? launch_attention<false, true>(a, l, s) : launch_attention<false, false>(a, l, s);
 }
 
 }  // extern "C"
