@@ -14,7 +14,7 @@
 // converted, and V alike, so a warp has its 8 KB in flight all the time.
 #include <climits>
 
-#include "attention_work.cuh"
+#include "attention_args.cuh"
 #include "launch.cuh"
 
 namespace macko {
@@ -22,19 +22,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-
-struct AttentionArgs {
-    CacheView cache;
-    RowsView rows;
-    WorkShape work;
-    const uint16_t *q;
-    uint16_t *out;
-    SplitUnit *split;        // [ctas], or null: one unit per CTA, nothing is split
-    float *partial;          // [ctas][2][unit rows][head_dim + 2]
-    long long q_row_stride, q_head_stride;
-    int heads, unit_rows;
-    float scale;             // times log2 e
-};
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
@@ -47,13 +34,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
 {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-
-__device__ __forceinline__ float exp2_fast(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -81,25 +61,6 @@ __device__ __forceinline__ Codes<BYTES> load_codes(const uint8_t *p, bool there)
         }
     }
     return c;
-}
-
-// Row ρ of a unit is row ρ / heads of its rows and head ρ % heads of its heads.
-struct UnitRows {
-    int first_row, queries, heads, head;   // first row of the call, rows, heads, first head
-    int begin;                             // position of the first row
-    __device__ __forceinline__ int rows() const { return queries * heads; }
-};
-
-__device__ __forceinline__ UnitRows unit_rows(const AttentionArgs &a, const SequenceWork &s, const Piece &p)
-{
-    UnitRows u;
-    const WorkShape &w = a.work;
-    u.first_row = s.rows.first + p.block * w.queries;
-    u.queries = min(w.queries, s.rows.count - p.block * w.queries);
-    u.heads = min(w.heads, w.group - p.part * w.heads);
-    u.head = p.kv_head * w.group + p.part * w.heads;
-    u.begin = s.rows.begin() + p.block * w.queries;
-    return u;
 }
 
 template <bool BF16, bool E4M3, int D, int RB>
@@ -174,10 +135,8 @@ few_rows_kernel(const AttentionArgs a)
                 }
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                // the largest to 2^14 .. 2^15; the exponent stays inside what fp32 can give back
-                const int e = most > 0.f && most < INFINITY ? min(max((int)(__float_as_uint(most) >> 23) - 127 - 14, -112), 113) : 0;
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                own = __uint_as_float((uint32_t)(127 + e) << 23);
+                float down;
+                row_power(most, down, own);
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
                     const float2 f = unpack2<true>((&q[nb][0][0])[i]);
@@ -336,10 +295,11 @@ few_rows_kernel(const AttentionArgs a)
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[mt][nb][i] = exp2_fast(x[mt][nb][i] - base[nb][i & 1]);
-                    // a masked block of tokens may have any scale: it adds nothing
-                    if (there[mt]) {
-                        l[nb][0] += (x[mt][nb][0] + x[mt][nb][2]) * inverse[mt];
-                        l[nb][1] += (x[mt][nb][1] + x[mt][nb][3]) * inverse[mt];
+                    // tokens that a row does not see may have any scale: they add nothing
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float sum = x[mt][nb][i] + x[mt][nb][2 + i];
+                        l[nb][i] += sum == 0.f ? 0.f : sum * inverse[mt];
                     }
                     p[mt][nb][0] = transpose8x8(pack2<false>(x[mt][nb][0], x[mt][nb][1]));
                     p[mt][nb][1] = transpose8x8(pack2<false>(x[mt][nb][2], x[mt][nb][3]));
@@ -421,16 +381,7 @@ few_rows_kernel(const AttentionArgs a)
         more = walk.next(a.work, r, piece);
     }
 
-    // rows of no sequence: those before the first and behind the last one's
-    if (r.start != nullptr) {
-        const int lo = r.sequences > 0 ? min(max(__ldcg(r.start), 0), r.rows) : r.rows;
-        const int hi = r.sequences > 0 ? min(max(__ldcg(r.start + r.sequences), lo), r.rows) : r.rows;
-        const long long per_row = (long long)a.heads * D / 8;
-        for (long long i = (long long)blockIdx.x * blockDim.x + tid; i < (lo + r.rows - hi) * per_row; i += (long long)gridDim.x * blockDim.x) {
-            const long long row = i / per_row, at = row < lo ? row : row - lo + hi;
-            reinterpret_cast<uint4 *>(a.out)[at * per_row + i % per_row] = make_uint4(0u, 0u, 0u, 0u);
-        }
-    }
+    clear_other_rows(a);
 }
 
 // Units that lie in several CTAs: one block per CTA with whose share such a unit begins, and gridDim.y blocks for its rows. A
@@ -544,7 +495,7 @@ int check_sizes(const macko_kv_cache *cache, const macko_kv_rows *batch, int hea
 // Which launch runs, and what it keeps in the workspace: host arithmetic on sizes alone.
 struct Launch {
     WorkShape work;
-    int unit_rows;      // 8 or 16
+    int unit_rows;      // 8 or 16, or kPromptRows: the kernel for many rows
     int ctas, smem;
     bool split;
     int join_rows;      // blocks per split unit
@@ -557,28 +508,35 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     const bool one_each = a.rows.start == nullptr;
     // rows that a head of the cache meets in a sequence, as far as the host knows: on average
     const int64_t mean = one_each ? group : ((int64_t)a.rows.rows * group + a.rows.sequences - 1) / (a.rows.sequences > 0 ? a.rows.sequences : 1);
-    const int rows = mean <= 8 ? 8 : 16;
+    const bool prompt = !one_each && mean > 16 && d <= 128;
+    const int rows = prompt ? kPromptRows : mean <= 8 ? 8 : 16;
     l->unit_rows = rows;
     l->work.heads = group < rows ? group : rows;
     l->work.parts = (group + l->work.heads - 1) / l->work.heads;
     l->work.queries = one_each ? 1 : rows / l->work.heads;
-    l->work.tile = kWarps * 16 * (d == 256 ? 1 : 2);
+    l->work.tile = prompt ? kPromptTile : kWarps * 16 * (d == 256 ? 1 : 2);
     l->work.group = group;
     l->work.kv_heads = a.cache.kv_heads;
     l->work.least_share = 4;
     l->smem = (kWarps * rows * d + 2 * kWarps * rows) * 4;
     const int64_t units = (int64_t)a.rows.sequences * a.cache.kv_heads * l->work.parts;
     l->split = !(one_each && a.rows.capacity <= 512);
-    l->ctas = l->split ? sm_count * (rows == 8 && d <= 128 ? 3 : 2) : 0;
+    l->ctas = l->split ? sm_count * (prompt ? 1 : rows == 8 && d <= 128 ? 3 : 2) : 0;
     if (!l->split) {
         if (units > INT_MAX) return fail(MACKO_ERR_SIZE_OVERFLOW, "paged_attention: too many sequences and heads");
         l->ctas = (int)units;
     }
     l->work.ctas = l->ctas;
-    l->join_rows = units < l->ctas / 4 ? rows : rows / 8;
+    l->join_rows = !prompt && units < l->ctas / 4 ? rows : rows / 8;
     l->split_bytes = l->split ? (int64_t)l->ctas * sizeof(SplitUnit) : 0;
     l->partial_bytes = l->split ? (int64_t)l->ctas * 2 * rows * (d + 2) * 4 : 0;
     return MACKO_OK;
+}
+
+template <bool BF16, int D>
+int launch_join(const AttentionArgs &a, const Launch &l, cudaStream_t s)
+{
+    return launch_pdl("paged_attention", join_kernel<BF16, D>, dim3(l.ctas, l.join_rows), dim3(256), 1, 0, s, a);
 }
 
 template <bool BF16, bool E4M3, int D, int RB>
@@ -593,13 +551,18 @@ int launch_few(const AttentionArgs &a, const Launch &l, cudaStream_t s)
     }
     if (e != cudaSuccess) return fail(MACKO_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
     if (int st = launch_pdl("paged_attention", few_rows_kernel<BF16, E4M3, D, RB>, dim3(l.ctas), dim3(kWarps * 32), 1, l.smem, s, a)) return st;
-    if (!l.split) return MACKO_OK;
-    return launch_pdl("paged_attention", join_kernel<BF16, D>, dim3(l.ctas, l.join_rows), dim3(256), 1, 0, s, a);
+    return l.split ? launch_join<BF16, D>(a, l, s) : MACKO_OK;
 }
 
 template <bool BF16, bool E4M3, int D>
 int launch_rows(const AttentionArgs &a, const Launch &l, cudaStream_t s)
 {
+    if constexpr (D <= 128) {
+        if (l.unit_rows == kPromptRows) {
+            if (int st = launch_prompt_attention(a, BF16, E4M3, s)) return st;
+            return launch_join<BF16, D>(a, l, s);
+        }
+    }
     return l.unit_rows == 8 ? launch_few<BF16, E4M3, D, 8>(a, l, s) : launch_few<BF16, E4M3, D, 16>(a, l, s);
 }
 

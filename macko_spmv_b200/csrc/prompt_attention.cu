@@ -1,0 +1,543 @@
+// Attention over the paged 8-bit cache, for many rows per sequence and head of the cache: prompts and pieces of prompts.
+//
+//   x(t) = scale * (q . k_t) * k_scale(page) * log2 e + log2 v_scale(page)        k_t, v_t: codes
+//   out  = sum 2^(x(t) - m) v_t  /  sum 2^(x(t) - m) / v_scale(page)
+//
+// as in the kernel for a few rows. One CTA per SM walks its share of the call's tiles (attention_work.cuh): units of 256 packed rows (rows
+// of the call times heads of a group) in two halves of 128, tiles of 128 tokens. Four groups of warps:
+//
+//   0, 1   softmax of one half each, one row per thread: S from tensor memory, maximum, 2^x, P as fp16 over S in tensor memory; the
+//          accumulator is rescaled there when the maximum has grown by more than 8 (so weights are at most 2^8 and none is lost)
+//   2      the cache: codes from global memory to fp16 (exact) in shared memory, in the 128-byte swizzle, two stages each of K and V,
+//          and the scales of the tile's pages
+//   3      one thread that issues tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it lies
+//          (token by token: its "N" dimension is the contiguous one)
+//
+// While one half's softmax runs the tensor core works for the other. A tile takes 2 x (512 + 512) cycles of tensor core and 2 x 1024 of the
+// exponential unit; the conversion of 32 K codes adds some 400 issue slots per scheduler.
+//
+// Every wait has a limit: if one runs out, no further wait waits, and what the CTA writes from then on is NaN.
+#include "attention_args.cuh"
+#include "launch.cuh"
+
+namespace macko {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kTile = kPromptTile;
+constexpr int kGroups = kTile / 16;     // blocks of 16 tokens: each lies on one page
+constexpr int kConstSlots = 4;
+constexpr int kWalkers = 13;            // warps that walk the CTA's pieces, each for itself
+
+// Shared memory, from a 1024-byte boundary: Q of both halves, K and V stages, each as [64 dimensions][128 rows][128 bytes].
+template <int D> struct Layout {
+    static constexpr int kOperand = 128 * D * 2;
+    static constexpr int kQ = 0, kK = 2 * kOperand, kV = 4 * kOperand, kEnd = 6 * kOperand;
+    static constexpr int kBytes = kEnd + 1024;
+};
+
+enum Barrier { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPFull = 12, kODone = 14, kBarriers = 16 };
+
+__device__ __forceinline__ uint32_t smem_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void arrive(uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_address(bar)) : "memory");
+}
+
+// Waits for the phase with parity `parity`; false (and from then on for every wait of the CTA) where it does not come.
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *given_up)
+{
+    const uint32_t at = smem_address(bar);
+    for (int i = 0; i < 1 << 22; ++i) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(at), "r"(parity) : "memory");
+        if (done) return true;
+        if (*given_up) return false;
+    }
+    *given_up = 1;
+    return false;
+}
+
+// Shared memory operand in the 128-byte swizzle. `leading`, `stride`: bytes between blocks of 64 elements along the contiguous dimension
+// (where that is not the one summed over) and between groups of 8 rows.
+__device__ __forceinline__ uint64_t descriptor(uint32_t address, uint32_t leading, uint32_t stride)
+{
+    return (uint64_t)((address & 0x3ffffu) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+// fp16 operands, fp32 accumulator, M = 128; B with its N dimension contiguous if `n_major`.
+__device__ __forceinline__ constexpr uint32_t instruction(int n, bool n_major)
+{
+    return 1u << 4 | (n_major ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(128 >> 4) << 24;
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+
+__device__ __forceinline__ void commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_address(bar)) : "memory");
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+#define MACKO_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define MACKO_W8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+
+// 32 columns of tensor memory for the warp's 32 lanes, one lane per thread. Complete when it returns.
+__device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t *v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+                 "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : MACKO_R8(v, 0), MACKO_R8(v, 8), MACKO_R8(v, 16), MACKO_R8(v, 24) : "r"(address) : "memory");
+}
+
+__device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+                 "%24,%25,%26,%27,%28,%29,%30,%31};"
+                 ::MACKO_W8(v, 0), MACKO_W8(v, 8), MACKO_W8(v, 16), MACKO_W8(v, 24), "r"(address) : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Tiles of a unit that each half of its rows takes part in, cut to a piece: [first, end[h]); rows[h] is 0 for a half without rows.
+struct HalfTiles {
+    int first, end[2], rows[2], last;   // last: the later end
+};
+
+__device__ __forceinline__ HalfTiles half_tiles(const AttentionArgs &a, const UnitRows &u, const Piece &p)
+{
+    HalfTiles h;
+    h.first = p.first_tile;
+    const int n = u.rows();
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        h.rows[w] = min(max(n - 128 * w, 0), 128);
+        const int last_query = (128 * w + h.rows[w] - 1) / u.heads;
+        const int seen = h.rows[w] > 0 ? max(0, min(u.begin + last_query + 1, a.rows.capacity)) : 0;
+        h.end[w] = min((seen + kTile - 1) / kTile, p.first_tile + p.tiles);
+    }
+    h.last = max(h.end[0], h.end[1]);
+    return h;
+}
+
+// The warp's next piece. The walk itself stays in shared memory: its registers are wanted elsewhere.
+__device__ __forceinline__ bool next_piece(WorkWalk &shared, const AttentionArgs &a, Piece &p)
+{
+    WorkWalk walk = shared;
+    __syncwarp();
+    const bool more = walk.next(a.work, a.rows, p);
+    if ((threadIdx.x & 31) == 0) shared = walk;
+    __syncwarp();
+    return more;
+}
+
+template <bool BF16, bool E4M3, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+prompt_kernel(const AttentionArgs a)
+{
+    using L = Layout<D>;
+    constexpr uint32_t kBlockBytes = 128 * 128;
+    extern __shared__ uint8_t raw[];
+    __shared__ long long found[40];
+    __shared__ __align__(8) uint64_t bars[kBarriers];
+    __shared__ float4 scales[kConstSlots][kGroups];   // of 16 tokens: scale of the keys, log2 and inverse of the values'
+    __shared__ uint32_t tmem_base;
+    __shared__ WorkWalk walks[kWalkers];
+    __shared__ int given_up_word;
+    volatile int *given_up = &given_up_word;
+    uint8_t *smem = raw + ((1024u - (smem_address(raw) & 1023u)) & 1023u);
+    const RowsView &r = a.rows;
+    const CacheView &c = a.cache;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = tid >> 7;
+
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (tid == 0) {
+        given_up_word = 0;
+        const int counts[kBarriers] = {128, 128, 128, 128, 1, 1, 128, 128, 1, 1, 1, 1, 128, 128, 1, 1};
+        for (int i = 0; i < kBarriers; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_address(bars + i)), "r"(counts[i]));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_address(&tmem_base)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (tid == 0) a.split[blockIdx.x].pieces = 0;
+    {
+        WorkWalk walk;
+        walk.start(a.work, r, blockIdx.x, found);
+        if (lane == 0 && warp < kWalkers) walks[warp] = walk;
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    WorkWalk &walk = walks[warp < kWalkers ? warp : 0];
+    const uint32_t tmem = tmem_base;   // columns: S of half 0 and 1 (128 each), O of half 0 and 1 (D each)
+    Piece piece;
+
+    if (group < 2) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        const int half = group, local = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        const uint32_t s_at = tmem + lanes + half * 128, o_at = tmem + lanes + 256 + half * D;
+        uint32_t s_phase = 0, o_phase = 0;
+        int slot0 = 0;                      // tiles of the pieces before: where this piece's scales begin
+        while (next_piece(walk, a, piece)) {
+            const UnitRows u = unit_rows(a, walk.s, piece);
+            const HalfTiles h = half_tiles(a, u, piece);
+            if (h.rows[half] > 0) {
+                const int row = half * 128 + local, query = row / u.heads, head = u.head + row % u.heads;
+                const bool there = local < h.rows[half];
+                float factor = fabsf(a.scale);
+                if (h.first < h.end[half]) {
+                    // this half of Q, as fp16, with the sign of the scale
+                    const uint16_t *qp = a.q + (long long)(u.first_row + query) * a.q_row_stride + (long long)head * a.q_head_stride;
+                    uint32_t q[D / 2];
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) {
+                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                        if (there) v = __ldcg(reinterpret_cast<const uint4 *>(qp) + i);
+                        q[4 * i] = v.x;
+                        q[4 * i + 1] = v.y;
+                        q[4 * i + 2] = v.z;
+                        q[4 * i + 3] = v.w;
+                    }
+                    if (BF16) {
+                        float most = 0.f, down, up;
+#pragma unroll
+                        for (int i = 0; i < D / 2; ++i) {
+                            const float2 f = unpack2<true>(q[i]);
+                            most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+                        }
+                        row_power(most, down, up);
+                        factor *= up;
+#pragma unroll
+                        for (int i = 0; i < D / 2; ++i) {
+                            const float2 f = unpack2<true>(q[i]);
+                            q[i] = pack2<false>(f.x * down, f.y * down);
+                        }
+                    }
+                    if (a.scale < 0.f) {
+#pragma unroll
+                        for (int i = 0; i < D / 2; ++i) q[i] ^= 0x80008000u;
+                    }
+                    uint8_t *to = smem + L::kQ + half * L::kOperand + local * 128;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i)
+                        *reinterpret_cast<uint4 *>(to + (i >> 3) * kBlockBytes + (((i & 7) ^ (local & 7)) << 4)) =
+                            make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+                    fence_shared();
+                    arrive(bars + kQFull + half);
+                }
+                const int limit = there ? min(u.begin + query + 1, r.capacity) : 0;           // tokens that this row sees
+                const int all_see = min(u.begin + 128 * half / u.heads + 1, r.capacity);      // that every row of this half sees
+                float m = -INFINITY, l = 0.f;
+                for (int j = h.first; j < h.end[half]; ++j) {
+                    wait(bars + kSFull + half, s_phase, given_up);
+                    __syncwarp();
+                    s_phase ^= 1u;
+                    fence_after();
+                    float s[kTile];
+#pragma unroll
+                    for (int i = 0; i < kTile; i += 32) tmem_load32(s_at + i, reinterpret_cast<uint32_t *>(s + i));
+                    const float4 *of_tile = scales[(slot0 + j - h.first) % kConstSlots];
+                    const bool masked = (j + 1) * kTile > all_see;
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        const float4 k = of_tile[g];
+                        float *x = s + 16 * g;
+                        const float by = k.x * factor;
+                        if (masked) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                x[i] = j * kTile + 16 * g + i < limit ? fmaf(x[i], by, k.y) : -INFINITY;
+                                most = fmaxf(most, x[i]);
+                            }
+                        } else {
+                            float top = x[0];
+#pragma unroll
+                            for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+                            most = fmaxf(most, fmaf(top, by, k.y));
+                        }
+                    }
+                    const bool grown = most > m + 8.f || (m == -INFINITY && most > m);
+                    if (__any_sync(0xffffffffu, grown)) {
+                        const float keep = grown ? exp2_fast(m - most) : 1.f;
+                        if (grown) m = most;
+                        l *= keep;
+                        if (j > h.first) {
+                            wait(bars + kODone + half, o_phase, given_up);
+                            __syncwarp();
+                            fence_after();
+#pragma unroll 1
+                            for (int i = 0; i < D; i += 32) {
+                                uint32_t o[32];
+                                tmem_load32(o_at + i, o);
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                                tmem_store32(o_at + i, o);
+                            }
+                            tmem_store_wait();
+                        }
+                    }
+                    if (j > h.first) o_phase ^= 1u;
+                    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        uint32_t p[32];
+#pragma unroll
+                        for (int gg = 0; gg < kGroups / 2; ++gg) {
+                            const int g = part * (kGroups / 2) + gg;
+                            const float4 k = of_tile[g];
+                            float *x = s + 16 * g;
+                            const float by = masked ? 1.f : k.x * factor, plus = masked ? -base : k.y - base;
+                            float sum = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const float e0 = exp2_fast(fmaf(x[i], by, plus)), e1 = exp2_fast(fmaf(x[i + 1], by, plus));
+                                sum += e0 + e1;
+                                p[8 * gg + i / 2] = pack2<false>(e0, e1);
+                            }
+                            l += sum == 0.f ? 0.f : sum * k.z;   // tokens that a row does not see may have any scale
+                        }
+                        tmem_store32(s_at + 32 * part, p);
+                    }
+                    tmem_store_wait();
+                    fence_before();
+                    arrive(bars + kPFull + half);
+                }
+                // the result of this half, divided or as a piece
+                if (h.first < h.end[half]) {
+                    wait(bars + kODone + half, o_phase, given_up);
+                    __syncwarp();
+                    o_phase ^= 1u;
+                    fence_after();
+                }
+                const bool alone = piece.begins && piece.ends, empty = h.first >= h.end[half];
+                float *partial = a.partial + ((long long)blockIdx.x * 2 + (piece.begins ? 1 : 0)) * kPromptRows * (D + 2);
+                float by = alone ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+                if (*given_up) by = __uint_as_float(0x7fffffffu);
+#pragma unroll 1
+                for (int i = 0; i < D; i += 32) {
+                    uint32_t o[32];
+                    if (!empty) {
+                        tmem_load32(o_at + i, o);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = 0u;
+                    }
+                    if (there) {
+                        if (alone) {
+                            uint4 *to = reinterpret_cast<uint4 *>(a.out + ((long long)(u.first_row + query) * a.heads + head) * D + i);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                uint4 v;
+#pragma unroll
+                                for (int n = 0; n < 4; ++n)
+                                    (&v.x)[n] = pack2<BF16>(__uint_as_float(o[8 * k + 2 * n]) * by, __uint_as_float(o[8 * k + 2 * n + 1]) * by);
+                                to[k] = v;
+                            }
+                        } else {
+                            float4 *to = reinterpret_cast<float4 *>(partial + row * D + i);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                to[k] = make_float4(__uint_as_float(o[4 * k]) * by, __uint_as_float(o[4 * k + 1]) * by, __uint_as_float(o[4 * k + 2]) * by,
+                                                    __uint_as_float(o[4 * k + 3]) * by);
+                        }
+                    }
+                }
+                if (there && !alone) {
+                    partial[kPromptRows * D + row] = m;
+                    partial[kPromptRows * D + kPromptRows + row] = l;
+                }
+                if (!alone && piece.begins && row == 0)
+                    a.split[blockIdx.x] = SplitUnit{u.first_row, u.rows(), u.head, piece.pieces, u.heads, {0, 0, 0}};
+                fence_before();   // O is read before this half arrives for the next piece's P
+            }
+            slot0 += max(h.last - h.first, 0);
+        }
+    } else if (group == 2) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        constexpr int kChunks = D / 16;                  // 16-byte chunks of a token
+        constexpr int kItems = kTile * kChunks / 128;    // that a thread converts of K, and of V
+        const int local = tid & 127, chunk = local % kChunks, token = local / kChunks;   // item i: token + i * 128 / kChunks
+        int n = 0;                                       // tiles so far
+        while (next_piece(walk, a, piece)) {
+            const UnitRows u = unit_rows(a, walk.s, piece);
+            const HalfTiles h = half_tiles(a, u, piece);
+            const int end = max(0, min(u.begin + u.queries, r.capacity));   // no row sees anything from here on
+            const long long head_at = ((long long)piece.kv_head << c.page_log2) * D + 16 * chunk;
+            const int page_mask = (1 << c.page_log2) - 1;
+            // page of the tile's block of 16 tokens `lane`, in the first 8 lanes
+            auto pages_of = [&](int tile) {
+                const int t = tile * kTile + 16 * lane;
+                return lane < kGroups && t < end ? page_at(c, r, piece.sequence, t) : -1;
+            };
+            auto load = [&](const uint8_t *base, long long stride, int tile, int pages, uint4 (&x)[kItems]) {
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) {
+                    const int row = token + i * (128 / kChunks), at = tile * kTile + row;
+                    const int page = __shfl_sync(0xffffffffu, pages, row >> 4);
+                    x[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (page >= 0 && at < end) x[i] = __ldcg(reinterpret_cast<const uint4 *>(base + page * stride + head_at + (long long)(at & page_mask) * D));
+                }
+            };
+            auto store = [&](uint8_t *to, const uint4 (&x)[kItems]) {
+                // chunk: 16 dimensions, two 16-byte pieces of the row in block chunk / 4; odd blocks store the second one first,
+                // so that eight neighbouring threads fill all banks
+                const int flip = (chunk >> 2) & 1;
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) {
+                    const int row = token + i * (128 / kChunks);
+                    uint4 lo, hi;
+                    codes_to_half<E4M3>(x[i].x, lo.x, lo.y);
+                    codes_to_half<E4M3>(x[i].y, lo.z, lo.w);
+                    codes_to_half<E4M3>(x[i].z, hi.x, hi.y);
+                    codes_to_half<E4M3>(x[i].w, hi.z, hi.w);
+                    uint8_t *at = to + (chunk >> 2) * kBlockBytes + row * 128;
+                    const int first = 2 * (chunk & 3) + flip;
+                    *reinterpret_cast<uint4 *>(at + ((first ^ (row & 7)) << 4)) = flip ? hi : lo;
+                    *reinterpret_cast<uint4 *>(at + (((first ^ 1) ^ (row & 7)) << 4)) = flip ? lo : hi;
+                }
+            };
+            uint4 kx[kItems], vx[kItems];
+            int pages = -1, pages_next = -1;
+            if (h.first < h.last) {
+                pages = pages_of(h.first);
+                load(c.k, c.k_stride, h.first, pages, kx);
+            }
+            for (int j = h.first; j < h.last; ++j, ++n) {
+                const int stage = n & 1;
+                const uint32_t empty = ((n >> 1) & 1) ^ 1;
+                load(c.v, c.v_stride, j, pages, vx);
+                float4 of_lane = make_float4(0.f, -INFINITY, 0.f, 0.f);
+                if (warp == 8 && lane < kGroups && pages >= 0) {
+                    const float ks = __ldcg(c.k_scale + pages * c.k_scale_stride + piece.kv_head);
+                    const float vs = value_scale(__ldcg(c.v_scale + pages * c.v_scale_stride + piece.kv_head));
+                    of_lane = make_float4(ks, __log2f(vs), 1.f / vs, 0.f);
+                }
+                if (j + 1 < h.last) pages_next = pages_of(j + 1);
+                wait(bars + kKEmpty + stage, empty, given_up);
+                store(smem + L::kK + stage * L::kOperand, kx);
+                if (warp == 8 && lane < kGroups) scales[n % kConstSlots][lane] = of_lane;
+                fence_shared();
+                arrive(bars + kKFull + stage);
+                if (j + 1 < h.last) load(c.k, c.k_stride, j + 1, pages_next, kx);
+                wait(bars + kVEmpty + stage, empty, given_up);
+                store(smem + L::kV + stage * L::kOperand, vx);
+                fence_shared();
+                arrive(bars + kVFull + stage);
+                pages = pages_next;
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 12) {
+            int n = 0;
+            uint32_t q_phase = 0, p_phase = 0;    // one bit per half
+            while (next_piece(walk, a, piece)) {
+                const HalfTiles h = half_tiles(a, unit_rows(a, walk.s, piece), piece);
+                if (lane == 0) {
+                    auto last_half = [&](int j) { return j < h.end[1] ? 1 : 0; };
+                    auto scores = [&](int w, int j) {
+                        const int tile = n + j - h.first, stage = tile & 1;
+                        if (j == h.first) {
+                            wait(bars + kQFull + w, (q_phase >> w) & 1u, given_up);
+                            q_phase ^= 1u << w;
+                        }
+                        wait(bars + kKFull + stage, (tile >> 1) & 1, given_up);
+                        fence_after();
+                        const uint32_t qa = smem_address(smem + L::kQ + w * L::kOperand), ka = smem_address(smem + L::kK + stage * L::kOperand);
+#pragma unroll
+                        for (int d = 0; d < D / 16; ++d) {
+                            const uint32_t at = (d >> 2) * kBlockBytes + (d & 3) * 32;
+                            mma_ss(tmem + w * 128, descriptor(qa + at, 16, 1024), descriptor(ka + at, 16, 1024), instruction(kTile, false), d > 0);
+                        }
+                        commit(bars + kSFull + w);
+                        if (w == last_half(j)) commit(bars + kKEmpty + stage);
+                    };
+                    if (h.first < h.end[0]) scores(0, h.first);
+                    if (h.first < h.end[1]) scores(1, h.first);
+                    for (int j = h.first; j < h.last; ++j) {
+                        const int tile = n + j - h.first, stage = tile & 1;
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            if (j >= h.end[w]) continue;
+                            wait(bars + kPFull + w, (p_phase >> w) & 1u, given_up);
+                            p_phase ^= 1u << w;
+                            wait(bars + kVFull + stage, (tile >> 1) & 1, given_up);
+                            fence_after();
+                            const uint32_t va = smem_address(smem + L::kV + stage * L::kOperand);
+#pragma unroll
+                            for (int t = 0; t < kTile / 16; ++t)
+                                mma_ts(tmem + 256 + w * D, tmem + w * 128 + 8 * t, descriptor(va + t * 2048, kBlockBytes, 1024), instruction(D, true),
+                                       j > h.first || t > 0);
+                            commit(bars + kODone + w);
+                            if (w == last_half(j)) commit(bars + kVEmpty + stage);
+                            if (j + 1 < h.end[w]) scores(w, j + 1);
+                        }
+                    }
+                }
+                n += max(h.last - h.first, 0);
+                __syncwarp();
+            }
+            // all that was issued has arrived before shared and tensor memory are given back
+            if (lane == 0 && n > 0) {
+                int never = 0;
+                wait(bars + kVEmpty + ((n - 1) & 1), ((n - 1) >> 1) & 1, &never);
+            }
+            __syncwarp();
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    clear_other_rows(a);
+}
+
+template <bool BF16, bool E4M3, int D>
+int launch(const AttentionArgs &a, cudaStream_t stream)
+{
+    static bool raised[kMaxDevices];   // dynamic shared memory above 48 KB is allowed per kernel and device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= kMaxDevices || !raised[dev])) {
+        e = cudaFuncSetAttribute(prompt_kernel<BF16, E4M3, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::kBytes);
+        if (e == cudaSuccess && dev < kMaxDevices) raised[dev] = true;
+    }
+    if (e != cudaSuccess) return fail(MACKO_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
+    return launch_pdl("paged_attention", prompt_kernel<BF16, E4M3, D>, dim3(a.work.ctas), dim3(kThreads), 1, Layout<D>::kBytes, stream, a);
+}
+
+template <int D>
+int launch_types(const AttentionArgs &a, bool bf16, bool e4m3, cudaStream_t s)
+{
+    if (bf16) return e4m3 ? launch<true, true, D>(a, s) : launch<true, false, D>(a, s);
+    return e4m3 ? launch<false, true, D>(a, s) : launch<false, false, D>(a, s);
+}
+
+}  // namespace
+
+int launch_prompt_attention(const AttentionArgs &a, bool bf16, bool e4m3, cudaStream_t stream)
+{
+    return a.cache.head_dim == 64 ? launch_types<64>(a, bf16, e4m3, stream) : launch_types<128>(a, bf16, e4m3, stream);
+}
+
+}  // namespace macko
