@@ -4,13 +4,13 @@
 //   out  = sum 2^(x(t) - m) v_t  /  sum 2^(x(t) - m) / v_scale(page)
 //
 // as in the kernel for a few rows. One CTA per SM walks its share of the call's tiles (attention_work.cuh): units of 256 packed rows (rows
-// of the call times heads of a group) in two halves of 128, tiles of 128 tokens. Four groups of warps:
+// of the call times heads of a group) in two halves of 128, tiles of 128 tokens. Five groups of warps:
 //
 //   0, 1   softmax of one half each, one row per thread: S from tensor memory, maximum, 2^x, P as fp16 over S in tensor memory; the
 //          accumulator is rescaled there when the maximum has grown by more than 8 (so weights are at most 2^8 and none is lost)
-//   2      the cache: codes from global memory to fp16 (exact) in shared memory, in the 128-byte swizzle, two stages each of K and V,
-//          and the scales of the tile's pages
-//   3      one thread that issues tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it lies
+//   2, 3   the cache, keys and values: codes from global memory to fp16 (exact) in shared memory, in the 128-byte swizzle, two stages
+//          each, and the scales of the tile's pages
+//   4      one thread that issues tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it lies
 //          (token by token: its "N" dimension is the contiguous one)
 //
 // While one half's softmax runs the tensor core works for the other. A tile takes 2 x (512 + 512) cycles of tensor core and 2 x 1024 of the
@@ -23,11 +23,12 @@
 namespace macko {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr int kTile = kPromptTile;
 constexpr int kGroups = kTile / 16;     // blocks of 16 tokens: each lies on one page
 constexpr int kConstSlots = 4;
-constexpr int kWalkers = 13;            // warps that walk the CTA's pieces, each for itself
+constexpr float kLeastFactor = 1e-36f;  // a score times nothing is still minus infinity where it is masked
+constexpr int kWalkers = 17;            // warps that walk the CTA's pieces, each for itself
 
 // Shared memory, from a 1024-byte boundary: Q of both halves, K and V stages, each as [64 dimensions][128 rows][128 bytes].
 template <int D> struct Layout {
@@ -45,14 +46,15 @@ __device__ __forceinline__ void arrive(uint64_t *bar)
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_address(bar)) : "memory");
 }
 
-// Waits for the phase with parity `parity`; false (and from then on for every wait of the CTA) where it does not come.
+// Waits for the phase with parity `parity`; false (and from then on for every wait of the CTA) where it does not come. The thread
+// sleeps meanwhile, up to a millisecond at a time.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *given_up)
 {
     const uint32_t at = smem_address(bar);
-    for (int i = 0; i < 1 << 22; ++i) {
+    for (int i = 0; i < 4096; ++i) {
         uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done) : "r"(at), "r"(parity) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(at), "r"(parity), "r"(1000000u) : "memory");
         if (done) return true;
         if (*given_up) return false;
     }
@@ -105,6 +107,15 @@ __device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t *v)
                  : MACKO_R8(v, 0), MACKO_R8(v, 8), MACKO_R8(v, 16), MACKO_R8(v, 24) : "r"(address) : "memory");
 }
 
+__device__ __forceinline__ void tmem_load64(uint32_t address, uint32_t *v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+                 "%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,"
+                 "%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : MACKO_R8(v, 0), MACKO_R8(v, 8), MACKO_R8(v, 16), MACKO_R8(v, 24), MACKO_R8(v, 32), MACKO_R8(v, 40), MACKO_R8(v, 48), MACKO_R8(v, 56)
+                 : "r"(address) : "memory");
+}
+
 __device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t *v)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
@@ -112,7 +123,49 @@ __device__ __forceinline__ void tmem_store32(uint32_t address, const uint32_t *v
                  ::MACKO_W8(v, 0), MACKO_W8(v, 8), MACKO_W8(v, 16), MACKO_W8(v, 24), "r"(address) : "memory");
 }
 
+__device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::MACKO_W8(v, 0), MACKO_W8(v, 8), "r"(address) : "memory");
+}
+
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two fp32 values in one register pair.
+__device__ __forceinline__ uint64_t pair(float lo, float hi)
+{
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+
+__device__ __forceinline__ float2 unpair(uint64_t v)
+{
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 // Tiles of a unit that each half of its rows takes part in, cut to a piece: [first, end[h]); rows[h] is 0 for a half without rows.
 struct HalfTiles {
@@ -155,7 +208,9 @@ prompt_kernel(const AttentionArgs a)
     extern __shared__ uint8_t raw[];
     __shared__ long long found[40];
     __shared__ __align__(8) uint64_t bars[kBarriers];
-    __shared__ float4 scales[kConstSlots][kGroups];   // of 16 tokens: scale of the keys, log2 and inverse of the values'
+    // of 16 tokens: scale of the keys, log2 and inverse of the values'. A scale that is not finite becomes (0, 1e30, NaN): a row that
+    // sees a token of such a page has a sum of NaN, and one that does not has nothing of it
+    __shared__ float4 scales[kConstSlots][kGroups];
     __shared__ uint32_t tmem_base;
     __shared__ WorkWalk walks[kWalkers];
     __shared__ int given_up_word;
@@ -172,7 +227,7 @@ prompt_kernel(const AttentionArgs a)
         for (int i = 0; i < kBarriers; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_address(bars + i)), "r"(counts[i]));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_address(&tmem_base)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -191,7 +246,7 @@ prompt_kernel(const AttentionArgs a)
     Piece piece;
 
     if (group < 2) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         const int half = group, local = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const uint32_t s_at = tmem + lanes + half * 128, o_at = tmem + lanes + 256 + half * D;
@@ -252,30 +307,36 @@ prompt_kernel(const AttentionArgs a)
                     __syncwarp();
                     s_phase ^= 1u;
                     fence_after();
-                    float s[kTile];
-#pragma unroll
-                    for (int i = 0; i < kTile; i += 32) tmem_load32(s_at + i, reinterpret_cast<uint32_t *>(s + i));
+                    // S is read twice in part: its first half for the maximum and, after the second half has been worked off, again
+                    // (128 scores of a row would not fit the registers beside their P). P takes the place of the second half.
                     const float4 *of_tile = scales[(slot0 + j - h.first) % kConstSlots];
-                    const bool masked = (j + 1) * kTile > all_see;
-                    float most = -INFINITY;
+                    const int see = (j + 1) * kTile > all_see ? limit - j * kTile : kTile;
+                    float s[64], most = -INFINITY;
+                    auto read = [&](int part) {
+                        tmem_load64(s_at + 64 * part, reinterpret_cast<uint32_t *>(s));
+                        if (__any_sync(0xffffffffu, see < kTile)) {
 #pragma unroll
-                    for (int g = 0; g < kGroups; ++g) {
-                        const float4 k = of_tile[g];
-                        float *x = s + 16 * g;
-                        const float by = k.x * factor;
-                        if (masked) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                x[i] = j * kTile + 16 * g + i < limit ? fmaf(x[i], by, k.y) : -INFINITY;
-                                most = fmaxf(most, x[i]);
-                            }
-                        } else {
-                            float top = x[0];
-#pragma unroll
-                            for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
-                            most = fmaxf(most, fmaf(top, by, k.y));
+                            for (int i = 0; i < 64; ++i) s[i] = i < see - 64 * part ? s[i] : -INFINITY;
                         }
-                    }
+                    };
+                    auto maximum = [&](int part) {
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const float4 k = of_tile[4 * part + g];
+                            const float *x = s + 16 * g;
+                            float top = max3(x[0], x[1], x[2]), top2 = max3(x[3], x[4], x[5]);
+                            top = max3(top, x[6], x[7]);
+                            top2 = max3(top2, x[8], x[9]);
+                            top = max3(top, x[10], x[11]);
+                            top2 = max3(top2, x[12], x[13]);
+                            top = max3(top, x[14], x[15]);
+                            most = fmaxf(most, fmaf(fmaxf(top, top2), fmaxf(k.x * factor, kLeastFactor), k.y));
+                        }
+                    };
+                    read(0);
+                    maximum(0);
+                    read(1);
+                    maximum(1);
                     const bool grown = most > m + 8.f || (m == -INFINITY && most > m);
                     if (__any_sync(0xffffffffu, grown)) {
                         const float keep = grown ? exp2_fast(m - most) : 1.f;
@@ -298,26 +359,34 @@ prompt_kernel(const AttentionArgs a)
                     }
                     if (j > h.first) o_phase ^= 1u;
                     const float base = m == -INFINITY ? 0.f : m;
+                    auto weights = [&](int part) {
 #pragma unroll
-                    for (int part = 0; part < 2; ++part) {
-                        uint32_t p[32];
+                        for (int two = 0; two < 2; ++two) {
+                            uint32_t p[16];
 #pragma unroll
-                        for (int gg = 0; gg < kGroups / 2; ++gg) {
-                            const int g = part * (kGroups / 2) + gg;
-                            const float4 k = of_tile[g];
-                            float *x = s + 16 * g;
-                            const float by = masked ? 1.f : k.x * factor, plus = masked ? -base : k.y - base;
-                            float sum = 0.f;
+                            for (int gg = 0; gg < 2; ++gg) {
+                                const int g = 2 * two + gg;
+                                const float4 k = of_tile[4 * part + g];
+                                const float by = fmaxf(k.x * factor, kLeastFactor), plus = k.y - base;
+                                const uint64_t by2 = pair(by, by), plus2 = pair(plus, plus);
+                                uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                const float e0 = exp2_fast(fmaf(x[i], by, plus)), e1 = exp2_fast(fmaf(x[i + 1], by, plus));
-                                sum += e0 + e1;
-                                p[8 * gg + i / 2] = pack2<false>(e0, e1);
+                                for (int i = 0; i < 16; i += 2) {
+                                    const float2 x = unpair(fma_pair(pair(s[16 * g + i], s[16 * g + i + 1]), by2, plus2));
+                                    const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
+                                    sum[(i >> 1) & 1] = add_pair(sum[(i >> 1) & 1], pair(e0, e1));
+                                    p[8 * gg + i / 2] = pack2<false>(e0, e1);
+                                }
+                                const float2 both = unpair(add_pair(sum[0], sum[1]));
+                                const float all = both.x + both.y;
+                                l += all == 0.f ? 0.f : all * k.z;
                             }
-                            l += sum == 0.f ? 0.f : sum * k.z;   // tokens that a row does not see may have any scale
+                            tmem_store16(s_at + 64 + 32 * part + 16 * two, p);
                         }
-                        tmem_store32(s_at + 32 * part, p);
-                    }
+                    };
+                    weights(1);
+                    read(0);
+                    weights(0);
                     tmem_store_wait();
                     fence_before();
                     arrive(bars + kPFull + half);
@@ -372,36 +441,53 @@ prompt_kernel(const AttentionArgs a)
             }
             slot0 += max(h.last - h.first, 0);
         }
-    } else if (group == 2) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    } else if (group < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        const bool is_v = group == 3;
         constexpr int kChunks = D / 16;                  // 16-byte chunks of a token
-        constexpr int kItems = kTile * kChunks / 128;    // that a thread converts of K, and of V
+        constexpr int kItems = kTile * kChunks / 128;    // that a thread converts
         const int local = tid & 127, chunk = local % kChunks, token = local / kChunks;   // item i: token + i * 128 / kChunks
+        const int page_mask = (1 << c.page_log2) - 1;
+        const long long page_stride = is_v ? c.v_stride : c.k_stride;
+        uint64_t *full = bars + (is_v ? kVFull : kKFull), *empty = bars + (is_v ? kVEmpty : kKEmpty);
+        // chunk: 16 dimensions, two 16-byte pieces of the row in block chunk / 4; odd blocks store the second one first, so that
+        // eight neighbouring threads fill all banks
+        const int flip = (chunk >> 2) & 1;
+        uint8_t *const to = smem + (is_v ? L::kV : L::kK) + (chunk >> 2) * kBlockBytes;
         int n = 0;                                       // tiles so far
         while (next_piece(walk, a, piece)) {
             const UnitRows u = unit_rows(a, walk.s, piece);
             const HalfTiles h = half_tiles(a, u, piece);
             const int end = max(0, min(u.begin + u.queries, r.capacity));   // no row sees anything from here on
-            const long long head_at = ((long long)piece.kv_head << c.page_log2) * D + 16 * chunk;
-            const int page_mask = (1 << c.page_log2) - 1;
+            const uint8_t *base = (is_v ? c.v : c.k) + ((long long)piece.kv_head << c.page_log2) * D + 16 * chunk;
             // page of the tile's block of 16 tokens `lane`, in the first 8 lanes
             auto pages_of = [&](int tile) {
                 const int t = tile * kTile + 16 * lane;
-                return lane < kGroups && t < end ? page_at(c, r, piece.sequence, t) : -1;
+                return lane < kGroups && tile < h.last && t < end ? page_at(c, r, piece.sequence, t) : -1;
             };
-            auto load = [&](const uint8_t *base, long long stride, int tile, int pages, uint4 (&x)[kItems]) {
+            uint4 x[kItems];
+            auto load = [&](int tile, int pages) {
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
                     const int row = token + i * (128 / kChunks), at = tile * kTile + row;
                     const int page = __shfl_sync(0xffffffffu, pages, row >> 4);
                     x[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (page >= 0 && at < end) x[i] = __ldcg(reinterpret_cast<const uint4 *>(base + page * stride + head_at + (long long)(at & page_mask) * D));
+                    if (page >= 0 && at < end) x[i] = __ldcg(reinterpret_cast<const uint4 *>(base + page * page_stride + (at & page_mask) * D));
                 }
             };
-            auto store = [&](uint8_t *to, const uint4 (&x)[kItems]) {
-                // chunk: 16 dimensions, two 16-byte pieces of the row in block chunk / 4; odd blocks store the second one first,
-                // so that eight neighbouring threads fill all banks
-                const int flip = (chunk >> 2) & 1;
+            int pages = pages_of(h.first), pages_next = pages_of(h.first + 1);
+            load(h.first, pages);
+            for (int j = h.first; j < h.last; ++j, ++n) {
+                const int stage = n & 1;
+                float4 of_lane = make_float4(0.f, -INFINITY, 0.f, 0.f);
+                if (warp == 8 && pages >= 0) {
+                    const float ks = __ldcg(c.k_scale + pages * c.k_scale_stride + piece.kv_head);
+                    const float vs = value_scale(__ldcg(c.v_scale + pages * c.v_scale_stride + piece.kv_head));
+                    of_lane = ks < INFINITY && vs < INFINITY ? make_float4(ks, __log2f(vs), 1.f / vs, 0.f)
+                                                             : make_float4(0.f, 1e30f, __uint_as_float(0x7fffffffu), 0.f);
+                }
+                wait(empty + stage, ((n >> 1) & 1) ^ 1, given_up);
+                __syncwarp();
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
                     const int row = token + i * (128 / kChunks);
@@ -410,45 +496,22 @@ prompt_kernel(const AttentionArgs a)
                     codes_to_half<E4M3>(x[i].y, lo.z, lo.w);
                     codes_to_half<E4M3>(x[i].z, hi.x, hi.y);
                     codes_to_half<E4M3>(x[i].w, hi.z, hi.w);
-                    uint8_t *at = to + (chunk >> 2) * kBlockBytes + row * 128;
+                    uint8_t *at = to + stage * L::kOperand + row * 128;
                     const int first = 2 * (chunk & 3) + flip;
                     *reinterpret_cast<uint4 *>(at + ((first ^ (row & 7)) << 4)) = flip ? hi : lo;
                     *reinterpret_cast<uint4 *>(at + (((first ^ 1) ^ (row & 7)) << 4)) = flip ? lo : hi;
                 }
-            };
-            uint4 kx[kItems], vx[kItems];
-            int pages = -1, pages_next = -1;
-            if (h.first < h.last) {
-                pages = pages_of(h.first);
-                load(c.k, c.k_stride, h.first, pages, kx);
-            }
-            for (int j = h.first; j < h.last; ++j, ++n) {
-                const int stage = n & 1;
-                const uint32_t empty = ((n >> 1) & 1) ^ 1;
-                load(c.v, c.v_stride, j, pages, vx);
-                float4 of_lane = make_float4(0.f, -INFINITY, 0.f, 0.f);
-                if (warp == 8 && lane < kGroups && pages >= 0) {
-                    const float ks = __ldcg(c.k_scale + pages * c.k_scale_stride + piece.kv_head);
-                    const float vs = value_scale(__ldcg(c.v_scale + pages * c.v_scale_stride + piece.kv_head));
-                    of_lane = make_float4(ks, __log2f(vs), 1.f / vs, 0.f);
-                }
-                if (j + 1 < h.last) pages_next = pages_of(j + 1);
-                wait(bars + kKEmpty + stage, empty, given_up);
-                store(smem + L::kK + stage * L::kOperand, kx);
                 if (warp == 8 && lane < kGroups) scales[n % kConstSlots][lane] = of_lane;
                 fence_shared();
-                arrive(bars + kKFull + stage);
-                if (j + 1 < h.last) load(c.k, c.k_stride, j + 1, pages_next, kx);
-                wait(bars + kVEmpty + stage, empty, given_up);
-                store(smem + L::kV + stage * L::kOperand, vx);
-                fence_shared();
-                arrive(bars + kVFull + stage);
+                arrive(full + stage);
                 pages = pages_next;
+                if (j + 1 < h.last) load(j + 1, pages);
+                pages_next = pages_of(j + 2);
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 16) {
             int n = 0;
             uint32_t q_phase = 0, p_phase = 0;    // one bit per half
             while (next_piece(walk, a, piece)) {
@@ -486,7 +549,7 @@ prompt_kernel(const AttentionArgs a)
                             const uint32_t va = smem_address(smem + L::kV + stage * L::kOperand);
 #pragma unroll
                             for (int t = 0; t < kTile / 16; ++t)
-                                mma_ts(tmem + 256 + w * D, tmem + w * 128 + 8 * t, descriptor(va + t * 2048, kBlockBytes, 1024), instruction(D, true),
+                                mma_ts(tmem + 256 + w * D, tmem + w * 128 + 64 + 8 * t, descriptor(va + t * 2048, kBlockBytes, 1024), instruction(D, true),
                                        j > h.first || t > 0);
                             commit(bars + kODone + w);
                             if (w == last_half(j)) commit(bars + kVEmpty + stage);
@@ -508,7 +571,7 @@ prompt_kernel(const AttentionArgs a)
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     clear_other_rows(a);
 }
 
