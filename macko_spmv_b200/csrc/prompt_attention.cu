@@ -62,6 +62,13 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile in
     return false;
 }
 
+__device__ __forceinline__ bool elected()
+{
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
+
 // Shared memory operand in the 128-byte swizzle. `leading`, `stride`: bytes between blocks of 64 elements along the contiguous dimension
 // (where that is not the one summed over) and between groups of 8 rows.
 __device__ __forceinline__ uint64_t descriptor(uint32_t address, uint32_t leading, uint32_t stride)
@@ -333,10 +340,11 @@ prompt_kernel(const AttentionArgs a)
                             most = fmaxf(most, fmaf(fmaxf(top, top2), fmaxf(k.x * factor, kLeastFactor), k.y));
                         }
                     };
-                    read(0);
-                    maximum(0);
-                    read(1);
-                    maximum(1);
+#pragma unroll 1
+                    for (int part = 0; part < 2; ++part) {   // rolled, like the other loops of this kernel that can be: its groups of
+                        read(part);                          // warps have little room for instructions (measured: a tenth of the time)
+                        maximum(part);
+                    }
                     const bool grown = most > m + 8.f || (m == -INFINITY && most > m);
                     if (__any_sync(0xffffffffu, grown)) {
                         const float keep = grown ? exp2_fast(m - most) : 1.f;
@@ -384,9 +392,12 @@ prompt_kernel(const AttentionArgs a)
                             tmem_store16(s_at + 64 + 32 * part + 16 * two, p);
                         }
                     };
-                    weights(1);
-                    read(0);
-                    weights(0);
+#pragma unroll 1
+                    for (int part = 1;; part = 0) {
+                        weights(part);
+                        if (part == 0) break;
+                        read(0);
+                    }
                     tmem_store_wait();
                     fence_before();
                     arrive(bars + kPFull + half);
@@ -512,56 +523,66 @@ prompt_kernel(const AttentionArgs a)
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 16) {
+            // The whole warp walks and waits; one elected thread issues. What the instructions take is the same in all lanes in a way
+            // that the compiler can see (shuffles, election), so that it stays in uniform registers: with `if (lane == 0)` an issue
+            // took some 200 cycles.
+            const uint32_t d_at = __shfl_sync(0xffffffffu, tmem, 0), operands = __shfl_sync(0xffffffffu, smem_address(smem), 0);
             int n = 0;
             uint32_t q_phase = 0, p_phase = 0;    // one bit per half
             while (next_piece(walk, a, piece)) {
                 const HalfTiles h = half_tiles(a, unit_rows(a, walk.s, piece), piece);
-                if (lane == 0) {
-                    auto last_half = [&](int j) { return j < h.end[1] ? 1 : 0; };
-                    auto scores = [&](int w, int j) {
-                        const int tile = n + j - h.first, stage = tile & 1;
-                        if (j == h.first) {
-                            wait(bars + kQFull + w, (q_phase >> w) & 1u, given_up);
-                            q_phase ^= 1u << w;
-                        }
-                        wait(bars + kKFull + stage, (tile >> 1) & 1, given_up);
-                        fence_after();
-                        const uint32_t qa = smem_address(smem + L::kQ + w * L::kOperand), ka = smem_address(smem + L::kK + stage * L::kOperand);
-#pragma unroll
-                        for (int d = 0; d < D / 16; ++d) {
-                            const uint32_t at = (d >> 2) * kBlockBytes + (d & 3) * 32;
-                            mma_ss(tmem + w * 128, descriptor(qa + at, 16, 1024), descriptor(ka + at, 16, 1024), instruction(kTile, false), d > 0);
-                        }
-                        commit(bars + kSFull + w);
-                        if (w == last_half(j)) commit(bars + kKEmpty + stage);
-                    };
-                    if (h.first < h.end[0]) scores(0, h.first);
-                    if (h.first < h.end[1]) scores(1, h.first);
-                    for (int j = h.first; j < h.last; ++j) {
-                        const int tile = n + j - h.first, stage = tile & 1;
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            if (j >= h.end[w]) continue;
+                const int first = __shfl_sync(0xffffffffu, h.first, 0), end0 = __shfl_sync(0xffffffffu, h.end[0], 0), end1 = __shfl_sync(0xffffffffu, h.end[1], 0);
+                const int last = max(end0, end1);
+                // S of the first tile, then for every tile and half: O += P V, and S of the tile behind it
+                for (int j = first - 1; j < last; ++j) {
+#pragma unroll 1
+                    for (int w = 0; w < 2; ++w) {
+                        const int end = w ? end1 : end0;
+                        if (j >= first && j < end) {
+                            const int tile = n + j - first, stage = tile & 1;
                             wait(bars + kPFull + w, (p_phase >> w) & 1u, given_up);
                             p_phase ^= 1u << w;
                             wait(bars + kVFull + stage, (tile >> 1) & 1, given_up);
+                            __syncwarp();
                             fence_after();
-                            const uint32_t va = smem_address(smem + L::kV + stage * L::kOperand);
+                            if (elected()) {
+                                const uint64_t v = descriptor(operands + L::kV + stage * L::kOperand, kBlockBytes, 1024);
+                                const uint32_t o = d_at + 256 + w * D, p = d_at + w * 128 + 64;
 #pragma unroll
-                            for (int t = 0; t < kTile / 16; ++t)
-                                mma_ts(tmem + 256 + w * D, tmem + w * 128 + 64 + 8 * t, descriptor(va + t * 2048, kBlockBytes, 1024), instruction(D, true),
-                                       j > h.first || t > 0);
-                            commit(bars + kODone + w);
-                            if (w == last_half(j)) commit(bars + kVEmpty + stage);
-                            if (j + 1 < h.end[w]) scores(w, j + 1);
+                                for (int t = 0; t < kTile / 16; ++t) mma_ts(o, p + 8 * t, v + t * (2048 >> 4), instruction(D, true), j > first || t > 0);
+                                commit(bars + kODone + w);
+                                if (w == (j < end1)) commit(bars + kVEmpty + stage);   // the last half that takes part
+                            }
+                            __syncwarp();
+                        }
+                        if (j + 1 < end) {
+                            const int tile = n + j + 1 - first, stage = tile & 1;
+                            if (j + 1 == first) {
+                                wait(bars + kQFull + w, (q_phase >> w) & 1u, given_up);
+                                q_phase ^= 1u << w;
+                            }
+                            wait(bars + kKFull + stage, (tile >> 1) & 1, given_up);
+                            __syncwarp();
+                            fence_after();
+                            if (elected()) {
+                                const uint64_t q = descriptor(operands + L::kQ + w * L::kOperand, 16, 1024);
+                                const uint64_t k = descriptor(operands + L::kK + stage * L::kOperand, 16, 1024);
+#pragma unroll
+                                for (int d = 0; d < D / 16; ++d) {
+                                    const uint32_t at = ((d >> 2) * kBlockBytes + (d & 3) * 32) >> 4;
+                                    mma_ss(d_at + w * 128, q + at, k + at, instruction(kTile, false), d > 0);
+                                }
+                                commit(bars + kSFull + w);
+                                if (w == (j + 1 < end1)) commit(bars + kKEmpty + stage);
+                            }
+                            __syncwarp();
                         }
                     }
                 }
-                n += max(h.last - h.first, 0);
-                __syncwarp();
+                n += max(last - first, 0);
             }
             // all that was issued has arrived before shared and tensor memory are given back
-            if (lane == 0 && n > 0) {
+            if (n > 0) {
                 int never = 0;
                 wait(bars + kVEmpty + ((n - 1) & 1), ((n - 1) >> 1) & 1, &never);
             }
