@@ -27,7 +27,7 @@ struct SplitUnit {
 };
 
 // sum of floor((a * i + b) / m) for i = 0 .. n - 1
-__host__ __device__ inline long long floor_sum(unsigned long long n, unsigned long long m, unsigned long long a, unsigned long long b)
+__host__ __device__ __noinline__ inline long long floor_sum(unsigned long long n, unsigned long long m, unsigned long long a, unsigned long long b)
 {
     unsigned long long sum = 0;
     while (n > 0) {

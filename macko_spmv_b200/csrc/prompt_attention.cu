@@ -28,7 +28,7 @@ constexpr int kTile = kPromptTile;
 constexpr int kGroups = kTile / 16;     // blocks of 16 tokens: each lies on one page
 constexpr int kConstSlots = 4;
 constexpr float kLeastFactor = 1e-36f;  // a score times nothing is still minus infinity where it is masked
-constexpr int kWalkers = 17;            // warps that walk the CTA's pieces, each for itself
+constexpr int kWorkers = 17;            // warps that are given the CTA's pieces
 
 // Shared memory, from a 1024-byte boundary: Q of both halves, K and V stages, each as [64 dimensions][128 rows][128 bytes].
 template <int D> struct Layout {
@@ -37,13 +37,16 @@ template <int D> struct Layout {
     static constexpr int kBytes = kEnd + 1024;
 };
 
-enum Barrier { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPFull = 12, kODone = 14, kBarriers = 16 };
+enum Barrier { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPFull = 12, kODone = 14, kJobFull = 16, kJobEmpty = 18, kBarriers = 20 };
 
 __device__ __forceinline__ uint32_t smem_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// One arrival for the warp, behind what all its lanes have done. (An arrival per lane is 32 atomic operations one after another.)
 __device__ __forceinline__ void arrive(uint64_t *bar)
 {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_address(bar)) : "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0)
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_address(bar)) : "memory");
 }
 
 // Waits for the phase with parity `parity`; false (and from then on for every wait of the CTA) where it does not come. The thread
@@ -51,6 +54,7 @@ __device__ __forceinline__ void arrive(uint64_t *bar)
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *given_up)
 {
     const uint32_t at = smem_address(bar);
+#pragma unroll 1
     for (int i = 0; i < 4096; ++i) {
         uint32_t done;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -60,6 +64,14 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile in
     }
     *given_up = 1;
     return false;
+}
+
+// 16 bytes of global memory, or zeros.
+__device__ __forceinline__ void load_if(uint4 &x, const uint8_t *p, bool there)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                 "@p ld.global.cg.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "=&r"(x.x), "=&r"(x.y), "=&r"(x.z), "=&r"(x.w) : "l"(p), "r"((int)there));
 }
 
 __device__ __forceinline__ bool elected()
@@ -195,15 +207,23 @@ __device__ __forceinline__ HalfTiles half_tiles(const AttentionArgs &a, const Un
     return h;
 }
 
-// The warp's next piece. The walk itself stays in shared memory: its registers are wanted elsewhere.
-__device__ __forceinline__ bool next_piece(WorkWalk &shared, const AttentionArgs &a, Piece &p)
+// A piece as the working warps are given it: by one warp that does nothing else, through two slots of shared memory. (Finding it
+// takes 64-bit divisions: as a part of every role it made the kernel three times as long, and the roles waited for their instructions.)
+struct Job {
+    UnitRows u;
+    HalfTiles h;             // first < 0: there are no more
+    int sequence, kv_head, pieces;
+    bool begins, ends;
+};
+
+__device__ __forceinline__ bool next_job(Job &job, const Job *jobs, uint64_t *bars, int &count, volatile int *given_up)
 {
-    WorkWalk walk = shared;
-    __syncwarp();
-    const bool more = walk.next(a.work, a.rows, p);
-    if ((threadIdx.x & 31) == 0) shared = walk;
-    __syncwarp();
-    return more;
+    const int slot = count & 1;
+    wait(bars + kJobFull + slot, (count >> 1) & 1, given_up);
+    job = jobs[slot];
+    arrive(bars + kJobEmpty + slot);
+    ++count;
+    return job.h.first >= 0 && !*given_up;
 }
 
 template <bool BF16, bool E4M3, int D>
@@ -219,7 +239,7 @@ prompt_kernel(const AttentionArgs a)
     // sees a token of such a page has a sum of NaN, and one that does not has nothing of it
     __shared__ float4 scales[kConstSlots][kGroups];
     __shared__ uint32_t tmem_base;
-    __shared__ WorkWalk walks[kWalkers];
+    __shared__ Job jobs[2];
     __shared__ int given_up_word;
     volatile int *given_up = &given_up_word;
     uint8_t *smem = raw + ((1024u - (smem_address(raw) & 1023u)) & 1023u);
@@ -230,7 +250,7 @@ prompt_kernel(const AttentionArgs a)
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
         given_up_word = 0;
-        const int counts[kBarriers] = {128, 128, 128, 128, 1, 1, 128, 128, 1, 1, 1, 1, 128, 128, 1, 1};
+        const int counts[kBarriers] = {4, 4, 4, 4, 1, 1, 4, 4, 1, 1, 1, 1, 4, 4, 1, 1, 1, 1, kWorkers, kWorkers};
         for (int i = 0; i < kBarriers; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_address(bars + i)), "r"(counts[i]));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -240,17 +260,14 @@ prompt_kernel(const AttentionArgs a)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (tid == 0) a.split[blockIdx.x].pieces = 0;
-    {
-        WorkWalk walk;
-        walk.start(a.work, r, blockIdx.x, found);
-        if (lane == 0 && warp < kWalkers) walks[warp] = walk;
-    }
+    WorkWalk walk;
+    walk.start(a.work, r, blockIdx.x, found);
     fence_before();
     __syncthreads();
     fence_after();
-    WorkWalk &walk = walks[warp < kWalkers ? warp : 0];
     const uint32_t tmem = tmem_base;   // columns: S of half 0 and 1 (128 each), O of half 0 and 1 (D each)
-    Piece piece;
+    Job job;
+    int job_count = 0;
 
     if (group < 2) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
@@ -259,9 +276,9 @@ prompt_kernel(const AttentionArgs a)
         const uint32_t s_at = tmem + lanes + half * 128, o_at = tmem + lanes + 256 + half * D;
         uint32_t s_phase = 0, o_phase = 0;
         int slot0 = 0;                      // tiles of the pieces before: where this piece's scales begin
-        while (next_piece(walk, a, piece)) {
-            const UnitRows u = unit_rows(a, walk.s, piece);
-            const HalfTiles h = half_tiles(a, u, piece);
+        while (next_job(job, jobs, bars, job_count, given_up)) {
+            const UnitRows &u = job.u;
+            const HalfTiles &h = job.h;
             if (h.rows[half] > 0) {
                 const int row = half * 128 + local, query = row / u.heads, head = u.head + row % u.heads;
                 const bool there = local < h.rows[half];
@@ -309,6 +326,7 @@ prompt_kernel(const AttentionArgs a)
                 const int limit = there ? min(u.begin + query + 1, r.capacity) : 0;           // tokens that this row sees
                 const int all_see = min(u.begin + 128 * half / u.heads + 1, r.capacity);      // that every row of this half sees
                 float m = -INFINITY, l = 0.f;
+#pragma unroll 1
                 for (int j = h.first; j < h.end[half]; ++j) {
                     wait(bars + kSFull + half, s_phase, given_up);
                     __syncwarp();
@@ -409,8 +427,8 @@ prompt_kernel(const AttentionArgs a)
                     o_phase ^= 1u;
                     fence_after();
                 }
-                const bool alone = piece.begins && piece.ends, empty = h.first >= h.end[half];
-                float *partial = a.partial + ((long long)blockIdx.x * 2 + (piece.begins ? 1 : 0)) * kPromptRows * (D + 2);
+                const bool alone = job.begins && job.ends, empty = h.first >= h.end[half];
+                float *partial = a.partial + ((long long)blockIdx.x * 2 + (job.begins ? 1 : 0)) * kPromptRows * (D + 2);
                 float by = alone ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 if (*given_up) by = __uint_as_float(0x7fffffffu);
 #pragma unroll 1
@@ -446,8 +464,8 @@ prompt_kernel(const AttentionArgs a)
                     partial[kPromptRows * D + row] = m;
                     partial[kPromptRows * D + kPromptRows + row] = l;
                 }
-                if (!alone && piece.begins && row == 0)
-                    a.split[blockIdx.x] = SplitUnit{u.first_row, u.rows(), u.head, piece.pieces, u.heads, {0, 0, 0}};
+                if (!alone && job.begins && row == 0)
+                    a.split[blockIdx.x] = SplitUnit{u.first_row, u.rows(), u.head, job.pieces, u.heads, {0, 0, 0}};
                 fence_before();   // O is read before this half arrives for the next piece's P
             }
             slot0 += max(h.last - h.first, 0);
@@ -466,34 +484,36 @@ prompt_kernel(const AttentionArgs a)
         const int flip = (chunk >> 2) & 1;
         uint8_t *const to = smem + (is_v ? L::kV : L::kK) + (chunk >> 2) * kBlockBytes;
         int n = 0;                                       // tiles so far
-        while (next_piece(walk, a, piece)) {
-            const UnitRows u = unit_rows(a, walk.s, piece);
-            const HalfTiles h = half_tiles(a, u, piece);
+        while (next_job(job, jobs, bars, job_count, given_up)) {
+            const UnitRows &u = job.u;
+            const HalfTiles &h = job.h;
             const int end = max(0, min(u.begin + u.queries, r.capacity));   // no row sees anything from here on
-            const uint8_t *base = (is_v ? c.v : c.k) + ((long long)piece.kv_head << c.page_log2) * D + 16 * chunk;
+            const uint8_t *base = (is_v ? c.v : c.k) + ((long long)job.kv_head << c.page_log2) * D + 16 * chunk;
             // page of the tile's block of 16 tokens `lane`, in the first 8 lanes
             auto pages_of = [&](int tile) {
                 const int t = tile * kTile + 16 * lane;
-                return lane < kGroups && tile < h.last && t < end ? page_at(c, r, piece.sequence, t) : -1;
+                return lane < kGroups && tile < h.last && t < end ? page_at(c, r, job.sequence, t) : -1;
             };
             uint4 x[kItems];
+            // all loads are issued before any is waited for, without branches between them
             auto load = [&](int tile, int pages) {
+                const long long page_off = pages >= 0 ? pages * page_stride : -1;
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
-                    const int row = token + i * (128 / kChunks), at = tile * kTile + row;
-                    const int page = __shfl_sync(0xffffffffu, pages, row >> 4);
-                    x[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (page >= 0 && at < end) x[i] = __ldcg(reinterpret_cast<const uint4 *>(base + page * page_stride + (at & page_mask) * D));
+                    const int row = token + i * (128 / kChunks);
+                    const long long off = __shfl_sync(0xffffffffu, page_off, row >> 4);
+                    load_if(x[i], base + off + (row & page_mask) * D, off >= 0 && tile * kTile + row < end);
                 }
             };
             int pages = pages_of(h.first), pages_next = pages_of(h.first + 1);
             load(h.first, pages);
+#pragma unroll 1
             for (int j = h.first; j < h.last; ++j, ++n) {
                 const int stage = n & 1;
                 float4 of_lane = make_float4(0.f, -INFINITY, 0.f, 0.f);
                 if (warp == 8 && pages >= 0) {
-                    const float ks = __ldcg(c.k_scale + pages * c.k_scale_stride + piece.kv_head);
-                    const float vs = value_scale(__ldcg(c.v_scale + pages * c.v_scale_stride + piece.kv_head));
+                    const float ks = __ldcg(c.k_scale + pages * c.k_scale_stride + job.kv_head);
+                    const float vs = value_scale(__ldcg(c.v_scale + pages * c.v_scale_stride + job.kv_head));
                     of_lane = ks < INFINITY && vs < INFINITY ? make_float4(ks, __log2f(vs), 1.f / vs, 0.f)
                                                              : make_float4(0.f, 1e30f, __uint_as_float(0x7fffffffu), 0.f);
                 }
@@ -529,11 +549,12 @@ prompt_kernel(const AttentionArgs a)
             const uint32_t d_at = __shfl_sync(0xffffffffu, tmem, 0), operands = __shfl_sync(0xffffffffu, smem_address(smem), 0);
             int n = 0;
             uint32_t q_phase = 0, p_phase = 0;    // one bit per half
-            while (next_piece(walk, a, piece)) {
-                const HalfTiles h = half_tiles(a, unit_rows(a, walk.s, piece), piece);
+            while (next_job(job, jobs, bars, job_count, given_up)) {
+                const HalfTiles &h = job.h;
                 const int first = __shfl_sync(0xffffffffu, h.first, 0), end0 = __shfl_sync(0xffffffffu, h.end[0], 0), end1 = __shfl_sync(0xffffffffu, h.end[1], 0);
                 const int last = max(end0, end1);
                 // S of the first tile, then for every tile and half: O += P V, and S of the tile behind it
+#pragma unroll 1
                 for (int j = first - 1; j < last; ++j) {
 #pragma unroll 1
                     for (int w = 0; w < 2; ++w) {
@@ -587,6 +608,26 @@ prompt_kernel(const AttentionArgs a)
                 wait(bars + kVEmpty + ((n - 1) & 1), ((n - 1) >> 1) & 1, &never);
             }
             __syncwarp();
+        } else if (warp == 17) {
+            Piece piece;
+            for (bool more = true; more; ++job_count) {
+                more = walk.next(a.work, r, piece);
+                wait(bars + kJobEmpty + (job_count & 1), ((job_count >> 1) & 1) ^ 1, given_up);
+                if (lane == 0) {
+                    job.h.first = -1;
+                    if (more) {
+                        job.u = unit_rows(a, walk.s, piece);
+                        job.h = half_tiles(a, job.u, piece);
+                        job.sequence = piece.sequence;
+                        job.kv_head = piece.kv_head;
+                        job.pieces = piece.pieces;
+                        job.begins = piece.begins;
+                        job.ends = piece.ends;
+                    }
+                    jobs[job_count & 1] = job;
+                }
+                arrive(bars + kJobFull + (job_count & 1));
+            }
         }
     }
     fence_before();
