@@ -20,7 +20,7 @@ struct AttentionArgs {
 
 // Rows per unit of the kernel for many rows, and its launch (no join): prompt_attention.cu. head_dim 64 or 128.
 constexpr int kPromptRows = 256;
-constexpr int kPromptTile = 128;
+constexpr int kPromptTile = 64;
 int launch_prompt_attention(const AttentionArgs &a, bool bf16, bool e4m3, cudaStream_t stream);
 
 #ifdef __CUDACC__

@@ -517,7 +517,7 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     l->work.tile = prompt ? kPromptTile : kWarps * 16 * (d == 256 ? 1 : 2);
     l->work.group = group;
     l->work.kv_heads = a.cache.kv_heads;
-    l->work.least_share = 4;
+    l->work.least_share = 512 / l->work.tile;
     l->smem = (kWarps * rows * d + 2 * kWarps * rows) * 4;
     const int64_t units = (int64_t)a.rows.sequences * a.cache.kv_heads * l->work.parts;
     l->split = !(one_each && a.rows.capacity <= 512);

@@ -4,17 +4,18 @@
 //   out  = sum 2^(x(t) - m) v_t  /  sum 2^(x(t) - m) / v_scale(page)
 //
 // as in the kernel for a few rows. One CTA per SM walks its share of the call's tiles (attention_work.cuh): units of 256 packed rows (rows
-// of the call times heads of a group) in two halves of 128, tiles of 128 tokens. Five groups of warps:
+// of the call times heads of a group) in two halves of 128, tiles of 64 tokens. Five groups of warps:
 //
 //   0, 1   softmax of one half each, one row per thread: S from tensor memory, maximum, 2^x, P as fp16 over S in tensor memory; the
 //          accumulator is rescaled there when the maximum has grown by more than 8 (so weights are at most 2^8 and none is lost)
-//   2, 3   the cache, keys and values: codes from global memory to fp16 (exact) in shared memory, in the 128-byte swizzle, two stages
+//   2, 3   the cache, keys and values: codes from global memory to fp16 (exact) in shared memory, in the 128-byte swizzle, four stages
 //          each, and the scales of the tile's pages
-//   4      one thread that issues tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it lies
-//          (token by token: its "N" dimension is the contiguous one)
+//   4      one warp that issues tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it lies
+//          (token by token: its "N" dimension is the contiguous one); one that finds the CTA's next piece
 //
-// While one half's softmax runs the tensor core works for the other. A tile takes 2 x (512 + 512) cycles of tensor core and 2 x 1024 of the
-// exponential unit; the conversion of 32 K codes adds some 400 issue slots per scheduler.
+// Tensor memory holds two S of 64 columns and one O for each half, 512 columns at head_dim 128: S of the tile behind is there before
+// the softmax of this one is done. (With one S of 128 columns a half waited for its P to go through the tensor core and for the next S,
+// 1900 of 5400 cycles for 128 tokens.)
 //
 // Every wait has a limit: if one runs out, no further wait waits, and what the CTA writes from then on is NaN.
 #include "attention_args.cuh"
@@ -26,18 +27,24 @@ namespace {
 constexpr int kThreads = 640;
 constexpr int kTile = kPromptTile;
 constexpr int kGroups = kTile / 16;     // blocks of 16 tokens: each lies on one page
-constexpr int kConstSlots = 4;
+constexpr int kStages = 4;              // of K, and of V
+constexpr int kConstSlots = 8;          // keys are converted at most 6 tiles ahead of the softmax
 constexpr float kLeastFactor = 1e-36f;  // a score times nothing is still minus infinity where it is masked
 constexpr int kWorkers = 17;            // warps that are given the CTA's pieces
 
-// Shared memory, from a 1024-byte boundary: Q of both halves, K and V stages, each as [64 dimensions][128 rows][128 bytes].
+// Shared memory, from a 1024-byte boundary: Q of both halves, K and V stages, each as [64 dimensions][rows][128 bytes].
 template <int D> struct Layout {
-    static constexpr int kOperand = 128 * D * 2;
-    static constexpr int kQ = 0, kK = 2 * kOperand, kV = 4 * kOperand, kEnd = 6 * kOperand;
+    static constexpr int kHalf = 128 * D * 2, kStage = kTile * D * 2;
+    static constexpr int kQ = 0, kK = 2 * kHalf, kV = kK + kStages * kStage, kEnd = kV + kStages * kStage;
     static constexpr int kBytes = kEnd + 1024;
 };
 
-enum Barrier { kQFull = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kSFull = 10, kPFull = 12, kODone = 14, kJobFull = 16, kJobEmpty = 18, kBarriers = 20 };
+// Barriers with two or four in a row: of a half, of a stage, of half * 2 + S buffer, of a slot. A wait tells a phase from its neighbours
+// only: whoever waits for one knows that the one before has come and that the one behind it needs the waiter. (So O += P V has two
+// barriers for each half as well: both of the last two products may be done before anybody asks.)
+enum Barrier {
+    kQFull = 0, kKFull = 2, kKEmpty = 6, kVFull = 10, kVEmpty = 14, kSFull = 18, kPFull = 22, kODone = 26, kJobFull = 30, kJobEmpty = 32, kBarriers = 34
+};
 
 __device__ __forceinline__ uint32_t smem_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -231,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 prompt_kernel(const AttentionArgs a)
 {
     using L = Layout<D>;
-    constexpr uint32_t kBlockBytes = 128 * 128;
+    constexpr uint32_t kQBlock = 128 * 128, kBlock = kTile * 128;   // 64 dimensions of Q, and of K or V
     extern __shared__ uint8_t raw[];
     __shared__ long long found[40];
     __shared__ __align__(8) uint64_t bars[kBarriers];
@@ -250,7 +257,7 @@ prompt_kernel(const AttentionArgs a)
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
         given_up_word = 0;
-        const int counts[kBarriers] = {4, 4, 4, 4, 1, 1, 4, 4, 1, 1, 1, 1, 4, 4, 1, 1, 1, 1, kWorkers, kWorkers};
+        const int counts[kBarriers] = {4, 4, 4, 4, 4, 4, 1, 1, 1, 1, 4, 4, 4, 4, 1, 1, 1, 1, 1, 1, 1, 1, 4, 4, 4, 4, 1, 1, 1, 1, 1, 1, kWorkers, kWorkers};
         for (int i = 0; i < kBarriers; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_address(bars + i)), "r"(counts[i]));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -265,7 +272,7 @@ prompt_kernel(const AttentionArgs a)
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_base;   // columns: S of half 0 and 1 (128 each), O of half 0 and 1 (D each)
+    const uint32_t tmem = tmem_base;   // columns: two S of 64 of half 0 and of half 1, O of half 0 and 1 (D each)
     Job job;
     int job_count = 0;
 
@@ -273,8 +280,8 @@ prompt_kernel(const AttentionArgs a)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         const int half = group, local = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-        const uint32_t s_at = tmem + lanes + half * 128, o_at = tmem + lanes + 256 + half * D;
-        uint32_t s_phase = 0, o_phase = 0;
+        const uint32_t s_half = tmem + lanes + half * 128, o_at = tmem + lanes + 256 + half * D;
+        int done = 0;                       // tiles of this half in the pieces before
         int slot0 = 0;                      // tiles of the pieces before: where this piece's scales begin
         while (next_job(job, jobs, bars, job_count, given_up)) {
             const UnitRows &u = job.u;
@@ -315,10 +322,10 @@ prompt_kernel(const AttentionArgs a)
 #pragma unroll
                         for (int i = 0; i < D / 2; ++i) q[i] ^= 0x80008000u;
                     }
-                    uint8_t *to = smem + L::kQ + half * L::kOperand + local * 128;
+                    uint8_t *to = smem + L::kQ + half * L::kHalf + local * 128;
 #pragma unroll
                     for (int i = 0; i < D / 8; ++i)
-                        *reinterpret_cast<uint4 *>(to + (i >> 3) * kBlockBytes + (((i & 7) ^ (local & 7)) << 4)) =
+                        *reinterpret_cast<uint4 *>(to + (i >> 3) * kQBlock + (((i & 7) ^ (local & 7)) << 4)) =
                             make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
                     fence_shared();
                     arrive(bars + kQFull + half);
@@ -328,40 +335,30 @@ prompt_kernel(const AttentionArgs a)
                 float m = -INFINITY, l = 0.f;
 #pragma unroll 1
                 for (int j = h.first; j < h.end[half]; ++j) {
-                    wait(bars + kSFull + half, s_phase, given_up);
+                    const int count = done + j - h.first, buffer = count & 1;
+                    const uint32_t s_at = s_half + 64 * buffer;
+                    wait(bars + kSFull + 2 * half + buffer, (count >> 1) & 1, given_up);
                     __syncwarp();
-                    s_phase ^= 1u;
                     fence_after();
-                    // S is read twice in part: its first half for the maximum and, after the second half has been worked off, again
-                    // (128 scores of a row would not fit the registers beside their P). P takes the place of the second half.
                     const float4 *of_tile = scales[(slot0 + j - h.first) % kConstSlots];
-                    const int see = (j + 1) * kTile > all_see ? limit - j * kTile : kTile;
-                    float s[64], most = -INFINITY;
-                    auto read = [&](int part) {
-                        tmem_load64(s_at + 64 * part, reinterpret_cast<uint32_t *>(s));
-                        if (__any_sync(0xffffffffu, see < kTile)) {
+                    float s[kTile], most = -INFINITY;
+                    tmem_load64(s_at, reinterpret_cast<uint32_t *>(s));
+                    if ((j + 1) * kTile > all_see) {
+                        const int see = limit - j * kTile;
 #pragma unroll
-                            for (int i = 0; i < 64; ++i) s[i] = i < see - 64 * part ? s[i] : -INFINITY;
-                        }
-                    };
-                    auto maximum = [&](int part) {
+                        for (int i = 0; i < kTile; ++i) s[i] = i < see ? s[i] : -INFINITY;
+                    }
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const float4 k = of_tile[4 * part + g];
-                            const float *x = s + 16 * g;
-                            float top = max3(x[0], x[1], x[2]), top2 = max3(x[3], x[4], x[5]);
-                            top = max3(top, x[6], x[7]);
-                            top2 = max3(top2, x[8], x[9]);
-                            top = max3(top, x[10], x[11]);
-                            top2 = max3(top2, x[12], x[13]);
-                            top = max3(top, x[14], x[15]);
-                            most = fmaxf(most, fmaf(fmaxf(top, top2), fmaxf(k.x * factor, kLeastFactor), k.y));
-                        }
-                    };
-#pragma unroll 1
-                    for (int part = 0; part < 2; ++part) {   // rolled, like the other loops of this kernel that can be: its groups of
-                        read(part);                          // warps have little room for instructions (measured: a tenth of the time)
-                        maximum(part);
+                    for (int g = 0; g < kGroups; ++g) {
+                        const float4 k = of_tile[g];
+                        const float *x = s + 16 * g;
+                        float top = max3(x[0], x[1], x[2]), top2 = max3(x[3], x[4], x[5]);
+                        top = max3(top, x[6], x[7]);
+                        top2 = max3(top2, x[8], x[9]);
+                        top = max3(top, x[10], x[11]);
+                        top2 = max3(top2, x[12], x[13]);
+                        top = max3(top, x[14], x[15]);
+                        most = fmaxf(most, fmaf(fmaxf(top, top2), fmaxf(k.x * factor, kLeastFactor), k.y));
                     }
                     const bool grown = most > m + 8.f || (m == -INFINITY && most > m);
                     if (__any_sync(0xffffffffu, grown)) {
@@ -369,7 +366,7 @@ prompt_kernel(const AttentionArgs a)
                         if (grown) m = most;
                         l *= keep;
                         if (j > h.first) {
-                            wait(bars + kODone + half, o_phase, given_up);
+                            wait(bars + kODone + 2 * half + (buffer ^ 1), ((count - 1) >> 1) & 1, given_up);
                             __syncwarp();
                             fence_after();
 #pragma unroll 1
@@ -383,48 +380,39 @@ prompt_kernel(const AttentionArgs a)
                             tmem_store_wait();
                         }
                     }
-                    if (j > h.first) o_phase ^= 1u;
                     const float base = m == -INFINITY ? 0.f : m;
-                    auto weights = [&](int part) {
 #pragma unroll
-                        for (int two = 0; two < 2; ++two) {
-                            uint32_t p[16];
+                    for (int two = 0; two < 2; ++two) {
+                        uint32_t p[16];
 #pragma unroll
-                            for (int gg = 0; gg < 2; ++gg) {
-                                const int g = 2 * two + gg;
-                                const float4 k = of_tile[4 * part + g];
-                                const float by = fmaxf(k.x * factor, kLeastFactor), plus = k.y - base;
-                                const uint64_t by2 = pair(by, by), plus2 = pair(plus, plus);
-                                uint64_t sum[2] = {0ull, 0ull};
+                        for (int gg = 0; gg < 2; ++gg) {
+                            const int g = 2 * two + gg;
+                            const float4 k = of_tile[g];
+                            const float by = fmaxf(k.x * factor, kLeastFactor), plus = k.y - base;
+                            const uint64_t by2 = pair(by, by), plus2 = pair(plus, plus);
+                            uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                                for (int i = 0; i < 16; i += 2) {
-                                    const float2 x = unpair(fma_pair(pair(s[16 * g + i], s[16 * g + i + 1]), by2, plus2));
-                                    const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
-                                    sum[(i >> 1) & 1] = add_pair(sum[(i >> 1) & 1], pair(e0, e1));
-                                    p[8 * gg + i / 2] = pack2<false>(e0, e1);
-                                }
-                                const float2 both = unpair(add_pair(sum[0], sum[1]));
-                                const float all = both.x + both.y;
-                                l += all == 0.f ? 0.f : all * k.z;
+                            for (int i = 0; i < 16; i += 2) {
+                                const float2 x = unpair(fma_pair(pair(s[16 * g + i], s[16 * g + i + 1]), by2, plus2));
+                                const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
+                                sum[(i >> 1) & 1] = add_pair(sum[(i >> 1) & 1], pair(e0, e1));
+                                p[8 * gg + i / 2] = pack2<false>(e0, e1);
                             }
-                            tmem_store16(s_at + 64 + 32 * part + 16 * two, p);
+                            const float2 both = unpair(add_pair(sum[0], sum[1]));
+                            const float all = both.x + both.y;
+                            l += all == 0.f ? 0.f : all * k.z;   // tokens that a row does not see may have any scale
                         }
-                    };
-#pragma unroll 1
-                    for (int part = 1;; part = 0) {
-                        weights(part);
-                        if (part == 0) break;
-                        read(0);
+                        tmem_store16(s_at + 16 * two, p);
                     }
                     tmem_store_wait();
                     fence_before();
-                    arrive(bars + kPFull + half);
+                    arrive(bars + kPFull + 2 * half + buffer);
                 }
                 // the result of this half, divided or as a piece
                 if (h.first < h.end[half]) {
-                    wait(bars + kODone + half, o_phase, given_up);
+                    done += h.end[half] - h.first;
+                    wait(bars + kODone + 2 * half + ((done - 1) & 1), ((done - 1) >> 1) & 1, given_up);
                     __syncwarp();
-                    o_phase ^= 1u;
                     fence_after();
                 }
                 const bool alone = job.begins && job.ends, empty = h.first >= h.end[half];
@@ -482,42 +470,44 @@ prompt_kernel(const AttentionArgs a)
         // chunk: 16 dimensions, two 16-byte pieces of the row in block chunk / 4; odd blocks store the second one first, so that
         // eight neighbouring threads fill all banks
         const int flip = (chunk >> 2) & 1;
-        uint8_t *const to = smem + (is_v ? L::kV : L::kK) + (chunk >> 2) * kBlockBytes;
+        uint8_t *const to = smem + (is_v ? L::kV : L::kK) + (chunk >> 2) * kBlock;
         int n = 0;                                       // tiles so far
         while (next_job(job, jobs, bars, job_count, given_up)) {
             const UnitRows &u = job.u;
             const HalfTiles &h = job.h;
             const int end = max(0, min(u.begin + u.queries, r.capacity));   // no row sees anything from here on
             const uint8_t *base = (is_v ? c.v : c.k) + ((long long)job.kv_head << c.page_log2) * D + 16 * chunk;
-            // page of the tile's block of 16 tokens `lane`, in the first 8 lanes
-            auto pages_of = [&](int tile) {
+            // What a tile needs is asked for one tile ahead, its pages two, and looked at where it is used: neither a comparison nor a
+            // move of a value on its way stands between two tiles.
+            const int *table = r.table + (long long)job.sequence * r.table_stride;
+            auto entry_of = [&](int tile) {   // table entry of the tile's block of 16 tokens `lane`, in the first lanes
                 const int t = tile * kTile + 16 * lane;
-                return lane < kGroups && tile < h.last && t < end ? page_at(c, r, job.sequence, t) : -1;
+                return lane < kGroups && tile < h.last && t < end ? __ldcg(table + (t >> c.page_log2)) : -1;
             };
             uint4 x[kItems];
-            // all loads are issued before any is waited for, without branches between them
-            auto load = [&](int tile, int pages) {
-                const long long page_off = pages >= 0 ? pages * page_stride : -1;
+            float ks = 0.f, vs = 1.f;
+            bool there = false;
+            auto load = [&](int tile, int entry) {
+                there = (unsigned)entry < (unsigned)c.pages;
+                const long long page_off = there ? entry * page_stride : -1;
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
                     const int row = token + i * (128 / kChunks);
                     const long long off = __shfl_sync(0xffffffffu, page_off, row >> 4);
-                    load_if(x[i], base + off + (row & page_mask) * D, off >= 0 && tile * kTile + row < end);
+                    load_if(x[i], base + off + ((tile * kTile + row) & page_mask) * D, off >= 0 && tile * kTile + row < end);
+                }
+                if (warp == 8 && there) {
+                    ks = __ldcg(c.k_scale + entry * c.k_scale_stride + job.kv_head);
+                    vs = __ldcg(c.v_scale + entry * c.v_scale_stride + job.kv_head);
                 }
             };
-            int pages = pages_of(h.first), pages_next = pages_of(h.first + 1);
-            load(h.first, pages);
+            int entry = entry_of(h.first);
+            load(h.first, entry);
+            entry = entry_of(h.first + 1);
 #pragma unroll 1
             for (int j = h.first; j < h.last; ++j, ++n) {
-                const int stage = n & 1;
-                float4 of_lane = make_float4(0.f, -INFINITY, 0.f, 0.f);
-                if (warp == 8 && pages >= 0) {
-                    const float ks = __ldcg(c.k_scale + pages * c.k_scale_stride + job.kv_head);
-                    const float vs = value_scale(__ldcg(c.v_scale + pages * c.v_scale_stride + job.kv_head));
-                    of_lane = ks < INFINITY && vs < INFINITY ? make_float4(ks, __log2f(vs), 1.f / vs, 0.f)
-                                                             : make_float4(0.f, 1e30f, __uint_as_float(0x7fffffffu), 0.f);
-                }
-                wait(empty + stage, ((n >> 1) & 1) ^ 1, given_up);
+                const int stage = n % kStages;
+                wait(empty + stage, ((n / kStages) & 1) ^ 1, given_up);
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
@@ -527,17 +517,25 @@ prompt_kernel(const AttentionArgs a)
                     codes_to_half<E4M3>(x[i].y, lo.z, lo.w);
                     codes_to_half<E4M3>(x[i].z, hi.x, hi.y);
                     codes_to_half<E4M3>(x[i].w, hi.z, hi.w);
-                    uint8_t *at = to + stage * L::kOperand + row * 128;
+                    uint8_t *at = to + stage * L::kStage + row * 128;
                     const int first = 2 * (chunk & 3) + flip;
                     *reinterpret_cast<uint4 *>(at + ((first ^ (row & 7)) << 4)) = flip ? hi : lo;
                     *reinterpret_cast<uint4 *>(at + (((first ^ 1) ^ (row & 7)) << 4)) = flip ? lo : hi;
                 }
-                if (warp == 8 && lane < kGroups) scales[n % kConstSlots][lane] = of_lane;
+                if (warp == 8 && lane < kGroups) {
+                    const float value = value_scale(vs);
+                    float4 of_lane = make_float4(0.f, -INFINITY, 0.f, 0.f);
+                    if (there)
+                        of_lane = ks < INFINITY && value < INFINITY ? make_float4(ks, __log2f(value), __fdividef(1.f, value), 0.f)
+                                                                   : make_float4(0.f, 1e30f, __uint_as_float(0x7fffffffu), 0.f);
+                    scales[n % kConstSlots][lane] = of_lane;
+                }
                 fence_shared();
                 arrive(full + stage);
-                pages = pages_next;
-                if (j + 1 < h.last) load(j + 1, pages);
-                pages_next = pages_of(j + 2);
+                if (j + 1 < h.last) {
+                    load(j + 1, entry);
+                    entry = entry_of(j + 2);
+                }
             }
         }
     } else {
@@ -548,64 +546,61 @@ prompt_kernel(const AttentionArgs a)
             // took some 200 cycles.
             const uint32_t d_at = __shfl_sync(0xffffffffu, tmem, 0), operands = __shfl_sync(0xffffffffu, smem_address(smem), 0);
             int n = 0;
-            uint32_t q_phase = 0, p_phase = 0;    // one bit per half
+            int done0 = 0, done1 = 0;             // tiles of each half in the pieces before
+            uint32_t q_phase = 0;                 // one bit per half
             while (next_job(job, jobs, bars, job_count, given_up)) {
                 const HalfTiles &h = job.h;
                 const int first = __shfl_sync(0xffffffffu, h.first, 0), end0 = __shfl_sync(0xffffffffu, h.end[0], 0), end1 = __shfl_sync(0xffffffffu, h.end[1], 0);
                 const int last = max(end0, end1);
-                // S of the first tile, then for every tile and half: O += P V, and S of the tile behind it
+                // S of the first two tiles, then for every tile and half: O += P V, and S of the second tile behind it
 #pragma unroll 1
-                for (int j = first - 1; j < last; ++j) {
+                for (int j = first - 2; j < last; ++j) {
+                    const int tile = n + j - first, stage = tile & (kStages - 1), ahead = (tile + 2) & (kStages - 1);
+                    if (j >= first) wait(bars + kVFull + stage, (tile / kStages) & 1, given_up);
+                    if (j + 2 >= first && j + 2 < last) wait(bars + kKFull + ahead, ((tile + 2) / kStages) & 1, given_up);
 #pragma unroll 1
                     for (int w = 0; w < 2; ++w) {
-                        const int end = w ? end1 : end0;
-                        if (j >= first && j < end) {
-                            const int tile = n + j - first, stage = tile & 1;
-                            wait(bars + kPFull + w, (p_phase >> w) & 1u, given_up);
-                            p_phase ^= 1u << w;
-                            wait(bars + kVFull + stage, (tile >> 1) & 1, given_up);
-                            __syncwarp();
-                            fence_after();
-                            if (elected()) {
-                                const uint64_t v = descriptor(operands + L::kV + stage * L::kOperand, kBlockBytes, 1024);
-                                const uint32_t o = d_at + 256 + w * D, p = d_at + w * 128 + 64;
+                        const int end = w ? end1 : end0, count = (w ? done1 : done0) + j - first, buffer = 2 * w + (count & 1);
+                        const bool values = j >= first && j < end, scores = j + 2 < end;
+                        if (values) wait(bars + kPFull + buffer, (count >> 1) & 1, given_up);
+                        if (scores && j + 2 == first) {
+                            wait(bars + kQFull + w, (q_phase >> w) & 1u, given_up);
+                            q_phase ^= 1u << w;
+                        }
+                        __syncwarp();
+                        fence_after();
+                        if (elected()) {
+                            const uint32_t s = d_at + 64 * buffer;   // of this tile and of the second one behind it
+                            if (values) {
+                                const uint64_t v = descriptor(operands + L::kV + stage * L::kStage, kBlock, 1024);
+                                const uint32_t o = d_at + 256 + w * D;
 #pragma unroll
-                                for (int t = 0; t < kTile / 16; ++t) mma_ts(o, p + 8 * t, v + t * (2048 >> 4), instruction(D, true), j > first || t > 0);
-                                commit(bars + kODone + w);
+                                for (int t = 0; t < kTile / 16; ++t) mma_ts(o, s + 8 * t, v + t * (2048 >> 4), instruction(D, true), j > first || t > 0);
+                                commit(bars + kODone + buffer);
                                 if (w == (j < end1)) commit(bars + kVEmpty + stage);   // the last half that takes part
                             }
-                            __syncwarp();
-                        }
-                        if (j + 1 < end) {
-                            const int tile = n + j + 1 - first, stage = tile & 1;
-                            if (j + 1 == first) {
-                                wait(bars + kQFull + w, (q_phase >> w) & 1u, given_up);
-                                q_phase ^= 1u << w;
-                            }
-                            wait(bars + kKFull + stage, (tile >> 1) & 1, given_up);
-                            __syncwarp();
-                            fence_after();
-                            if (elected()) {
-                                const uint64_t q = descriptor(operands + L::kQ + w * L::kOperand, 16, 1024);
-                                const uint64_t k = descriptor(operands + L::kK + stage * L::kOperand, 16, 1024);
+                            if (scores) {
+                                const uint64_t q = descriptor(operands + L::kQ + w * L::kHalf, 16, 1024);
+                                const uint64_t k = descriptor(operands + L::kK + ahead * L::kStage, 16, 1024);
 #pragma unroll
-                                for (int d = 0; d < D / 16; ++d) {
-                                    const uint32_t at = ((d >> 2) * kBlockBytes + (d & 3) * 32) >> 4;
-                                    mma_ss(d_at + w * 128, q + at, k + at, instruction(kTile, false), d > 0);
-                                }
-                                commit(bars + kSFull + w);
-                                if (w == (j + 1 < end1)) commit(bars + kKEmpty + stage);
+                                for (int d = 0; d < D / 16; ++d)
+                                    mma_ss(s, q + (((d >> 2) * kQBlock + (d & 3) * 32) >> 4), k + (((d >> 2) * kBlock + (d & 3) * 32) >> 4),
+                                           instruction(kTile, false), d > 0);
+                                commit(bars + kSFull + buffer);
+                                if (w == (j + 2 < end1)) commit(bars + kKEmpty + ahead);
                             }
-                            __syncwarp();
                         }
+                        __syncwarp();
                     }
                 }
+                done0 += max(end0 - first, 0);
+                done1 += max(end1 - first, 0);
                 n += max(last - first, 0);
             }
             // all that was issued has arrived before shared and tensor memory are given back
             if (n > 0) {
                 int never = 0;
-                wait(bars + kVEmpty + ((n - 1) & 1), ((n - 1) >> 1) & 1, &never);
+                wait(bars + kVEmpty + (n - 1) % kStages, ((n - 1) / kStages) & 1, &never);
             }
             __syncwarp();
         } else if (warp == 17) {
