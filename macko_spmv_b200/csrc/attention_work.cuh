@@ -26,24 +26,24 @@ struct SplitUnit {
     int heads, unused[3];
 };
 
-// sum of floor((a * i + b) / m) for i = 0 .. n - 1
-__host__ __device__ __noinline__ inline long long floor_sum(unsigned long long n, unsigned long long m, unsigned long long a, unsigned long long b)
+// sum of floor((a * i + b) / m) for i = 0 .. n - 1; a * n + b, once a and b are below m, fits 32 bits
+__host__ __device__ __noinline__ inline long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b)
 {
     unsigned long long sum = 0;
     while (n > 0) {
         if (a >= m) {
-            sum += (n - 1) * n / 2 * (a / m);
+            sum += (unsigned long long)(n - 1) * n / 2 * (a / m);
             a %= m;
         }
         if (b >= m) {
-            sum += n * (b / m);
+            sum += (unsigned long long)n * (b / m);
             b %= m;
         }
-        const unsigned long long last = a * n + b;
+        const unsigned last = a * n + b;
         if (last < m) break;
         n = last / m;
         b = last % m;
-        const unsigned long long t = m;
+        const unsigned t = m;
         m = a;
         a = t;
     }
@@ -55,16 +55,15 @@ __host__ __device__ inline long long tiles_before(const WorkShape &w, int begin,
 {
     if (blocks == 0) return 0;
     if (blocks == 1) return ((long long)begin + w.queries + w.tile - 1) / w.tile;
-    return floor_sum(blocks, w.tile, w.queries, (unsigned long long)begin + w.queries + w.tile - 1);
+    return floor_sum(blocks, w.tile, w.queries, (unsigned)begin + w.queries + w.tile - 1);
 }
 
 #ifdef __CUDACC__
 
-// One sequence's place in the numbering.
+// One sequence's rows in blocks.
 struct SequenceWork {
     Sequence rows;
     int begin, blocks;       // begin: first position, kept inside 0 .. capacity for counting
-    long long per_head, total;
 };
 
 __device__ __forceinline__ SequenceWork sequence_work(const WorkShape &w, const RowsView &r, int i)
@@ -73,9 +72,13 @@ __device__ __forceinline__ SequenceWork sequence_work(const WorkShape &w, const 
     s.rows = sequence_at(r, i);
     s.begin = min(max(s.rows.begin(), 0), r.capacity);
     s.blocks = (s.rows.count + w.queries - 1) / w.queries;
-    s.per_head = tiles_before(w, s.begin, s.blocks);
-    s.total = s.per_head * (w.kv_heads * w.parts);
     return s;
+}
+
+__device__ __forceinline__ long long sequence_tiles(const WorkShape &w, const RowsView &r, int i)
+{
+    const SequenceWork s = sequence_work(w, r, i);
+    return tiles_before(w, s.begin, s.blocks) * (w.kv_heads * w.parts);
 }
 
 // A run of tiles of one unit, as one CTA walks it.
@@ -86,20 +89,20 @@ struct Piece {
     int pieces;              // CTAs that share the unit, counted where it begins
 };
 
-// Walks the pieces of CTA `cta`. Every thread of the block calls both functions with the same arguments; `shared`: 40 words.
+// Walks the pieces of CTA `cta`. Every thread of the block calls start(); `shared`: 40 words.
 struct WorkWalk {
     long long at, end, share;
-    long long base;          // number of the current sequence's first tile
-    int sequence;
+    int cta, sequence, head_part, block, tile;   // where the walk is; tile: of the unit
     SequenceWork s;
 
-    __device__ void start(const WorkShape &w, const RowsView &r, int cta, long long *shared)
+    __device__ void start(const WorkShape &w, const RowsView &r, int of_cta, long long *shared)
     {
+        cta = of_cta;
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (blockDim.x + 31) >> 5;
         // the total, then the sequence with this CTA's first tile
         long long total = 0, first_own = 0;
         for (int i = tid; i < r.sequences; i += blockDim.x) {
-            const long long own = sequence_work(w, r, i).total;
+            const long long own = sequence_tiles(w, r, i);
             if (i == tid) first_own = own;
             total += own;
         }
@@ -114,12 +117,11 @@ struct WorkWalk {
         at = share * cta;
         end = min(at + share, total);
         sequence = r.sequences;
-        base = 0;
         __syncthreads();
         if (at >= end) return;
         long long before = 0;
         for (int first = 0; first < r.sequences; first += blockDim.x) {
-            const long long own = first == 0 ? first_own : first + tid < r.sequences ? sequence_work(w, r, first + tid).total : 0;
+            const long long own = first == 0 ? first_own : first + tid < r.sequences ? sequence_tiles(w, r, first + tid) : 0;
             long long sum = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -147,49 +149,54 @@ struct WorkWalk {
             at = end;
             return;
         }
-        base = shared[33];
         s = sequence_work(w, r, sequence);
+        const long long local = at - shared[33], per_head = tiles_before(w, s.begin, s.blocks);
+        head_part = (int)(local / per_head);
+        const long long rest = local - head_part * per_head;
+        before = 0;
+        int lo = 0, hi = s.blocks;   // tiles_before(lo) <= rest < tiles_before(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            const long long t = tiles_before(w, s.begin, mid);
+            if (t <= rest) {
+                lo = mid;
+                before = t;
+            } else {
+                hi = mid;
+            }
+        }
+        block = lo;
+        tile = (int)(rest - before);
     }
 
     // The next piece, or false.
     __device__ bool next(const WorkShape &w, const RowsView &r, Piece &p)
     {
         if (at >= end) return false;
-        while (at >= base + s.total) {
-            base += s.total;
+        while (s.blocks == 0 || head_part >= w.kv_heads * w.parts) {
             if (++sequence >= r.sequences) return false;
             s = sequence_work(w, r, sequence);
-        }
-        const long long local = at - base;
-        const int head_part = (int)(local / s.per_head);
-        const long long rest = local - head_part * s.per_head;
-        int block = 0;
-        long long before = 0;
-        if (s.blocks > 1) {
-            int lo = 0, hi = s.blocks;   // tiles_before(lo) <= rest < tiles_before(hi)
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                const long long t = tiles_before(w, s.begin, mid);
-                if (t <= rest) {
-                    lo = mid;
-                    before = t;
-                } else {
-                    hi = mid;
-                }
-            }
-            block = lo;
+            head_part = block = tile = 0;
         }
         const int of_unit = (int)(((long long)s.begin + (long long)(block + 1) * w.queries + w.tile - 1) / w.tile);
         p.sequence = sequence;
         p.block = block;
         p.kv_head = head_part / w.parts;
         p.part = head_part % w.parts;
-        p.first_tile = (int)(rest - before);
-        p.tiles = (int)min((long long)(of_unit - p.first_tile), end - at);
-        p.begins = p.first_tile == 0;
-        p.ends = p.first_tile + p.tiles == of_unit;
-        p.pieces = p.begins ? (int)((at + of_unit - 1) / share - at / share) + 1 : 0;
+        p.first_tile = tile;
+        p.tiles = (int)min((long long)max(of_unit - tile, 0), end - at);
+        p.begins = tile == 0;
+        p.ends = tile + p.tiles >= of_unit;
+        p.pieces = p.begins ? p.ends ? 1 : (int)((at + of_unit - 1) / share - cta) + 1 : 0;
         at += p.tiles;
+        tile += p.tiles;
+        if (p.ends) {
+            tile = 0;
+            if (++block == s.blocks) {
+                block = 0;
+                ++head_part;
+            }
+        }
         return true;
     }
 };

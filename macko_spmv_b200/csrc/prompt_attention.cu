@@ -8,10 +8,10 @@
 //
 //   0, 1   softmax of one half each, one row per thread: S from tensor memory, maximum, 2^x, P as fp16 over S in tensor memory; the
 //          accumulator is rescaled there when the maximum has grown by more than 8 (so weights are at most 2^8 and none is lost)
-//   2, 3   the cache, keys and values: codes from global memory to fp16 (exact) in shared memory, in the 128-byte swizzle, four stages
-//          each, and the scales of the tile's pages
+//   2, 3   keys and values: codes from shared memory to fp16 (exact) in shared memory, in the 128-byte swizzle, three stages each
 //   4      one warp that issues tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it lies
-//          (token by token: its "N" dimension is the contiguous one); one that finds the CTA's next piece
+//          (token by token: its "N" dimension is the contiguous one); two that fetch the codes of 16 tokens at a time with bulk copies, one
+//          of them with the scales of their pages; one that finds the CTA's next piece
 //
 // Tensor memory holds two S of 64 columns and one O for each half, 512 columns at head_dim 128: S of the tile behind is there before
 // the softmax of this one is done. (With one S of 128 columns a half waited for its P to go through the tensor core and for the next S,
@@ -27,24 +27,40 @@ namespace {
 constexpr int kThreads = 640;
 constexpr int kTile = kPromptTile;
 constexpr int kGroups = kTile / 16;     // blocks of 16 tokens: each lies on one page
-constexpr int kStages = 4;              // of K, and of V
-constexpr int kConstSlots = 8;          // keys are converted at most 6 tiles ahead of the softmax
+constexpr int kStages = 3;              // of K, of V, and of the codes of each
+constexpr int kConstSlots = 16;         // scales are fetched at most 9 tiles ahead of the softmax (codes, K, S)
 constexpr float kLeastFactor = 1e-36f;  // a score times nothing is still minus infinity where it is masked
-constexpr int kWorkers = 17;            // warps that are given the CTA's pieces
+constexpr int kWorkers = 19;            // warps that are given the CTA's pieces
 
-// Shared memory, from a 1024-byte boundary: Q of both halves, K and V stages, each as [64 dimensions][rows][128 bytes].
+// Shared memory, from a 1024-byte boundary: Q of both halves, K and V stages, each as [64 dimensions][rows][128 bytes]; codes of K and V.
 template <int D> struct Layout {
-    static constexpr int kHalf = 128 * D * 2, kStage = kTile * D * 2;
-    static constexpr int kQ = 0, kK = 2 * kHalf, kV = kK + kStages * kStage, kEnd = kV + kStages * kStage;
-    static constexpr int kBytes = kEnd + 1024;
+    static constexpr int kHalf = 128 * D * 2, kStage = kTile * D * 2, kCodes = kTile * D;
+    static constexpr int kQ = 0, kK = 2 * kHalf, kV = kK + kStages * kStage, kKCodes = kV + kStages * kStage, kVCodes = kKCodes + kStages * kCodes;
+    static constexpr int kBytes = kVCodes + kStages * kCodes + 1024;
 };
 
-// Barriers with two or four in a row: of a half, of a stage, of half * 2 + S buffer, of a slot. A wait tells a phase from its neighbours
+// Barriers with several in a row: of a half, of a stage, of half * 2 + S buffer, of a slot. A wait tells a phase from its neighbours
 // only: whoever waits for one knows that the one before has come and that the one behind it needs the waiter. (So O += P V has two
 // barriers for each half as well: both of the last two products may be done before anybody asks.)
 enum Barrier {
-    kQFull = 0, kKFull = 2, kKEmpty = 6, kVFull = 10, kVEmpty = 14, kSFull = 18, kPFull = 22, kODone = 26, kJobFull = 30, kJobEmpty = 32, kBarriers = 34
+    kQFull = 0, kSFull = 2, kPFull = 6, kODone = 10, kJobFull = 14, kJobEmpty = 16, kKFull = 18, kKEmpty = 21, kVFull = 24, kVEmpty = 27,
+    kKCodesFull = 30, kKCodesEmpty = 33, kVCodesFull = 36, kVCodesEmpty = 39, kBarriers = 42
 };
+
+__device__ __forceinline__ int arrivals(int bar)
+{
+    if (bar < kSFull) return 4;                                // warps of a half
+    if (bar < kPFull) return 1;                                // commits
+    if (bar < kODone) return 4;
+    if (bar < kJobEmpty) return 1;
+    if (bar < kKFull) return kWorkers;
+    if (bar < kKEmpty) return 4;
+    if (bar < kVFull) return 1;
+    if (bar < kVEmpty) return 4;
+    if (bar < kKCodesEmpty) return 1;
+    if (bar < kVCodesFull) return 4;
+    return bar < kVCodesEmpty ? 1 : 4;
+}
 
 __device__ __forceinline__ uint32_t smem_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -73,8 +89,20 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile in
     return false;
 }
 
-// 16 bytes of global memory, or zeros.
-__device__ __forceinline__ void load_if(uint4 &x, const uint8_t *p, bool there)
+// `bytes` of global memory to shared memory; their arrival counts for the barrier.
+__device__ __forceinline__ void bulk_load(uint32_t to, const void *from, uint32_t bytes, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(to), "l"(from), "r"(bytes), "r"(smem_address(bar)) : "memory");
+}
+
+__device__ __forceinline__ void arrive_expecting(uint64_t *bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_address(bar)), "r"(bytes) : "memory");
+}
+
+// 16 bytes of global memory, or zeros; without a branch, so that many of these are under way at a time.
+__device__ __forceinline__ void load_if(uint4 &x, const void *p, bool there)
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
                  "@p ld.global.cg.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
@@ -246,6 +274,7 @@ prompt_kernel(const AttentionArgs a)
     // sees a token of such a page has a sum of NaN, and one that does not has nothing of it
     __shared__ float4 scales[kConstSlots][kGroups];
     __shared__ uint32_t tmem_base;
+    __shared__ int present[2][kConstSlots];           // of a tile of keys and of values: which of its blocks of 16 tokens lie on a page
     __shared__ Job jobs[2];
     __shared__ int given_up_word;
     volatile int *given_up = &given_up_word;
@@ -257,8 +286,7 @@ prompt_kernel(const AttentionArgs a)
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) {
         given_up_word = 0;
-        const int counts[kBarriers] = {4, 4, 4, 4, 4, 4, 1, 1, 1, 1, 4, 4, 4, 4, 1, 1, 1, 1, 1, 1, 1, 1, 4, 4, 4, 4, 1, 1, 1, 1, 1, 1, kWorkers, kWorkers};
-        for (int i = 0; i < kBarriers; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_address(bars + i)), "r"(counts[i]));
+        for (int i = 0; i < kBarriers; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_address(bars + i)), "r"(arrivals(i)));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 16) {
@@ -291,42 +319,48 @@ prompt_kernel(const AttentionArgs a)
                 const bool there = local < h.rows[half];
                 float factor = fabsf(a.scale);
                 if (h.first < h.end[half]) {
-                    // this half of Q, as fp16, with the sign of the scale
-                    const uint16_t *qp = a.q + (long long)(u.first_row + query) * a.q_row_stride + (long long)head * a.q_head_stride;
-                    uint32_t q[D / 2];
+                    // this half of Q, as fp16, with the sign of the scale: a warp its own 32 rows, some lanes a row
+                    constexpr int kLanes = D / 8, kRows = 32 / kLanes;   // lanes of a row, rows at a time
+                    const int chunk = lane % kLanes;
+                    const long long own_at = (long long)(u.first_row + query) * a.q_row_stride + (long long)head * a.q_head_stride;
+                    uint4 q[32 / kRows];
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                        if (there) v = __ldcg(reinterpret_cast<const uint4 *>(qp) + i);
-                        q[4 * i] = v.x;
-                        q[4 * i + 1] = v.y;
-                        q[4 * i + 2] = v.z;
-                        q[4 * i + 3] = v.w;
+                    for (int i = 0; i < 32 / kRows; ++i) {
+                        const int from = i * kRows + lane / kLanes;
+                        const long long at = __shfl_sync(0xffffffffu, own_at, from);
+                        load_if(q[i], a.q + at + 8 * chunk, (local & ~31) + from < h.rows[half]);
                     }
-                    if (BF16) {
-                        float most = 0.f, down, up;
+                    uint8_t *to = smem + L::kQ + half * L::kHalf + (chunk >> 3) * kQBlock;
+                    float own_up = 1.f;
 #pragma unroll
-                        for (int i = 0; i < D / 2; ++i) {
-                            const float2 f = unpack2<true>(q[i]);
-                            most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    for (int i = 0; i < 32 / kRows; ++i) {
+                        const int row_at = (local & ~31) + i * kRows + lane / kLanes;
+                        uint32_t *x = &q[i].x;
+                        if (BF16) {
+                            float most = 0.f, down, up;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float2 f = unpack2<true>(x[k]);
+                                most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+                            }
+#pragma unroll
+                            for (int o = 1; o < kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                            row_power(most, down, up);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float2 f = unpack2<true>(x[k]);
+                                x[k] = pack2<false>(f.x * down, f.y * down);
+                            }
+                            up = __shfl_sync(0xffffffffu, up, (lane % kRows) * kLanes);
+                            if (lane / kRows == i) own_up = up;
                         }
-                        row_power(most, down, up);
-                        factor *= up;
+                        if (a.scale < 0.f) {
 #pragma unroll
-                        for (int i = 0; i < D / 2; ++i) {
-                            const float2 f = unpack2<true>(q[i]);
-                            q[i] = pack2<false>(f.x * down, f.y * down);
+                            for (int k = 0; k < 4; ++k) x[k] ^= 0x80008000u;
                         }
+                        *reinterpret_cast<uint4 *>(to + row_at * 128 + (((chunk & 7) ^ (row_at & 7)) << 4)) = q[i];
                     }
-                    if (a.scale < 0.f) {
-#pragma unroll
-                        for (int i = 0; i < D / 2; ++i) q[i] ^= 0x80008000u;
-                    }
-                    uint8_t *to = smem + L::kQ + half * L::kHalf + local * 128;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        *reinterpret_cast<uint4 *>(to + (i >> 3) * kQBlock + (((i & 7) ^ (local & 7)) << 4)) =
-                            make_uint4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+                    factor *= own_up;
                     fence_shared();
                     arrive(bars + kQFull + half);
                 }
@@ -419,33 +453,51 @@ prompt_kernel(const AttentionArgs a)
                 float *partial = a.partial + ((long long)blockIdx.x * 2 + (job.begins ? 1 : 0)) * kPromptRows * (D + 2);
                 float by = alone ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 if (*given_up) by = __uint_as_float(0x7fffffffu);
+                // through this half's place for Q, which the tensor core is done with, so that some lanes write a row: 16-bit values in
+                // one pass, fp32 in two
+                const long long own_to = alone ? ((long long)(u.first_row + query) * a.heads + head) * D : (long long)row * D;
+                uint8_t *mine = smem + L::kQ + half * L::kHalf + (local >> 5) * (L::kHalf / 4);
 #pragma unroll 1
-                for (int i = 0; i < D; i += 32) {
-                    uint32_t o[32];
-                    if (!empty) {
-                        tmem_load32(o_at + i, o);
-                    } else {
+                for (int pass = 0; pass < (alone ? 1 : 2); ++pass) {
+                    __syncwarp();
+#pragma unroll 1
+                    for (int i = 0; i < (alone ? D : D / 2); i += 32) {
+                        uint32_t o[32];
+                        if (!empty) {
+                            tmem_load32(o_at + pass * (D / 2) + i, o);
+                        } else {
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = 0u;
-                    }
-                    if (there) {
+                            for (int k = 0; k < 32; ++k) o[k] = 0u;
+                        }
+                        uint8_t *at = mine + lane * (2 * D);
                         if (alone) {
-                            uint4 *to = reinterpret_cast<uint4 *>(a.out + ((long long)(u.first_row + query) * a.heads + head) * D + i);
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 uint4 v;
 #pragma unroll
                                 for (int n = 0; n < 4; ++n)
                                     (&v.x)[n] = pack2<BF16>(__uint_as_float(o[8 * k + 2 * n]) * by, __uint_as_float(o[8 * k + 2 * n + 1]) * by);
-                                to[k] = v;
+                                *reinterpret_cast<uint4 *>(at + (((i / 8 + k) ^ (lane & 7)) << 4)) = v;
                             }
                         } else {
-                            float4 *to = reinterpret_cast<float4 *>(partial + row * D + i);
 #pragma unroll
                             for (int k = 0; k < 8; ++k)
-                                to[k] = make_float4(__uint_as_float(o[4 * k]) * by, __uint_as_float(o[4 * k + 1]) * by, __uint_as_float(o[4 * k + 2]) * by,
-                                                    __uint_as_float(o[4 * k + 3]) * by);
+                                *reinterpret_cast<float4 *>(at + (((i / 4 + k) ^ (lane & 7)) << 4)) =
+                                    make_float4(__uint_as_float(o[4 * k]) * by, __uint_as_float(o[4 * k + 1]) * by, __uint_as_float(o[4 * k + 2]) * by,
+                                                __uint_as_float(o[4 * k + 3]) * by);
                         }
+                    }
+                    __syncwarp();
+                    constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+                    const int chunk = lane % kLanes;
+#pragma unroll 4
+                    for (int i = 0; i < 32; i += kRows) {
+                        const int from = i + lane / kLanes;
+                        const long long to = __shfl_sync(0xffffffffu, own_to, from);
+                        const uint4 v = *reinterpret_cast<const uint4 *>(mine + from * (2 * D) + ((chunk ^ (from & 7)) << 4));
+                        if ((local & ~31) + from >= h.rows[half]) continue;
+                        if (alone) reinterpret_cast<uint4 *>(a.out + to)[chunk] = v;
+                        else reinterpret_cast<uint4 *>(partial + to + pass * (D / 2))[chunk] = v;
                     }
                 }
                 if (there && !alone) {
@@ -456,90 +508,62 @@ prompt_kernel(const AttentionArgs a)
                     a.split[blockIdx.x] = SplitUnit{u.first_row, u.rows(), u.head, job.pieces, u.heads, {0, 0, 0}};
                 fence_before();   // O is read before this half arrives for the next piece's P
             }
+            // nobody's part of Q is written while another warp still has results there
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
             slot0 += max(h.last - h.first, 0);
         }
     } else if (group < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // Eight neighbouring threads take 16 codes each of two rows: of one its first 64 dimensions, of the other the last (at head_dim 64:
+        // all of both), so that what they read and both 16-byte pieces of what they write lie in different banks.
         const bool is_v = group == 3;
-        constexpr int kChunks = D / 16;                  // 16-byte chunks of a token
-        constexpr int kItems = kTile * kChunks / 128;    // that a thread converts
-        const int local = tid & 127, chunk = local % kChunks, token = local / kChunks;   // item i: token + i * 128 / kChunks
-        const int page_mask = (1 << c.page_log2) - 1;
-        const long long page_stride = is_v ? c.v_stride : c.k_stride;
+        constexpr int kItems = kTile * D / 16 / 128;     // that a thread converts
+        constexpr int kApart = D == 64 ? 32 : 16;        // rows between them
+        const int local = tid & 127, eight = local & 7;
+        const int row = 2 * (local >> (D == 64 ? 3 : 4)) + (eight >> 2);
+        const int chunk = D == 64 ? eight & 3 : eight ^ (((local >> 3) & 1) << 2);
         uint64_t *full = bars + (is_v ? kVFull : kKFull), *empty = bars + (is_v ? kVEmpty : kKEmpty);
-        // chunk: 16 dimensions, two 16-byte pieces of the row in block chunk / 4; odd blocks store the second one first, so that
-        // eight neighbouring threads fill all banks
-        const int flip = (chunk >> 2) & 1;
-        uint8_t *const to = smem + (is_v ? L::kV : L::kK) + (chunk >> 2) * kBlock;
-        int n = 0;                                       // tiles so far
+        uint64_t *codes_full = bars + (is_v ? kVCodesFull : kKCodesFull), *codes_empty = bars + (is_v ? kVCodesEmpty : kKCodesEmpty);
+        const uint8_t *const from = smem + (is_v ? L::kVCodes : L::kKCodes) + row * D + chunk * 16;
+        uint8_t *const to = smem + (is_v ? L::kV : L::kK) + (chunk >> 2) * kBlock + row * 128;
+        const int lo_at = ((2 * (chunk & 3)) ^ (row & 7)) << 4, hi_at = lo_at ^ 16;
+        int n = 0, stage = 0;                            // tiles so far, and modulo kStages
+        uint32_t phase = 0;
         while (next_job(job, jobs, bars, job_count, given_up)) {
-            const UnitRows &u = job.u;
             const HalfTiles &h = job.h;
-            const int end = max(0, min(u.begin + u.queries, r.capacity));   // no row sees anything from here on
-            const uint8_t *base = (is_v ? c.v : c.k) + ((long long)job.kv_head << c.page_log2) * D + 16 * chunk;
-            // What a tile needs is asked for one tile ahead, its pages two, and looked at where it is used: neither a comparison nor a
-            // move of a value on its way stands between two tiles.
-            const int *table = r.table + (long long)job.sequence * r.table_stride;
-            auto entry_of = [&](int tile) {   // table entry of the tile's block of 16 tokens `lane`, in the first lanes
-                const int t = tile * kTile + 16 * lane;
-                return lane < kGroups && tile < h.last && t < end ? __ldcg(table + (t >> c.page_log2)) : -1;
-            };
-            uint4 x[kItems];
-            float ks = 0.f, vs = 1.f;
-            bool there = false;
-            auto load = [&](int tile, int entry) {
-                there = (unsigned)entry < (unsigned)c.pages;
-                const long long page_off = there ? entry * page_stride : -1;
-#pragma unroll
-                for (int i = 0; i < kItems; ++i) {
-                    const int row = token + i * (128 / kChunks);
-                    const long long off = __shfl_sync(0xffffffffu, page_off, row >> 4);
-                    load_if(x[i], base + off + ((tile * kTile + row) & page_mask) * D, off >= 0 && tile * kTile + row < end);
-                }
-                if (warp == 8 && there) {
-                    ks = __ldcg(c.k_scale + entry * c.k_scale_stride + job.kv_head);
-                    vs = __ldcg(c.v_scale + entry * c.v_scale_stride + job.kv_head);
-                }
-            };
-            int entry = entry_of(h.first);
-            load(h.first, entry);
-            entry = entry_of(h.first + 1);
+            const int end = max(0, min(job.u.begin + job.u.queries, r.capacity));   // no row sees anything from here on
 #pragma unroll 1
             for (int j = h.first; j < h.last; ++j, ++n) {
-                const int stage = n % kStages;
-                wait(empty + stage, ((n / kStages) & 1) ^ 1, given_up);
+                wait(codes_full + stage, phase, given_up);
+                wait(empty + stage, phase ^ 1u, given_up);
                 __syncwarp();
+                const int blocks = present[is_v][n % kConstSlots];
+                const int rows = blocks == (1 << kGroups) - 1 ? end - j * kTile : -1;   // that are there, if all pages are
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
-                    const int row = token + i * (128 / kChunks);
-                    uint4 lo, hi;
-                    codes_to_half<E4M3>(x[i].x, lo.x, lo.y);
-                    codes_to_half<E4M3>(x[i].y, lo.z, lo.w);
-                    codes_to_half<E4M3>(x[i].z, hi.x, hi.y);
-                    codes_to_half<E4M3>(x[i].w, hi.z, hi.w);
-                    uint8_t *at = to + stage * L::kStage + row * 128;
-                    const int first = 2 * (chunk & 3) + flip;
-                    *reinterpret_cast<uint4 *>(at + ((first ^ (row & 7)) << 4)) = flip ? hi : lo;
-                    *reinterpret_cast<uint4 *>(at + (((first ^ 1) ^ (row & 7)) << 4)) = flip ? lo : hi;
-                }
-                if (warp == 8 && lane < kGroups) {
-                    const float value = value_scale(vs);
-                    float4 of_lane = make_float4(0.f, -INFINITY, 0.f, 0.f);
-                    if (there)
-                        of_lane = ks < INFINITY && value < INFINITY ? make_float4(ks, __log2f(value), __fdividef(1.f, value), 0.f)
-                                                                   : make_float4(0.f, 1e30f, __uint_as_float(0x7fffffffu), 0.f);
-                    scales[n % kConstSlots][lane] = of_lane;
+                    uint4 x = *reinterpret_cast<const uint4 *>(from + stage * L::kCodes + i * kApart * D), lo, hi;
+                    if (rows < kTile) {   // the same for all threads: nothing behind the last token and on pages that are none may be NaN
+                        const int at = row + i * kApart;
+                        if (!(blocks >> (at >> 4) & 1) || j * kTile + at >= end) x = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    codes_to_half<E4M3>(x.x, lo.x, lo.y);
+                    codes_to_half<E4M3>(x.y, lo.z, lo.w);
+                    codes_to_half<E4M3>(x.z, hi.x, hi.y);
+                    codes_to_half<E4M3>(x.w, hi.z, hi.w);
+                    *reinterpret_cast<uint4 *>(to + stage * L::kStage + i * kApart * 128 + lo_at) = lo;
+                    *reinterpret_cast<uint4 *>(to + stage * L::kStage + i * kApart * 128 + hi_at) = hi;
                 }
                 fence_shared();
+                arrive(codes_empty + stage);
                 arrive(full + stage);
-                if (j + 1 < h.last) {
-                    load(j + 1, entry);
-                    entry = entry_of(j + 2);
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp == 16) {
             // The whole warp walks and waits; one elected thread issues. What the instructions take is the same in all lanes in a way
             // that the compiler can see (shuffles, election), so that it stays in uniform registers: with `if (lane == 0)` an issue
@@ -555,17 +579,21 @@ prompt_kernel(const AttentionArgs a)
                 // S of the first two tiles, then for every tile and half: O += P V, and S of the second tile behind it
 #pragma unroll 1
                 for (int j = first - 2; j < last; ++j) {
-                    const int tile = n + j - first, stage = tile & (kStages - 1), ahead = (tile + 2) & (kStages - 1);
-                    if (j >= first) wait(bars + kVFull + stage, (tile / kStages) & 1, given_up);
-                    if (j + 2 >= first && j + 2 < last) wait(bars + kKFull + ahead, ((tile + 2) / kStages) & 1, given_up);
+                    const int tile = n + j - first;
+                    const unsigned use = (unsigned)max(tile, 0) / kStages, use_ahead = (unsigned)(tile + 2) / kStages;
+                    const int stage = max(tile, 0) - use * kStages, ahead = tile + 2 - use_ahead * kStages;
 #pragma unroll 1
                     for (int w = 0; w < 2; ++w) {
                         const int end = w ? end1 : end0, count = (w ? done1 : done0) + j - first, buffer = 2 * w + (count & 1);
                         const bool values = j >= first && j < end, scores = j + 2 < end;
-                        if (values) wait(bars + kPFull + buffer, (count >> 1) & 1, given_up);
+                        if (scores) wait(bars + kKFull + ahead, use_ahead & 1, given_up);
                         if (scores && j + 2 == first) {
                             wait(bars + kQFull + w, (q_phase >> w) & 1u, given_up);
                             q_phase ^= 1u << w;
+                        }
+                        if (values) {
+                            wait(bars + kVFull + stage, use & 1, given_up);
+                            wait(bars + kPFull + buffer, (count >> 1) & 1, given_up);
                         }
                         __syncwarp();
                         fence_after();
@@ -601,6 +629,57 @@ prompt_kernel(const AttentionArgs a)
             if (n > 0) {
                 int never = 0;
                 wait(bars + kVEmpty + (n - 1) % kStages, ((n - 1) / kStages) & 1, &never);
+            }
+            __syncwarp();
+        } else if (warp >= 18) {
+            // codes of keys (warp 18, with the scales of both) or of values: one lane for each block of 16 tokens, eight tiles at a time
+            const bool is_v = warp == 19;
+            uint64_t *full = bars + (is_v ? kVCodesFull : kKCodesFull), *empty = bars + (is_v ? kVCodesEmpty : kKCodesEmpty);
+            const uint32_t codes = smem_address(smem + (is_v ? L::kVCodes : L::kKCodes));
+            const int page_mask = (1 << c.page_log2) - 1, own_tile = lane / kGroups, block = lane % kGroups;
+            int n = 0, stage = 0;
+            uint32_t phase = 0;
+            asm volatile("fence.proxy.async.global;" ::: "memory");   // the cache may have been written by the kernel in front
+            while (next_job(job, jobs, bars, job_count, given_up)) {
+                const HalfTiles &h = job.h;
+                const int end = max(0, min(job.u.begin + job.u.queries, r.capacity));
+                const uint8_t *base = (is_v ? c.v : c.k) + ((long long)job.kv_head << c.page_log2) * D;
+                const long long page_stride = is_v ? c.v_stride : c.k_stride;
+#pragma unroll 1
+                for (int j0 = h.first; j0 < h.last; j0 += 32 / kGroups) {
+                    const int tile = j0 + own_tile, token = tile * kTile + 16 * block;
+                    const int page = tile < h.last && token < end ? page_at(c, r, job.sequence, token) : -1;
+                    const uint8_t *source = base + page * page_stride + (token & page_mask) * D;
+                    float4 of_lane = make_float4(0.f, -INFINITY, 0.f, 0.f);
+                    if (!is_v && page >= 0) {
+                        const float ks = __ldcg(c.k_scale + page * c.k_scale_stride + job.kv_head);
+                        const float vs = value_scale(__ldcg(c.v_scale + page * c.v_scale_stride + job.kv_head));
+                        of_lane = ks < INFINITY && vs < INFINITY ? make_float4(ks, __log2f(vs), __fdividef(1.f, vs), 0.f)
+                                                                 : make_float4(0.f, 1e30f, __uint_as_float(0x7fffffffu), 0.f);
+                    }
+                    const uint32_t all = __ballot_sync(0xffffffffu, page >= 0);
+#pragma unroll 1
+                    for (int t = 0; t < 32 / kGroups && j0 + t < h.last; ++t, ++n) {
+                        wait(empty + stage, phase ^ 1u, given_up);
+                        __syncwarp();
+                        const int blocks = (all >> (t * kGroups)) & ((1 << kGroups) - 1);
+                        if (lane == 0) present[is_v][n % kConstSlots] = blocks;
+                        if (!is_v && own_tile == t) scales[n % kConstSlots][block] = of_lane;
+                        __syncwarp();
+                        if (lane == 0) arrive_expecting(full + stage, __popc(blocks) * 16 * D);
+                        __syncwarp();
+                        if (own_tile == t && page >= 0) bulk_load(codes + stage * L::kCodes + block * 16 * D, source, 16 * D, full + stage);
+                        if (++stage == kStages) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
+                    }
+                }
+            }
+            // no copy is in flight when the CTA's shared memory is given back
+            for (int k = max(n - kStages, 0); k < n; ++k) {
+                int never = 0;
+                wait(full + k % kStages, (k / kStages) & 1, &never);
             }
             __syncwarp();
         } else if (warp == 17) {
