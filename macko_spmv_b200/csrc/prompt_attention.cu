@@ -9,9 +9,9 @@
 //   0, 1   softmax of one half each, one row per thread: S from tensor memory, maximum, 2^x, P as fp16 over S in tensor memory; the
 //          accumulator is rescaled there when the maximum has grown by more than 8 (so weights are at most 2^8 and none is lost)
 //   2, 3   keys and values: codes from shared memory to fp16 (exact) in shared memory, in the 128-byte swizzle, three stages each
-//   4      one warp that issues tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it lies
-//          (token by token: its "N" dimension is the contiguous one); two that fetch the codes of 16 tokens at a time with bulk copies, one
-//          of them with the scales of their pages; one that finds the CTA's next piece
+//   4      one warp for each half that issues its tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it
+//          lies (token by token: its "N" dimension is the contiguous one); two that fetch the codes of 16 tokens at a time with bulk
+//          copies, one of them with the scales of their pages and after finding the CTA's next piece
 //
 // Tensor memory holds two S of 64 columns and one O for each half, 512 columns at head_dim 128: S of the tile behind is there before
 // the softmax of this one is done. (With one S of 128 columns a half waited for its P to go through the tensor core and for the next S,
@@ -55,8 +55,9 @@ __device__ __forceinline__ int arrivals(int bar)
     if (bar < kJobEmpty) return 1;
     if (bar < kKFull) return kWorkers;
     if (bar < kKEmpty) return 4;
-    if (bar < kVFull) return 1;
+    if (bar < kVFull) return 2;                                // halves
     if (bar < kVEmpty) return 4;
+    if (bar < kKCodesFull) return 2;
     if (bar < kKCodesEmpty) return 1;
     if (bar < kVCodesFull) return 4;
     return bar < kVCodesEmpty ? 1 : 4;
@@ -259,6 +260,29 @@ __device__ __forceinline__ bool next_job(Job &job, const Job *jobs, uint64_t *ba
     arrive(bars + kJobEmpty + slot);
     ++count;
     return job.h.first >= 0 && !*given_up;
+}
+
+// Finds the next piece and gives it to the others, and to the caller.
+__device__ __forceinline__ bool publish_job(Job &job, Job *jobs, WorkWalk &walk, const AttentionArgs &a, uint64_t *bars, int &count, volatile int *given_up)
+{
+    Piece piece;
+    const bool more = walk.next(a.work, a.rows, piece);
+    job.h.first = -1;
+    if (more) {
+        job.u = unit_rows(a, walk.s, piece);
+        job.h = half_tiles(a, job.u, piece);
+        job.sequence = piece.sequence;
+        job.kv_head = piece.kv_head;
+        job.pieces = piece.pieces;
+        job.begins = piece.begins;
+        job.ends = piece.ends;
+    }
+    const int slot = count & 1;
+    wait(bars + kJobEmpty + slot, ((count >> 1) & 1) ^ 1, given_up);
+    if ((threadIdx.x & 31) == 0) jobs[slot] = job;
+    arrive(bars + kJobFull + slot);
+    ++count;
+    return more && !*given_up;
 }
 
 template <bool BF16, bool E4M3, int D>
@@ -564,66 +588,73 @@ prompt_kernel(const AttentionArgs a)
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 16) {
-            // The whole warp walks and waits; one elected thread issues. What the instructions take is the same in all lanes in a way
-            // that the compiler can see (shuffles, election), so that it stays in uniform registers: with `if (lane == 0)` an issue
-            // took some 200 cycles.
+        if (warp < 18) {
+            // One half's products. The whole warp walks and waits; one elected thread issues. What the instructions take is the same in all
+            // lanes in a way that the compiler can see (shuffles, election), so that it stays in uniform registers: with `if (lane == 0)`
+            // an issue took some 200 cycles. Each half has a warp of its own because a wait for what is there already takes some 150.
+            const int w = warp - 16;
             const uint32_t d_at = __shfl_sync(0xffffffffu, tmem, 0), operands = __shfl_sync(0xffffffffu, smem_address(smem), 0);
-            int n = 0;
-            int done0 = 0, done1 = 0;             // tiles of each half in the pieces before
-            uint32_t q_phase = 0;                 // one bit per half
+            const uint32_t o = d_at + 256 + w * D;
+            const uint64_t q = descriptor(operands + L::kQ + w * L::kHalf, 16, 1024);
+            int n = 0, done = 0;                  // tiles of the pieces before, and those of them that this half took part in
+            uint32_t q_phase = 0;
             while (next_job(job, jobs, bars, job_count, given_up)) {
-                const HalfTiles &h = job.h;
-                const int first = __shfl_sync(0xffffffffu, h.first, 0), end0 = __shfl_sync(0xffffffffu, h.end[0], 0), end1 = __shfl_sync(0xffffffffu, h.end[1], 0);
-                const int last = max(end0, end1);
-                // S of the first two tiles, then for every tile and half: O += P V, and S of the second tile behind it
+                const int first = __shfl_sync(0xffffffffu, job.h.first, 0), end = __shfl_sync(0xffffffffu, w ? job.h.end[1] : job.h.end[0], 0);
+                const int last = __shfl_sync(0xffffffffu, job.h.last, 0);
+                // S of the first two tiles, then for every tile: O += P V, and S of the second tile behind it. Tiles that the other half
+                // alone takes part in are let go as they come.
 #pragma unroll 1
                 for (int j = first - 2; j < last; ++j) {
-                    const int tile = n + j - first;
-                    const unsigned use = (unsigned)max(tile, 0) / kStages, use_ahead = (unsigned)(tile + 2) / kStages;
-                    const int stage = max(tile, 0) - use * kStages, ahead = tile + 2 - use_ahead * kStages;
-#pragma unroll 1
-                    for (int w = 0; w < 2; ++w) {
-                        const int end = w ? end1 : end0, count = (w ? done1 : done0) + j - first, buffer = 2 * w + (count & 1);
-                        const bool values = j >= first && j < end, scores = j + 2 < end;
-                        if (scores) wait(bars + kKFull + ahead, use_ahead & 1, given_up);
-                        if (scores && j + 2 == first) {
-                            wait(bars + kQFull + w, (q_phase >> w) & 1u, given_up);
-                            q_phase ^= 1u << w;
-                        }
-                        if (values) {
-                            wait(bars + kVFull + stage, use & 1, given_up);
-                            wait(bars + kPFull + buffer, (count >> 1) & 1, given_up);
-                        }
-                        __syncwarp();
-                        fence_after();
-                        if (elected()) {
-                            const uint32_t s = d_at + 64 * buffer;   // of this tile and of the second one behind it
-                            if (values) {
+                    const int tile = n + j - first, count = done + j - first;
+                    const uint32_t s = d_at + 128 * w + 64 * (count & 1);   // of this tile and of the second one behind it
+                    if (j >= first) {
+                        const unsigned use = (unsigned)tile / kStages;
+                        const int stage = tile - use * kStages;
+                        wait(bars + kVFull + stage, use & 1, given_up);
+                        if (j < end) {
+                            wait(bars + kPFull + 2 * w + (count & 1), (count >> 1) & 1, given_up);
+                            __syncwarp();
+                            fence_after();
+                            if (elected()) {
                                 const uint64_t v = descriptor(operands + L::kV + stage * L::kStage, kBlock, 1024);
-                                const uint32_t o = d_at + 256 + w * D;
 #pragma unroll
                                 for (int t = 0; t < kTile / 16; ++t) mma_ts(o, s + 8 * t, v + t * (2048 >> 4), instruction(D, true), j > first || t > 0);
-                                commit(bars + kODone + buffer);
-                                if (w == (j < end1)) commit(bars + kVEmpty + stage);   // the last half that takes part
+                                commit(bars + kODone + 2 * w + (count & 1));
+                                commit(bars + kVEmpty + stage);
                             }
-                            if (scores) {
-                                const uint64_t q = descriptor(operands + L::kQ + w * L::kHalf, 16, 1024);
-                                const uint64_t k = descriptor(operands + L::kK + ahead * L::kStage, 16, 1024);
+                            __syncwarp();
+                        } else {
+                            arrive(bars + kVEmpty + stage);
+                        }
+                    }
+                    if (j + 2 < last) {
+                        const unsigned use = (unsigned)(tile + 2) / kStages;
+                        const int stage = tile + 2 - use * kStages;
+                        wait(bars + kKFull + stage, use & 1, given_up);
+                        if (j + 2 < end) {
+                            if (j + 2 == first) {
+                                wait(bars + kQFull + w, q_phase, given_up);
+                                q_phase ^= 1u;
+                            }
+                            __syncwarp();
+                            fence_after();
+                            if (elected()) {
+                                const uint64_t k = descriptor(operands + L::kK + stage * L::kStage, 16, 1024);
 #pragma unroll
                                 for (int d = 0; d < D / 16; ++d)
                                     mma_ss(s, q + (((d >> 2) * kQBlock + (d & 3) * 32) >> 4), k + (((d >> 2) * kBlock + (d & 3) * 32) >> 4),
                                            instruction(kTile, false), d > 0);
-                                commit(bars + kSFull + buffer);
-                                if (w == (j + 2 < end1)) commit(bars + kKEmpty + ahead);
+                                commit(bars + kSFull + 2 * w + (count & 1));
+                                commit(bars + kKEmpty + stage);
                             }
+                            __syncwarp();
+                        } else {
+                            arrive(bars + kKEmpty + stage);
                         }
-                        __syncwarp();
                     }
                 }
-                done0 += max(end0 - first, 0);
-                done1 += max(end1 - first, 0);
                 n += max(last - first, 0);
+                done += max(end - first, 0);
             }
             // all that was issued has arrived before shared and tensor memory are given back
             if (n > 0) {
@@ -631,7 +662,7 @@ prompt_kernel(const AttentionArgs a)
                 wait(bars + kVEmpty + (n - 1) % kStages, ((n - 1) / kStages) & 1, &never);
             }
             __syncwarp();
-        } else if (warp >= 18) {
+        } else {
             // codes of keys (warp 18, with the scales of both) or of values: one lane for each block of 16 tokens, eight tiles at a time
             const bool is_v = warp == 19;
             uint64_t *full = bars + (is_v ? kVCodesFull : kKCodesFull), *empty = bars + (is_v ? kVCodesEmpty : kKCodesEmpty);
@@ -640,7 +671,7 @@ prompt_kernel(const AttentionArgs a)
             int n = 0, stage = 0;
             uint32_t phase = 0;
             asm volatile("fence.proxy.async.global;" ::: "memory");   // the cache may have been written by the kernel in front
-            while (next_job(job, jobs, bars, job_count, given_up)) {
+            while (is_v ? next_job(job, jobs, bars, job_count, given_up) : publish_job(job, jobs, walk, a, bars, job_count, given_up)) {
                 const HalfTiles &h = job.h;
                 const int end = max(0, min(job.u.begin + job.u.queries, r.capacity));
                 const uint8_t *base = (is_v ? c.v : c.k) + ((long long)job.kv_head << c.page_log2) * D;
@@ -682,26 +713,6 @@ prompt_kernel(const AttentionArgs a)
                 wait(full + k % kStages, (k / kStages) & 1, &never);
             }
             __syncwarp();
-        } else if (warp == 17) {
-            Piece piece;
-            for (bool more = true; more; ++job_count) {
-                more = walk.next(a.work, r, piece);
-                wait(bars + kJobEmpty + (job_count & 1), ((job_count >> 1) & 1) ^ 1, given_up);
-                if (lane == 0) {
-                    job.h.first = -1;
-                    if (more) {
-                        job.u = unit_rows(a, walk.s, piece);
-                        job.h = half_tiles(a, job.u, piece);
-                        job.sequence = piece.sequence;
-                        job.kv_head = piece.kv_head;
-                        job.pieces = piece.pieces;
-                        job.begins = piece.begins;
-                        job.ends = piece.ends;
-                    }
-                    jobs[job_count & 1] = job;
-                }
-                arrive(bars + kJobFull + (job_count & 1));
-            }
         }
     }
     fence_before();
