@@ -89,69 +89,60 @@ struct Piece {
     int pieces;              // CTAs that share the unit, counted where it begins
 };
 
-// Walks the pieces of CTA `cta`. Every thread of the block calls start(); `shared`: 40 words.
+__device__ __forceinline__ long long quotient(long long a, long long b)   // of numbers that are not negative; most fit 32 bits
+{
+    return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
+// Walks the pieces of CTA `cta`. All lanes of a warp call start(); next() is each thread's own.
 struct WorkWalk {
     long long at, end, share;
     int cta, sequence, head_part, block, tile;   // where the walk is; tile: of the unit
     SequenceWork s;
 
-    __device__ void start(const WorkShape &w, const RowsView &r, int of_cta, long long *shared)
+    __device__ void start(const WorkShape &w, const RowsView &r, int of_cta)
     {
+        const int lane = threadIdx.x & 31;
         cta = of_cta;
-        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (blockDim.x + 31) >> 5;
         // the total, then the sequence with this CTA's first tile
         long long total = 0, first_own = 0;
-        for (int i = tid; i < r.sequences; i += blockDim.x) {
+        for (int i = lane; i < r.sequences; i += 32) {
             const long long own = sequence_tiles(w, r, i);
-            if (i == tid) first_own = own;
+            if (i == lane) first_own = own;
             total += own;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (lane == 0) shared[warp] = total;
-        if (tid == 0) shared[32] = r.sequences;
-        __syncthreads();
-        total = 0;
-        for (int v = 0; v < warps; ++v) total += shared[v];
-        share = max((total + w.ctas - 1) / w.ctas, (long long)w.least_share);
+        share = max(quotient(total + w.ctas - 1, w.ctas), (long long)w.least_share);
         at = share * cta;
         end = min(at + share, total);
         sequence = r.sequences;
-        __syncthreads();
         if (at >= end) return;
-        long long before = 0;
-        for (int first = 0; first < r.sequences; first += blockDim.x) {
-            const long long own = first == 0 ? first_own : first + tid < r.sequences ? sequence_tiles(w, r, first + tid) : 0;
+        long long before = 0, base = 0;
+        for (int first = 0; first < r.sequences; first += 32) {
+            const long long own = first == 0 ? first_own : first + lane < r.sequences ? sequence_tiles(w, r, first + lane) : 0;
             long long sum = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long v = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += v;
             }
-            if (lane == 31) shared[warp] = sum;
-            __syncthreads();
-            long long all = 0;
-            for (int v = 0; v < warps; ++v) {
-                if (v < warp) sum += shared[v];
-                all += shared[v];
-            }
             const long long lo = before + sum - own;
-            if (at >= lo && at < lo + own) {
-                shared[32] = first + tid;
-                shared[33] = lo;
+            const uint32_t here = __ballot_sync(0xffffffffu, at >= lo && at < lo + own);
+            if (here != 0) {
+                sequence = first + __ffs(here) - 1;
+                base = __shfl_sync(0xffffffffu, lo, __ffs(here) - 1);
+                break;
             }
-            before += all;
-            __syncthreads();
-            if (at < before) break;
+            before += __shfl_sync(0xffffffffu, sum, 31);
         }
-        sequence = (int)shared[32];
         if (sequence >= r.sequences) {   // the lengths have changed under the call: nothing outside the arrays is read for that
             at = end;
             return;
         }
         s = sequence_work(w, r, sequence);
-        const long long local = at - shared[33], per_head = tiles_before(w, s.begin, s.blocks);
-        head_part = (int)(local / per_head);
+        const long long local = at - base, per_head = tiles_before(w, s.begin, s.blocks);
+        head_part = (int)quotient(local, max(per_head, 1ll));
         const long long rest = local - head_part * per_head;
         before = 0;
         int lo = 0, hi = s.blocks;   // tiles_before(lo) <= rest < tiles_before(hi)
@@ -187,7 +178,7 @@ struct WorkWalk {
         p.tiles = (int)min((long long)max(of_unit - tile, 0), end - at);
         p.begins = tile == 0;
         p.ends = tile + p.tiles >= of_unit;
-        p.pieces = p.begins ? p.ends ? 1 : (int)((at + of_unit - 1) / share - cta) + 1 : 0;
+        p.pieces = p.begins ? p.ends ? 1 : (int)(quotient(at + of_unit - 1, share) - cta) + 1 : 0;
         at += p.tiles;
         tile += p.tiles;
         if (p.ends) {

@@ -73,7 +73,6 @@ few_rows_kernel(const AttentionArgs a)
     constexpr int KC = D / 64;              // 16-byte chunks of a key that a lane holds
     constexpr int VB = D / 8;               // bytes of a value that a lane holds
     constexpr int DT = D / 16;              // blocks of 16 dimensions
-    __shared__ long long found[40];
     extern __shared__ __align__(16) float merge[];   // [warps][RB][D], then maxima and sums [warps][RB]
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -87,7 +86,7 @@ few_rows_kernel(const AttentionArgs a)
     bool more;
     if (a.split != nullptr) {
         if (tid == 0) a.split[blockIdx.x].pieces = 0;
-        walk.start(a.work, r, blockIdx.x, found);
+        walk.start(a.work, r, blockIdx.x);
         more = walk.next(a.work, r, piece);
     } else {
         // one unit per CTA: sequences of one row each
@@ -482,6 +481,65 @@ join_kernel(const AttentionArgs a)
     }
 }
 
+// The same for units of many rows, which lie in two or three CTAs: a warp has four rows at a time.
+template <bool BF16, int D>
+__global__ void __launch_bounds__(512)
+join_many_kernel(const AttentionArgs a)
+{
+    constexpr int V = D / 32, R = 4;
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 *at = reinterpret_cast<const int4 *>(a.split + blockIdx.x);
+    const int4 s = __ldcg(at);   // first row, rows, head, pieces
+    const int unit_heads = __ldcg(at + 1).x, lane = threadIdx.x & 31;
+    const int row0 = (blockIdx.y * 16 + (threadIdx.x >> 5)) * R;
+    if (s.w == 0 || row0 >= s.y) return;
+    const int stride = a.unit_rows * (D + 2);
+    float m[R], l[R], o[R][V];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[i][j] = 0.f;
+    }
+    for (int p = 0; p < s.w; ++p) {
+        // the first piece is the second result of its CTA, the others are the first of theirs; rows behind the unit's have whatever
+        // was there: they are not written
+        const float *from = a.partial + ((long long)(blockIdx.x + p) * 2 + (p == 0)) * stride;
+        float pm[R], pl[R], po[R][V];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            pm[i] = __ldcg(from + a.unit_rows * D + row0 + i);
+            pl[i] = __ldcg(from + a.unit_rows * D + a.unit_rows + row0 + i);
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                const float2 x = __ldcg(reinterpret_cast<const float2 *>(from + (row0 + i) * D + lane * V + j));
+                po[i][j] = x.x;
+                po[i][j + 1] = x.y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const float most = fmaxf(m[i], pm[i]), base = most == -INFINITY ? 0.f : most;
+            const float keep = exp2_fast(m[i] - base), f = exp2_fast(pm[i] - base);
+            m[i] = most;
+            l[i] = l[i] * keep + f * pl[i];
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[i][j] = o[i][j] * keep + f * po[i][j];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int row = row0 + i;
+        if (row >= s.y) break;
+        const float inverse = l[i] == 0.f ? 0.f : 1.f / l[i];
+        uint16_t *to = a.out + ((long long)(s.x + row / unit_heads) * a.heads + s.z + row % unit_heads) * D + lane * V;
+#pragma unroll
+        for (int j = 0; j < V; j += 2) *reinterpret_cast<uint32_t *>(to + j) = pack2<BF16>(o[i][j] * inverse, o[i][j + 1] * inverse);
+    }
+}
+
 int check_sizes(const macko_kv_cache *cache, const macko_kv_rows *batch, int heads, AttentionArgs *a)
 {
     if (int st = check_cache("paged_attention", cache, &a->cache)) return st;
@@ -527,7 +585,7 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
         l->ctas = (int)units;
     }
     l->work.ctas = l->ctas;
-    l->join_rows = !prompt && units < l->ctas / 4 ? rows : rows / 8;
+    l->join_rows = units < l->ctas / 4 ? rows : rows / 8;
     l->split_bytes = l->split ? (int64_t)l->ctas * sizeof(SplitUnit) : 0;
     l->partial_bytes = l->split ? (int64_t)l->ctas * 2 * rows * (d + 2) * 4 : 0;
     return MACKO_OK;
@@ -560,7 +618,7 @@ int launch_rows(const AttentionArgs &a, const Launch &l, cudaStream_t s)
     if constexpr (D <= 128) {
         if (l.unit_rows == kPromptRows) {
             if (int st = launch_prompt_attention(a, BF16, E4M3, s)) return st;
-            return launch_join<BF16, D>(a, l, s);
+            return launch_pdl("paged_attention", join_many_kernel<BF16, D>, dim3(l.ctas, kPromptRows / 64), dim3(512), 1, 0, s, a);
         }
     }
     return l.unit_rows == 8 ? launch_few<BF16, E4M3, D, 8>(a, l, s) : launch_few<BF16, E4M3, D, 16>(a, l, s);

@@ -292,7 +292,6 @@ prompt_kernel(const AttentionArgs a)
     using L = Layout<D>;
     constexpr uint32_t kQBlock = 128 * 128, kBlock = kTile * 128;   // 64 dimensions of Q, and of K or V
     extern __shared__ uint8_t raw[];
-    __shared__ long long found[40];
     __shared__ __align__(8) uint64_t bars[kBarriers];
     // of 16 tokens: scale of the keys, log2 and inverse of the values'. A scale that is not finite becomes (0, 1e30, NaN): a row that
     // sees a token of such a page has a sum of NaN, and one that does not has nothing of it
@@ -319,8 +318,6 @@ prompt_kernel(const AttentionArgs a)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (tid == 0) a.split[blockIdx.x].pieces = 0;
-    WorkWalk walk;
-    walk.start(a.work, r, blockIdx.x, found);
     fence_before();
     __syncthreads();
     fence_after();
@@ -670,6 +667,8 @@ prompt_kernel(const AttentionArgs a)
             const int page_mask = (1 << c.page_log2) - 1, own_tile = lane / kGroups, block = lane % kGroups;
             int n = 0, stage = 0;
             uint32_t phase = 0;
+            WorkWalk walk;
+            if (!is_v) walk.start(a.work, r, blockIdx.x);
             asm volatile("fence.proxy.async.global;" ::: "memory");   // the cache may have been written by the kernel in front
             while (is_v ? next_job(job, jobs, bars, job_count, given_up) : publish_job(job, jobs, walk, a, bars, job_count, given_up)) {
                 const HalfTiles &h = job.h;
