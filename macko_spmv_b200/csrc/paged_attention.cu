@@ -21,6 +21,7 @@ namespace macko {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kAhead = 1;   // turns of a warp between asking for its tokens and loading them
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -41,19 +42,17 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
 template <int BYTES> struct Codes { uint32_t w[BYTES / 4]; };
 
 template <int BYTES>
-__device__ __forceinline__ Codes<BYTES> load_codes(const uint8_t *p, bool there)
+__device__ __forceinline__ Codes<BYTES> load_codes(const uint8_t *p)
 {
     Codes<BYTES> c;
     if (BYTES == 8) {
-        uint2 v = make_uint2(0u, 0u);
-        if (there) v = __ldcg(reinterpret_cast<const uint2 *>(p));
+        const uint2 v = __ldcg(reinterpret_cast<const uint2 *>(p));
         c.w[0] = v.x;
         c.w[1] = v.y;
     } else {
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (there) v = __ldcg(reinterpret_cast<const uint4 *>(p) + i);
+            const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(p) + i);
             c.w[4 * i] = v.x;
             c.w[4 * i + 1] = v.y;
             c.w[4 * i + 2] = v.z;
@@ -61,6 +60,21 @@ __device__ __forceinline__ Codes<BYTES> load_codes(const uint8_t *p, bool there)
         }
     }
     return c;
+}
+
+template <int BYTES>
+__device__ __forceinline__ Codes<BYTES> no_codes()
+{
+    Codes<BYTES> c;
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) c.w[i] = 0u;
+    return c;
+}
+
+// Has `bytes` of global memory brought to the L2 cache.
+__device__ __forceinline__ void prefetch(const void *p, int bytes)
+{
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
 template <bool BF16, bool E4M3, int D, int RB>
@@ -179,32 +193,53 @@ few_rows_kernel(const AttentionArgs a)
                 vs_of_lane = value_scale(__ldcg(c.v_scale + page_of_lane * c.v_scale_stride + piece.kv_head));
             }
         };
-        auto load_k = [&](int token, int index, int mt) {
+        // `whole`: all of the warp's tokens are there
+        auto load_k = [&](int token, int index, int mt, bool whole) {
             const int page = __shfl_sync(0xffffffffu, page_of_lane, index * MT + mt);
-            const uint8_t *base = c.k + page * c.k_stride + head_at + (long long)((token + mt * 16) & page_mask) * D + 16 * t;
+            const uint8_t *base = c.k + page * c.k_stride + head_at + (long long)((token + mt * 16) & page_mask) * D + 16 * t + g * D;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int ch = 0; ch < KC; ++ch)
-                    kc[mt][h][ch] = load_codes<16>(base + (g + 8 * h) * D + 64 * ch, page >= 0 && token + mt * 16 + g + 8 * h < end);
+                for (int ch = 0; ch < KC; ++ch) {
+                    if (whole || (page >= 0 && token + mt * 16 + g + 8 * h < end)) kc[mt][h][ch] = load_codes<16>(base + 8 * h * D + 64 * ch);
+                    else kc[mt][h][ch] = no_codes<16>();
+                }
         };
-        auto load_v = [&](int token, int index, int mt) {
+        auto load_v = [&](int token, int index, int mt, bool whole) {
             const int page = __shfl_sync(0xffffffffu, page_of_lane, index * MT + mt);
-            const uint8_t *base = c.v + page * c.v_stride + head_at + (long long)((token + mt * 16) & page_mask) * D + VB * g;
+            const uint8_t *base = c.v + page * c.v_stride + head_at + (long long)((token + mt * 16) & page_mask) * D + VB * g + 2 * t * D;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = 2 * t + (i & 1) + 8 * (i >> 1);
-                vc[mt][i] = load_codes<VB>(base + row * D, page >= 0 && token + mt * 16 + row < end);
+                const int row = (i & 1) + 8 * (i >> 1);
+                if (whole || (page >= 0 && token + mt * 16 + 2 * t + row < end)) vc[mt][i] = load_codes<VB>(base + row * D);
+                else vc[mt][i] = no_codes<VB>();
+            }
+        };
+        auto is_whole = [&](int token, int index) {
+            const bool there = __all_sync(0xffffffffu, page_of_lane >= 0 || lane / MT != index);
+            return there && token + 16 * MT <= end;
+        };
+        // the warp's tokens `ahead` turns on, K and V, to the L2 cache: the registers hold no more than one turn, and a load from memory
+        // takes longer than a turn
+        auto ask = [&](int token, int index) {
+            const int mt = lane % MT, at = token + mt * 16;
+            const int page = __shfl_sync(0xffffffffu, page_of_lane, (index * MT + mt) & 31);
+            if (lane < 2 * MT && index * MT < 32 && page >= 0 && at < end) {
+                const long long off = head_at + (long long)(at & page_mask) * D;
+                prefetch(lane < MT ? c.k + page * c.k_stride + off : c.v + page * c.v_stride + off, 16 * D);
             }
         };
         constexpr int kPerFetch = 32 / MT;
         int index = 0;
         if (first < stop) {
             fetch_pages(first);
+            const bool whole = is_whole(first, 0);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) load_k(first, 0, mt);
+            for (int mt = 0; mt < MT; ++mt) load_k(first, 0, mt, whole);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) load_v(first, 0, mt);
+            for (int mt = 0; mt < MT; ++mt) load_v(first, 0, mt, whole);
+#pragma unroll
+            for (int i = 1; i <= kAhead; ++i) ask(first + i * kTile, i);
         }
         for (int token = first; token < stop; token += kTile) {
             float x[MT][NB][4], inverse[MT];
@@ -240,9 +275,17 @@ few_rows_kernel(const AttentionArgs a)
                 index = 0;
                 fetch_pages(next);
             }
+            bool next_whole = false;
             if (go_on) {
+                next_whole = is_whole(next, index);
+                if (next_whole) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) load_k(next, index, mt);
+                    for (int mt = 0; mt < MT; ++mt) load_k(next, index, mt, true);
+                } else {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) load_k(next, index, mt, false);
+                }
+                ask(next + kAhead * kTile, index + kAhead);
             }
 
             float top[NB][2];
@@ -317,9 +360,12 @@ few_rows_kernel(const AttentionArgs a)
                         for (int nb = 0; nb < NB; ++nb) mma(o[2 * w + half][nb], a0, a1, a2, a3, p[mt][nb][0], p[mt][nb][1]);
                     }
                 }
-            if (go_on) {
+            if (next_whole) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) load_v(next, index, mt);
+                for (int mt = 0; mt < MT; ++mt) load_v(next, index, mt, true);
+            } else if (go_on) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) load_v(next, index, mt, false);
             }
         }
 
