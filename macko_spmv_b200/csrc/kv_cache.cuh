@@ -93,22 +93,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
 // The scale of a page's values as the softmax counts it: NaN stays NaN.
 __device__ __forceinline__ float value_scale(float scale) { return scale < kLowestScale ? kLowestScale : scale; }
 
-// Two e4m3 codes (the low half of `codes`) as two fp16 values, exactly.
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint16_t codes)
-{
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(codes));
-    return h;
-}
-
 // Four codes, as they lie in memory, as two pairs of fp16 values, exactly. int8: the byte with its sign bit flipped, put under
 // the exponent of 1024, is 1024 + 128 + code; 1152 is taken off again.
 template <bool E4M3>
 __device__ __forceinline__ void codes_to_half(uint32_t codes, uint32_t &lo, uint32_t &hi)
 {
     if (E4M3) {
-        lo = e4m3x2_to_half2((uint16_t)(codes & 0xffffu));
-        hi = e4m3x2_to_half2((uint16_t)(codes >> 16));
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(codes));
     } else {
         const uint32_t x = codes ^ 0x80808080u;
         const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
