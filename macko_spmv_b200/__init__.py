@@ -453,7 +453,11 @@ def multiply_batched(compressed_M, V):
     return torch.ops.macko_spmv.multiply_batched.default(*compressed_M[:5], V)
 
 
-from .kv_cache import KVCache, new_cache, paged_attention, rope_append  # noqa: E402  (needs the loaded operators)
+from . import kv_cache as _kv_cache  # noqa: E402  (needs the loaded operators)
+from .kv_cache import KVCache, new_cache, paged_attention, rope_append  # noqa: E402
+
+if _direct is not None:
+    _kv_cache._direct_append, _kv_cache._direct_attention = _direct.rope_append, _direct.paged_attention
 
 __all__ = ["KVCache", "new_cache", "rope_append", "paged_attention", "compress", "multiply", "multiply_batched", "decompress", "move_to_device", "freeze", "rows_are_even", "FrozenMatrix",
            "native_library_paths", "native_version", "LIB_NAME"]

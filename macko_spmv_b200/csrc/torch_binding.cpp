@@ -588,9 +588,9 @@ at::Tensor paged_attention_cuda(const at::Tensor &q, const at::Tensor &k_cache, 
     const int64_t bytes = macko_cache_attention_workspace_bytes(rows.sequences, rows.rows, rows.table_width, (int32_t)heads, cache.kv_heads,
                                                                 cache.page_size, cache.head_dim, rows.query_start == nullptr);
     TORCH_CHECK(bytes >= 0, "macko_cache_attention_workspace_bytes: ", macko_last_error());
-    const at::Tensor workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+    const at::Tensor workspace = bytes > 0 ? at::empty({bytes}, q.options().dtype(at::kByte)) : at::Tensor();
     check_status(macko_cache_attention(&cache, &rows, q.data_ptr(), row_stride, head_stride, type, out.data_ptr(), (int32_t)heads,
-                                       (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)hd)), workspace.data_ptr(), bytes,
+                                       (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)hd)), bytes > 0 ? workspace.data_ptr() : nullptr, bytes,
                                        c10::cuda::getCurrentCUDAStream()),
                  "macko_cache_attention");
     return out;

@@ -1,4 +1,5 @@
-// `multiply` and the batched product of a frozen matrix without the operator dispatcher, a Python module beside the operator library.
+// `multiply`, the batched product of a frozen matrix and the operators of the paged cache without the operator dispatcher, a Python module
+// beside the operator library.
 //
 // A product of a small matrix takes less time on the GPU than the way of its arguments through the operator boundary
 // (Python asserts, schema matching, boxing). The module function below takes that way out for calls that only
@@ -161,6 +162,75 @@ PyObject *direct_multiply_batched(PyObject *, PyObject *const *args, Py_ssize_t 
     END_HANDLE_TH_ERRORS
 }
 
+// The four tensors of a cache if it is a tuple of plain ones.
+bool plain_cache(PyObject *o, at::Tensor (&cache)[4])
+{
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+    for (int i = 0; i < 4; ++i) {
+        const at::Tensor *t = plain_tensor(PyTuple_GET_ITEM(o, i));
+        if (!t) return false;
+        cache[i] = *t;
+    }
+    return true;
+}
+
+// A tensor or None.
+bool plain_or_none(PyObject *o, std::optional<at::Tensor> &t)
+{
+    if (o == Py_None) return true;
+    const at::Tensor *p = plain_tensor(o);
+    if (p) t = *p;
+    return p != nullptr;
+}
+
+// rope_append(qkv, cos_table, sin_table, cache, page_table, lengths, query_start) -> q, or None where the call has to go through the operator
+PyObject *direct_rope_append(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    HANDLE_TH_ERRORS
+    at::Tensor cache[4];
+    std::optional<at::Tensor> start;
+    if (n_args != 7 || !nobody_watches() || !plain_cache(args[3], cache) || !plain_or_none(args[6], start)) Py_RETURN_NONE;
+    const at::Tensor *in[5] = {plain_tensor(args[0]), plain_tensor(args[1]), plain_tensor(args[2]), plain_tensor(args[4]), plain_tensor(args[5])};
+    for (const at::Tensor *t : in)
+        if (!t) Py_RETURN_NONE;
+    const at::Tensor qkv = *in[0], cos = *in[1], sin = *in[2], table = *in[3], lengths = *in[4];
+    at::Tensor q;
+    {
+        struct NoGil { PyThreadState *s = PyEval_SaveThread(); ~NoGil() { PyEval_RestoreThread(s); } } no_gil;
+        q = macko_torch::rope_append_cuda(qkv, cos, sin, cache[0], cache[1], cache[2], cache[3], table, lengths, start);
+    }
+    // PyTorch counts writes: so that whoever saved the cache for a backward pass hears of this one
+    for (at::Tensor &t : cache)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    return THPVariable_Wrap(std::move(q));
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, cache, page_table, lengths, query_start, scale) -> out, or None where the call has to go through the operator
+PyObject *direct_paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n_args)
+{
+    HANDLE_TH_ERRORS
+    at::Tensor cache[4];
+    std::optional<at::Tensor> start;
+    std::optional<double> scale;
+    if (n_args != 6 || !nobody_watches() || !plain_cache(args[1], cache) || !plain_or_none(args[4], start)) Py_RETURN_NONE;
+    if (args[5] != Py_None) {
+        if (!PyFloat_CheckExact(args[5])) Py_RETURN_NONE;
+        scale = PyFloat_AS_DOUBLE(args[5]);
+    }
+    const at::Tensor *in[3] = {plain_tensor(args[0]), plain_tensor(args[2]), plain_tensor(args[3])};
+    for (const at::Tensor *t : in)
+        if (!t) Py_RETURN_NONE;
+    const at::Tensor q = *in[0], table = *in[1], lengths = *in[2];
+    at::Tensor out;
+    {
+        struct NoGil { PyThreadState *s = PyEval_SaveThread(); ~NoGil() { PyEval_RestoreThread(s); } } no_gil;
+        out = macko_torch::paged_attention_cuda(q, cache[0], cache[1], cache[2], cache[3], table, lengths, start, scale);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 // set_frozen_type(FrozenMatrix): the class that `freeze` returns
 PyObject *set_frozen_type(PyObject *, PyObject *type)
 {
@@ -172,6 +242,8 @@ PyObject *set_frozen_type(PyObject *, PyObject *type)
 PyMethodDef g_methods[] = {
     {"multiply", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&direct_multiply)), METH_FASTCALL, nullptr},
     {"multiply_batched", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&direct_multiply_batched)), METH_FASTCALL, nullptr},
+    {"rope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&direct_rope_append)), METH_FASTCALL, nullptr},
+    {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&direct_paged_attention)), METH_FASTCALL, nullptr},
     {"set_frozen_type", &set_frozen_type, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_direct", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

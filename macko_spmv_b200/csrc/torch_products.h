@@ -1,4 +1,4 @@
-// The products of torch_binding.cpp as functions: what the operators `multiply` / `multiply_frozen` / `multiply_planned`
+// The products and the cache operators of torch_binding.cpp as functions: what the operators of their names
 // do on CUDA tensors, with all their checks. torch_direct.cpp calls them without the operator dispatcher.
 #pragma once
 

@@ -22,6 +22,17 @@ from typing import NamedTuple
 import torch
 
 
+_is_compiling = torch.compiler.is_compiling
+
+
+def _direct_append(*args):
+    """The way past the operator dispatcher, where the package has it (see `multiply`); None: through the operator."""
+
+
+def _direct_attention(*args):
+    """The same for `paged_attention`."""
+
+
 class KVCache(NamedTuple):
     """Codes of the keys and values and their scales. Any tuple of the four tensors is taken where one is asked for; pages may
     be strided (k and v as halves of one tensor, say), what is inside a page is contiguous."""
@@ -58,6 +69,10 @@ def rope_append(qkv, cos_table, sin_table, cache, page_table, lengths, query_sta
 
     A page may be read by many sequences but written for one: calls that write the same page must not overlap on the GPU, and the
     rows of one call must not share a page between sequences."""
+    if not _is_compiling():
+        q = _direct_append(qkv, cos_table, sin_table, cache, page_table, lengths, query_start)   # None: not a plain call
+        if q is not None:
+            return q
     k, v, k_scale, v_scale = cache
     return torch.ops.macko_spmv.rope_append.default(qkv, cos_table, sin_table, k, v, k_scale, v_scale, page_table, lengths, query_start)
 
@@ -68,5 +83,9 @@ def paged_attention(q, cache, page_table, lengths, query_start=None, scale=None)
     q [rows, heads, head_dim], fp16 or bfloat16, rotated (heads and rows may be strided); heads must be a multiple of the cache's, and head h reads
     the cache's head h // (heads // kv_heads). scale: 1 / sqrt(head_dim) if None. A row that sees no token (an empty sequence, rows of no
     sequence) gives zeros. Sums and the softmax are kept in fp32; the weights of the values are rounded to fp16 on the way."""
+    if not _is_compiling():
+        out = _direct_attention(q, cache, page_table, lengths, query_start, scale)   # None: not a plain call
+        if out is not None:
+            return out
     k, v, k_scale, v_scale = cache
     return torch.ops.macko_spmv.paged_attention.default(q, k, v, k_scale, v_scale, page_table, lengths, query_start, scale)
