@@ -18,8 +18,8 @@ struct AttentionArgs {
     float scale;             // times log2 e
 };
 
-// Rows per unit of the kernel for many rows, and its launch (no join): prompt_attention.cu. head_dim 64 or 128.
-constexpr int kPromptRows = 256;
+// Rows per unit of the kernel for many rows, and its launch (no join): prompt_attention.cu.
+constexpr int prompt_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
 constexpr int kPromptTile = 64;
 int launch_prompt_attention(const AttentionArgs &a, bool bf16, bool e4m3, cudaStream_t stream);
 

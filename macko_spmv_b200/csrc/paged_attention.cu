@@ -599,7 +599,7 @@ int check_sizes(const macko_kv_cache *cache, const macko_kv_rows *batch, int hea
 // Which launch runs, and what it keeps in the workspace: host arithmetic on sizes alone.
 struct Launch {
     WorkShape work;
-    int unit_rows;      // 8 or 16, or kPromptRows: the kernel for many rows
+    int unit_rows;      // 8 or 16; 128 or more: the kernel for many rows
     int ctas, smem;
     bool split;
     int join_rows;      // blocks per split unit
@@ -612,8 +612,8 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     const bool one_each = a.rows.start == nullptr;
     // rows that a head of the cache meets in a sequence, as far as the host knows: on average
     const int64_t mean = one_each ? group : ((int64_t)a.rows.rows * group + a.rows.sequences - 1) / (a.rows.sequences > 0 ? a.rows.sequences : 1);
-    const bool prompt = !one_each && mean > 16 && d <= 128;
-    const int rows = prompt ? kPromptRows : mean <= 8 ? 8 : 16;
+    const bool prompt = !one_each && mean > 16;
+    const int rows = prompt ? prompt_rows(d) : mean <= 8 ? 8 : 16;
     l->unit_rows = rows;
     l->work.heads = group < rows ? group : rows;
     l->work.parts = (group + l->work.heads - 1) / l->work.heads;
@@ -661,11 +661,9 @@ int launch_few(const AttentionArgs &a, const Launch &l, cudaStream_t s)
 template <bool BF16, bool E4M3, int D>
 int launch_rows(const AttentionArgs &a, const Launch &l, cudaStream_t s)
 {
-    if constexpr (D <= 128) {
-        if (l.unit_rows == kPromptRows) {
-            if (int st = launch_prompt_attention(a, BF16, E4M3, s)) return st;
-            return launch_pdl("paged_attention", join_many_kernel<BF16, D>, dim3(l.ctas, kPromptRows / 64), dim3(512), 1, 0, s, a);
-        }
+    if (l.unit_rows >= 128) {
+        if (int st = launch_prompt_attention(a, BF16, E4M3, s)) return st;
+        return launch_pdl("paged_attention", join_many_kernel<BF16, D>, dim3(l.ctas, l.unit_rows / 64), dim3(512), 1, 0, s, a);
     }
     return l.unit_rows == 8 ? launch_few<BF16, E4M3, D, 8>(a, l, s) : launch_few<BF16, E4M3, D, 16>(a, l, s);
 }

@@ -27,16 +27,31 @@ namespace {
 constexpr int kThreads = 640;
 constexpr int kTile = kPromptTile;
 constexpr int kGroups = kTile / 16;     // blocks of 16 tokens: each lies on one page
-constexpr int kStages = 3;              // of K, of V, and of the codes of each
 constexpr int kConstSlots = 16;         // scales are fetched at most 9 tiles ahead of the softmax (codes, K, S)
 constexpr float kLeastFactor = 1e-36f;  // a score times nothing is still minus infinity where it is masked
 constexpr int kWorkers = 19;            // warps that are given the CTA's pieces
 
-// Shared memory, from a 1024-byte boundary: Q of both halves, K and V stages, each as [64 dimensions][rows][128 bytes]; codes of K and V.
+// Shared memory, from a 1024-byte boundary: Q of the halves, K and V stages, each as [64 dimensions][rows][128 bytes]; codes of K and V.
+// At head_dim 256 O takes 256 columns of tensor memory: units have one half, and there is room for two stages and for one of codes.
 template <int D> struct Layout {
+    static constexpr int kHalves = D == 256 ? 1 : 2, kRows = 128 * kHalves;
+    static constexpr int kStages = D == 256 ? 2 : 3, kCodeStages = D == 256 ? 1 : 3;
     static constexpr int kHalf = 128 * D * 2, kStage = kTile * D * 2, kCodes = kTile * D;
-    static constexpr int kQ = 0, kK = 2 * kHalf, kV = kK + kStages * kStage, kKCodes = kV + kStages * kStage, kVCodes = kKCodes + kStages * kCodes;
-    static constexpr int kBytes = kVCodes + kStages * kCodes + 1024;
+    static constexpr int kQ = 0, kK = kHalves * kHalf, kV = kK + kStages * kStage, kKCodes = kV + kStages * kStage, kVCodes = kKCodes + kCodeStages * kCodes;
+    static constexpr int kBytes = kVCodes + kCodeStages * kCodes + 1024;
+};
+
+// A place in a ring of N and how often it has been around, modulo 2.
+template <int N> struct Ring {
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next()
+    {
+        if (++stage == N) {
+            stage = 0;
+            phase ^= 1u;
+        }
+    }
 };
 
 // Barriers with several in a row: of a half, of a stage, of half * 2 + S buffer, of a slot. A wait tells a phase from its neighbours
@@ -290,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 prompt_kernel(const AttentionArgs a)
 {
     using L = Layout<D>;
+    constexpr int kStages = L::kStages;
     constexpr uint32_t kQBlock = 128 * 128, kBlock = kTile * 128;   // 64 dimensions of Q, and of K or V
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t bars[kBarriers];
@@ -321,7 +337,7 @@ prompt_kernel(const AttentionArgs a)
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = tmem_base;   // columns: two S of 64 of half 0 and of half 1, O of half 0 and 1 (D each)
+    const uint32_t tmem = tmem_base;   // columns: two S of 64 of half 0 and of half 1, O of the halves (D each)
     Job job;
     int job_count = 0;
 
@@ -344,42 +360,46 @@ prompt_kernel(const AttentionArgs a)
                     constexpr int kLanes = D / 8, kRows = 32 / kLanes;   // lanes of a row, rows at a time
                     const int chunk = lane % kLanes;
                     const long long own_at = (long long)(u.first_row + query) * a.q_row_stride + (long long)head * a.q_head_stride;
-                    uint4 q[32 / kRows];
-#pragma unroll
-                    for (int i = 0; i < 32 / kRows; ++i) {
-                        const int from = i * kRows + lane / kLanes;
-                        const long long at = __shfl_sync(0xffffffffu, own_at, from);
-                        load_if(q[i], a.q + at + 8 * chunk, (local & ~31) + from < h.rows[half]);
-                    }
                     uint8_t *to = smem + L::kQ + half * L::kHalf + (chunk >> 3) * kQBlock;
                     float own_up = 1.f;
+                    constexpr int kBatch = 8;                            // loads under way
+#pragma unroll 1
+                    for (int b = 0; b < 32 / kRows; b += kBatch) {
+                        uint4 q[kBatch];
 #pragma unroll
-                    for (int i = 0; i < 32 / kRows; ++i) {
-                        const int row_at = (local & ~31) + i * kRows + lane / kLanes;
-                        uint32_t *x = &q[i].x;
-                        if (BF16) {
-                            float most = 0.f, down, up;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float2 f = unpack2<true>(x[k]);
-                                most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
-                            }
-#pragma unroll
-                            for (int o = 1; o < kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                            row_power(most, down, up);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float2 f = unpack2<true>(x[k]);
-                                x[k] = pack2<false>(f.x * down, f.y * down);
-                            }
-                            up = __shfl_sync(0xffffffffu, up, (lane % kRows) * kLanes);
-                            if (lane / kRows == i) own_up = up;
+                        for (int i = 0; i < kBatch; ++i) {
+                            const int from = (b + i) * kRows + lane / kLanes;
+                            const long long at = __shfl_sync(0xffffffffu, own_at, from);
+                            load_if(q[i], a.q + at + 8 * chunk, (local & ~31) + from < h.rows[half]);
                         }
-                        if (a.scale < 0.f) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) x[k] ^= 0x80008000u;
+                        for (int i = 0; i < kBatch; ++i) {
+                            const int row_at = (local & ~31) + (b + i) * kRows + lane / kLanes;
+                            uint32_t *x = &q[i].x;
+                            if (BF16) {
+                                float most = 0.f, down, up;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const float2 f = unpack2<true>(x[k]);
+                                    most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+                                }
+#pragma unroll
+                                for (int o = 1; o < kLanes; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                                row_power(most, down, up);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const float2 f = unpack2<true>(x[k]);
+                                    x[k] = pack2<false>(f.x * down, f.y * down);
+                                }
+                                up = __shfl_sync(0xffffffffu, up, (lane % kRows) * kLanes);
+                                if (lane / kRows == b + i) own_up = up;
+                            }
+                            if (a.scale < 0.f) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) x[k] ^= 0x80008000u;
+                            }
+                            *reinterpret_cast<uint4 *>(to + row_at * 128 + (((chunk & 7) ^ (row_at & 7)) << 4)) = q[i];
                         }
-                        *reinterpret_cast<uint4 *>(to + row_at * 128 + (((chunk & 7) ^ (row_at & 7)) << 4)) = q[i];
                     }
                     factor *= own_up;
                     fence_shared();
@@ -471,7 +491,7 @@ prompt_kernel(const AttentionArgs a)
                     fence_after();
                 }
                 const bool alone = job.begins && job.ends, empty = h.first >= h.end[half];
-                float *partial = a.partial + ((long long)blockIdx.x * 2 + (job.begins ? 1 : 0)) * kPromptRows * (D + 2);
+                float *partial = a.partial + ((long long)blockIdx.x * 2 + (job.begins ? 1 : 0)) * L::kRows * (D + 2);
                 float by = alone ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 if (*given_up) by = __uint_as_float(0x7fffffffu);
                 // through this half's place for Q, which the tensor core is done with, so that some lanes write a row: 16-bit values in
@@ -522,8 +542,8 @@ prompt_kernel(const AttentionArgs a)
                     }
                 }
                 if (there && !alone) {
-                    partial[kPromptRows * D + row] = m;
-                    partial[kPromptRows * D + kPromptRows + row] = l;
+                    partial[L::kRows * D + row] = m;
+                    partial[L::kRows * D + L::kRows + row] = l;
                 }
                 if (!alone && job.begins && row == 0)
                     a.split[blockIdx.x] = SplitUnit{u.first_row, u.rows(), u.head, job.pieces, u.heads, {0, 0, 0}};
@@ -535,34 +555,35 @@ prompt_kernel(const AttentionArgs a)
         }
     } else if (group < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        // Eight neighbouring threads take 16 codes each of two rows: of one its first 64 dimensions, of the other the last (at head_dim 64:
-        // all of both), so that what they read and both 16-byte pieces of what they write lie in different banks.
+        // Eight neighbouring threads take 16 codes each of two rows: of one the first 64 of 128 dimensions, of the other the last (at
+        // head_dim 64: all of both), so that what they read and both 16-byte pieces of what they write lie in different banks.
         const bool is_v = group == 3;
         constexpr int kItems = kTile * D / 16 / 128;     // that a thread converts
-        constexpr int kApart = D == 64 ? 32 : 16;        // rows between them
+        constexpr int kApart = D == 64 ? 32 : D == 128 ? 16 : 8;        // rows between them
         const int local = tid & 127, eight = local & 7;
-        const int row = 2 * (local >> (D == 64 ? 3 : 4)) + (eight >> 2);
-        const int chunk = D == 64 ? eight & 3 : eight ^ (((local >> 3) & 1) << 2);
+        const int row = 2 * (local >> (D == 64 ? 3 : D == 128 ? 4 : 5)) + (eight >> 2);
+        const int chunk = D == 64 ? eight & 3 : (eight ^ (((local >> 3) & 1) << 2)) + (D == 256 ? ((local >> 4) & 1) * 8 : 0);
         uint64_t *full = bars + (is_v ? kVFull : kKFull), *empty = bars + (is_v ? kVEmpty : kKEmpty);
         uint64_t *codes_full = bars + (is_v ? kVCodesFull : kKCodesFull), *codes_empty = bars + (is_v ? kVCodesEmpty : kKCodesEmpty);
         const uint8_t *const from = smem + (is_v ? L::kVCodes : L::kKCodes) + row * D + chunk * 16;
         uint8_t *const to = smem + (is_v ? L::kV : L::kK) + (chunk >> 2) * kBlock + row * 128;
         const int lo_at = ((2 * (chunk & 3)) ^ (row & 7)) << 4, hi_at = lo_at ^ 16;
-        int n = 0, stage = 0;                            // tiles so far, and modulo kStages
-        uint32_t phase = 0;
+        int n = 0;                                       // tiles so far
+        Ring<L::kStages> ring;
+        Ring<L::kCodeStages> codes_ring;
         while (next_job(job, jobs, bars, job_count, given_up)) {
             const HalfTiles &h = job.h;
             const int end = max(0, min(job.u.begin + job.u.queries, r.capacity));   // no row sees anything from here on
 #pragma unroll 1
             for (int j = h.first; j < h.last; ++j, ++n) {
-                wait(codes_full + stage, phase, given_up);
-                wait(empty + stage, phase ^ 1u, given_up);
+                wait(codes_full + codes_ring.stage, codes_ring.phase, given_up);
+                wait(empty + ring.stage, ring.phase ^ 1u, given_up);
                 __syncwarp();
                 const int blocks = present[is_v][n % kConstSlots];
                 const int rows = blocks == (1 << kGroups) - 1 ? end - j * kTile : -1;   // that are there, if all pages are
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
-                    uint4 x = *reinterpret_cast<const uint4 *>(from + stage * L::kCodes + i * kApart * D), lo, hi;
+                    uint4 x = *reinterpret_cast<const uint4 *>(from + codes_ring.stage * L::kCodes + i * kApart * D), lo, hi;
                     if (rows < kTile) {   // the same for all threads: nothing behind the last token and on pages that are none may be NaN
                         const int at = row + i * kApart;
                         if (!(blocks >> (at >> 4) & 1) || j * kTile + at >= end) x = make_uint4(0u, 0u, 0u, 0u);
@@ -571,16 +592,14 @@ prompt_kernel(const AttentionArgs a)
                     codes_to_half<E4M3>(x.y, lo.z, lo.w);
                     codes_to_half<E4M3>(x.z, hi.x, hi.y);
                     codes_to_half<E4M3>(x.w, hi.z, hi.w);
-                    *reinterpret_cast<uint4 *>(to + stage * L::kStage + i * kApart * 128 + lo_at) = lo;
-                    *reinterpret_cast<uint4 *>(to + stage * L::kStage + i * kApart * 128 + hi_at) = hi;
+                    *reinterpret_cast<uint4 *>(to + ring.stage * L::kStage + i * kApart * 128 + lo_at) = lo;
+                    *reinterpret_cast<uint4 *>(to + ring.stage * L::kStage + i * kApart * 128 + hi_at) = hi;
                 }
                 fence_shared();
-                arrive(codes_empty + stage);
-                arrive(full + stage);
-                if (++stage == kStages) {
-                    stage = 0;
-                    phase ^= 1u;
-                }
+                arrive(codes_empty + codes_ring.stage);
+                arrive(full + ring.stage);
+                ring.next();
+                codes_ring.next();
             }
         }
     } else {
@@ -665,8 +684,8 @@ prompt_kernel(const AttentionArgs a)
             uint64_t *full = bars + (is_v ? kVCodesFull : kKCodesFull), *empty = bars + (is_v ? kVCodesEmpty : kKCodesEmpty);
             const uint32_t codes = smem_address(smem + (is_v ? L::kVCodes : L::kKCodes));
             const int page_mask = (1 << c.page_log2) - 1, own_tile = lane / kGroups, block = lane % kGroups;
-            int n = 0, stage = 0;
-            uint32_t phase = 0;
+            int n = 0;
+            Ring<L::kCodeStages> ring;
             WorkWalk walk;
             if (!is_v) walk.start(a.work, r, blockIdx.x);
             asm volatile("fence.proxy.async.global;" ::: "memory");   // the cache may have been written by the kernel in front
@@ -687,29 +706,29 @@ prompt_kernel(const AttentionArgs a)
                         of_lane = ks < INFINITY && vs < INFINITY ? make_float4(ks, __log2f(vs), __fdividef(1.f, vs), 0.f)
                                                                  : make_float4(0.f, 1e30f, __uint_as_float(0x7fffffffu), 0.f);
                     }
+                    // with one stage of codes the way from memory would be a part of every tile: from the L2 cache it is a short one
+                    if (L::kCodeStages == 1 && page >= 0)
+                        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(source), "r"(16 * D) : "memory");
                     const uint32_t all = __ballot_sync(0xffffffffu, page >= 0);
 #pragma unroll 1
                     for (int t = 0; t < 32 / kGroups && j0 + t < h.last; ++t, ++n) {
-                        wait(empty + stage, phase ^ 1u, given_up);
+                        wait(empty + ring.stage, ring.phase ^ 1u, given_up);
                         __syncwarp();
                         const int blocks = (all >> (t * kGroups)) & ((1 << kGroups) - 1);
                         if (lane == 0) present[is_v][n % kConstSlots] = blocks;
                         if (!is_v && own_tile == t) scales[n % kConstSlots][block] = of_lane;
                         __syncwarp();
-                        if (lane == 0) arrive_expecting(full + stage, __popc(blocks) * 16 * D);
+                        if (lane == 0) arrive_expecting(full + ring.stage, __popc(blocks) * 16 * D);
                         __syncwarp();
-                        if (own_tile == t && page >= 0) bulk_load(codes + stage * L::kCodes + block * 16 * D, source, 16 * D, full + stage);
-                        if (++stage == kStages) {
-                            stage = 0;
-                            phase ^= 1u;
-                        }
+                        if (own_tile == t && page >= 0) bulk_load(codes + ring.stage * L::kCodes + block * 16 * D, source, 16 * D, full + ring.stage);
+                        ring.next();
                     }
                 }
             }
             // no copy is in flight when the CTA's shared memory is given back
-            for (int k = max(n - kStages, 0); k < n; ++k) {
+            for (int k = max(n - L::kCodeStages, 0); k < n; ++k) {
                 int never = 0;
-                wait(full + k % kStages, (k / kStages) & 1, &never);
+                wait(full + k % L::kCodeStages, (k / L::kCodeStages) & 1, &never);
             }
             __syncwarp();
         }
@@ -746,7 +765,11 @@ int launch_types(const AttentionArgs &a, bool bf16, bool e4m3, cudaStream_t s)
 
 int launch_prompt_attention(const AttentionArgs &a, bool bf16, bool e4m3, cudaStream_t stream)
 {
-    return a.cache.head_dim == 64 ? launch_types<64>(a, bf16, e4m3, stream) : launch_types<128>(a, bf16, e4m3, stream);
+    switch (a.cache.head_dim) {
+    case 64: return launch_types<64>(a, bf16, e4m3, stream);
+    case 128: return launch_types<128>(a, bf16, e4m3, stream);
+    default: return launch_types<256>(a, bf16, e4m3, stream);
+    }
 }
 
 }  // namespace macko
