@@ -90,6 +90,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     return raw;
 }
 
+// 16 bytes of global memory, or zeros; without a branch, so that many of these are under way at a time.
+__device__ __forceinline__ void load_if(uint4 &x, const void *p, bool there)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                 "@p ld.global.cg.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "=&r"(x.x), "=&r"(x.y), "=&r"(x.z), "=&r"(x.w) : "l"(p), "r"((int)there));
+}
+
 // The scale of a page's values as the softmax counts it: NaN stays NaN.
 __device__ __forceinline__ float value_scale(float scale) { return scale < kLowestScale ? kLowestScale : scale; }
 

@@ -117,14 +117,6 @@ __device__ __forceinline__ void arrive_expecting(uint64_t *bar, uint32_t bytes)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_address(bar)), "r"(bytes) : "memory");
 }
 
-// 16 bytes of global memory, or zeros; without a branch, so that many of these are under way at a time.
-__device__ __forceinline__ void load_if(uint4 &x, const void *p, bool there)
-{
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-                 "@p ld.global.cg.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
-                 : "=&r"(x.x), "=&r"(x.y), "=&r"(x.z), "=&r"(x.w) : "l"(p), "r"((int)there));
-}
-
 __device__ __forceinline__ bool elected()
 {
     uint32_t yes;

@@ -22,7 +22,7 @@ namespace macko {
 namespace {
 
 constexpr int kItems = 4;         // pairs of 8 dimensions, D/2 apart, that a thread of a page's block holds
-constexpr int kQueryItems = 2;    // the same for a thread that rotates q
+constexpr int kQueryItems = 4;    // the same for a thread that rotates q
 
 struct AppendArgs {
     CacheView cache;
@@ -32,6 +32,7 @@ struct AppendArgs {
     uint16_t *q;
     long long row_stride;
     int heads, units, page_blocks;
+    int query_items;   // of a thread that rotates q: 1 or kQueryItems
 };
 
 // Page `unit` of those that the call's rows fall on, in the order of the sequences: the rows on it and where they go.
@@ -127,55 +128,66 @@ rope_append_kernel(const AppendArgs a)
     const int hq = a.heads, hkv = c.kv_heads;
 
     if ((int)blockIdx.x >= a.page_blocks) {
-        // q: blocks over (row, head, part of the head); the sequence of the block's first row by counting, the others' from there
-        const long long items = (long long)r.rows * hq * kPerRow;
-        const long long base = (long long)((int)blockIdx.x - a.page_blocks) * blockDim.x * kQueryItems;
-        const int row0 = (int)(base / (hq * kPerRow));
-        int seq0 = row0;
+        // q: blocks over (row, head, part of the head). The sequence of the block's first row is looked for by all threads at once, in one
+        // way to memory; the others' rows are nearly always its own.
+        const long long base = (long long)((int)blockIdx.x - a.page_blocks) * blockDim.x * a.query_items / kPerRow;   // row and head
+        const int row0 = (int)(base / hq), head0 = (int)(base % hq);
         if (r.start != nullptr) {
-            int n = 0;
-            for (int i = 1 + tid; i <= r.sequences; i += blockDim.x) n += __ldcg(r.start + i) <= row0;
-            if (tid == 0) found[0] = 0;
+            if (tid == 0) found[0] = r.sequences;
             __syncthreads();
-            n = __reduce_add_sync(0xffffffffu, n);
-            if ((tid & 31) == 0 && n) atomicAdd(found, n);
+            for (int i = tid; i < r.sequences; i += blockDim.x) {
+                const Sequence s = sequence_at(r, i);
+                if (row0 >= s.first && row0 < s.first + s.count) {
+                    found[0] = i;
+                    found[1] = s.first;
+                    found[2] = s.count;
+                    found[3] = s.length;
+                }
+            }
             __syncthreads();
-            seq0 = found[0];
+        }
+        uint4 lo[kQueryItems], hi[kQueryItems], co[kQueryItems], si[kQueryItems];
+        long long to[kQueryItems];   // in q, or -1
+#pragma unroll
+        for (int i = 0; i < kQueryItems; ++i) {
+            if (i >= a.query_items) break;
+            const int item = i * (int)blockDim.x + tid, part = item % kPerRow, row_head = head0 + item / kPerRow;
+            const int row = row0 + row_head / hq, head = row_head % hq;
+            int position = -1;
+            if (row < r.rows) {
+                Sequence s = {0, 0, 0};
+                if (r.start == nullptr) {
+                    s = sequence_at(r, row);
+                } else {
+                    int seq = found[0];
+                    if (seq < r.sequences) s = Sequence{found[1], found[2], found[3]};
+                    else seq = -1;
+                    while (row >= s.first + s.count && ++seq < r.sequences) s = sequence_at(r, seq);
+                }
+                if (row >= s.first && row < s.first + s.count) position = s.begin() + row - s.first;
+            }
+            const bool there = position >= 0 && position < r.capacity;
+            to[i] = row < r.rows ? ((long long)row * hq + head) * D + 8 * part : -1;
+            const uint16_t *x = a.qkv + (long long)row * a.row_stride + head * D + 8 * part;
+            const long long at = (long long)position * D + 8 * part;
+            load_if(lo[i], x, there);
+            load_if(hi[i], x + D / 2, there);
+            load_if(co[i], a.cos_table + at, there);
+            load_if(si[i], a.sin_table + at, there);
         }
 #pragma unroll
         for (int i = 0; i < kQueryItems; ++i) {
-            const long long item = base + i * (int)blockDim.x + tid;
-            if (item >= items) break;
-            const int part = (int)(item % kPerRow);
-            const long long row_head = item / kPerRow;
-            const int row = (int)(row_head / hq), head = (int)(row_head % hq);
-            int seq = seq0;
-            if (r.start != nullptr) {
-                while (seq < r.sequences && __ldcg(r.start + seq + 1) <= row) ++seq;
-            } else {
-                seq = row;
-            }
-            int position = -1;
-            if (seq < r.sequences) {
-                const Sequence s = sequence_at(r, seq);
-                if (row >= s.first && row < s.first + s.count) position = s.begin() + row - s.first;
-            }
-            uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-            if (position >= 0 && position < r.capacity) {
-                const uint16_t *x = a.qkv + (long long)row * a.row_stride + head * D + 8 * part;
-                const long long at = (long long)position * D + 8 * part;
-                float y[16];
-                rotate<BF16>(__ldcg(reinterpret_cast<const uint4 *>(x)), __ldcg(reinterpret_cast<const uint4 *>(x + D / 2)),
-                             __ldg(reinterpret_cast<const uint4 *>(a.cos_table + at)), __ldg(reinterpret_cast<const uint4 *>(a.sin_table + at)), y);
+            if (i >= a.query_items) break;
+            float y[16];
+            rotate<BF16>(lo[i], hi[i], co[i], si[i], y);
+            if (to[i] < 0) continue;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    (&lo.x)[j] = pack2<BF16>(y[2 * j], y[2 * j + 1]);
-                    (&hi.x)[j] = pack2<BF16>(y[8 + 2 * j], y[8 + 2 * j + 1]);
-                }
+            for (int j = 0; j < 4; ++j) {
+                (&lo[i].x)[j] = pack2<BF16>(y[2 * j], y[2 * j + 1]);
+                (&hi[i].x)[j] = pack2<BF16>(y[8 + 2 * j], y[8 + 2 * j + 1]);
             }
-            uint16_t *out = a.q + row_head * D + 8 * part;
-            *reinterpret_cast<uint4 *>(out) = lo;
-            *reinterpret_cast<uint4 *>(out + D / 2) = hi;
+            *reinterpret_cast<uint4 *>(a.q + to[i]) = lo[i];
+            *reinterpret_cast<uint4 *>(a.q + to[i] + D / 2) = hi[i];
         }
         return;
     }
@@ -191,31 +203,39 @@ rope_append_kernel(const AppendArgs a)
     float *scale = is_v ? c.v_scale + (long long)page * c.v_scale_stride + head : c.k_scale + (long long)page * c.k_scale_stride + head;
     const float old = slot > 0 ? __ldcg(scale) : 0.f;
 
+    const int rows_apart = (int)blockDim.x / kPerRow;   // between a thread's items
+    uint4 lo[kItems], hi[kItems], co[kItems], si[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        if (i * rows_apart >= rows.count) break;
+        const int item = i * (int)blockDim.x + tid, row = item / kPerRow, part = item % kPerRow;
+        const bool there = row < rows.count;
+        const uint16_t *x = a.qkv + (long long)(rows.first_row + row) * a.row_stride + (hq + (is_v ? hkv : 0) + head) * D + 8 * part;
+        const long long at = (long long)(rows.position + row) * D + 8 * part;
+        load_if(lo[i], x, there);
+        load_if(hi[i], x + D / 2, there);
+        load_if(co[i], a.cos_table + at, there && !is_v);
+        load_if(si[i], a.sin_table + at, there && !is_v);
+    }
     float y[kItems][16];
     uint32_t most = 0u;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-        const int item = i * (int)blockDim.x + tid, row = item / kPerRow, part = item % kPerRow;
-        if (row < rows.count) {
-            const uint16_t *x = a.qkv + (long long)(rows.first_row + row) * a.row_stride + (hq + (is_v ? hkv : 0) + head) * D + 8 * part;
-            const uint4 lo = __ldcg(reinterpret_cast<const uint4 *>(x)), hi = __ldcg(reinterpret_cast<const uint4 *>(x + D / 2));
-            if (is_v) {
+        if (i * rows_apart >= rows.count) break;
+        if (is_v) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 l = unpack2<BF16>((&lo.x)[j]), h = unpack2<BF16>((&hi.x)[j]);
-                    y[i][2 * j] = l.x;
-                    y[i][2 * j + 1] = l.y;
-                    y[i][8 + 2 * j] = h.x;
-                    y[i][8 + 2 * j + 1] = h.y;
-                }
-            } else {
-                const long long at = (long long)(rows.position + row) * D + 8 * part;
-                rotate<BF16>(lo, hi, __ldg(reinterpret_cast<const uint4 *>(a.cos_table + at)),
-                             __ldg(reinterpret_cast<const uint4 *>(a.sin_table + at)), y[i]);
+            for (int j = 0; j < 4; ++j) {
+                const float2 l = unpack2<BF16>((&lo[i].x)[j]), h = unpack2<BF16>((&hi[i].x)[j]);
+                y[i][2 * j] = l.x;
+                y[i][2 * j + 1] = l.y;
+                y[i][8 + 2 * j] = h.x;
+                y[i][8 + 2 * j + 1] = h.y;
             }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) most = max(most, __float_as_uint(y[i][j]) & 0x7fffffffu);
+        } else {
+            rotate<BF16>(lo[i], hi[i], co[i], si[i], y[i]);
         }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) most = max(most, __float_as_uint(y[i][j]) & 0x7fffffffu);
     }
     most = __reduce_max_sync(0xffffffffu, most);
     if ((tid & 31) == 0) largest[tid >> 5] = most;
@@ -244,6 +264,7 @@ rope_append_kernel(const AppendArgs a)
     const float inverse = finite ? 1.f / now : 0.f;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
+        if (i * rows_apart >= rows.count) break;
         const int item = i * (int)blockDim.x + tid, row = item / kPerRow, part = item % kPerRow;
         if (row < rows.count) {
             uint2 out[2];
@@ -344,8 +365,11 @@ extern "C" int macko_cache_rope_append(const macko_kv_cache *cache, const macko_
     const int64_t pages = a.rows.rows / page + 2 * (int64_t)a.rows.sequences;
     a.units = (int)(a.rows.rows < pages ? a.rows.rows : pages);
     const int64_t page_blocks = a.rows.sequences > 0 ? (int64_t)a.units * cache->kv_heads * 2 : 0;
-    const int64_t per_block = (int64_t)threads * kQueryItems;
-    const int64_t q_blocks = ((int64_t)a.rows.rows * heads * (d / 16) + per_block - 1) / per_block;
+    // one item a thread where all of them fit the GPU at once (64 rows of 32 + 8 heads of 128: 3.4 us for the whole call),
+    // else four items a thread, whose loads are under way together (8192 rows: 46 us, 54 with two)
+    a.query_items = (int64_t)a.rows.rows * heads * (d / 16) <= 148 * 1024 ? 1 : kQueryItems;
+    const int64_t per_block = (int64_t)threads * a.query_items;
+    const int64_t q_blocks = ((int64_t)a.rows.rows * heads * (d / 16) + per_block - 1) / per_block;   // per_block: whole heads
     if (page_blocks + q_blocks > INT_MAX)
         return fail(MACKO_ERR_SIZE_OVERFLOW, "rope_append: rows=%d heads=%d need too many blocks", a.rows.rows, heads);
     a.page_blocks = (int)page_blocks;
