@@ -23,6 +23,12 @@ The decode step runs the code between the products as three kernels of this pack
 (`torch.ops.macko_spmv.add_rmsnorm`, `rope_attention`, `silu_mul`: residual add + RMSNorm, rotary embedding +
 KV-cache append + attention, SwiGLU gate), eight launches per block in all, for MACKO and dense layers alike;
 `LlamaDecoder(..., fused_glue=False)` and `Block.forward` keep the same step in plain PyTorch operators.
+
+Cache in 8 bits: `LlamaDecoder(..., cache_dtype=torch.int8 or torch.float8_e4m3fn, sequences=B)` keeps the keys and values of B sequences in
+paged caches (`kv_cache`), half the bytes of the fp16 ones. A block then runs `rope_append` and `paged_attention` in the place of `rope_attention`,
+for prompts as well, and `extend` takes rows of several sequences in one pass: whole prompts, pieces of them, and single tokens side by side.
+
+    python -m macko_spmv_b200.llama_decode --density 0.5 --cache fp8 --sequences 16
 """
 from __future__ import annotations
 
@@ -36,6 +42,7 @@ import torch
 from torch import nn
 
 from . import compress, workloads
+from .kv_cache import new_cache, paged_attention, rope_append
 from .linear import ColumnShardedMackoLinear, MackoLinear, RowShardedMackoLinear
 
 LLAMA2_7B = dict(hidden=4096, heads=32, ffn=11008, vocab=32000, layers=32, eps=1e-5, rope_theta=10000.0)
@@ -100,7 +107,7 @@ class Block(nn.Module):
     """One transformer block. q/k/v and gate/up are stored as one matrix each (rows concatenated), so a
     token costs four SpMVs per block; the glue around them is kept to a handful of kernels."""
 
-    def __init__(self, cfg, density, seed, device, max_len, peer=None):
+    def __init__(self, cfg, density, seed, device, max_len, peer=None, cache_pages=0, page_size=32, cache_dtype=None):
         super().__init__()
         h, f = cfg["hidden"], cfg["ffn"]
         world = peer.world if peer is not None else 1
@@ -121,6 +128,10 @@ class Block(nn.Module):
             self.down_proj = _tp_linear(h, f, density, seed + 6, device, peer, "cols")
         self.input_norm = RMSNorm(h, cfg["eps"], device)
         self.post_norm = RMSNorm(h, cfg["eps"], device)
+        self.cache = None   # the paged cache in 8 bits, in the place of k_cache and v_cache
+        if cache_dtype is not None:
+            self.cache = new_cache(cache_pages, self.heads, page_size, self.head_dim, cache_dtype, device)
+            return
         self.register_buffer("k_cache", torch.zeros(1, self.heads, max_len, self.head_dim, dtype=torch.float16, device=device))
         self.register_buffer("v_cache", torch.zeros(1, self.heads, max_len, self.head_dim, dtype=torch.float16, device=device))
 
@@ -137,16 +148,29 @@ class Block(nn.Module):
         return x + self.down_proj(torch.nn.functional.silu(gu[: self.ffn]) * gu[self.ffn :])
 
 
-    def step_fused(self, x, pending, pos, cos_table, sin_table):
+    def step_fused(self, x, pending, pos, cos_table, sin_table, rows=None):
         """The same block as `forward` with three kernels of this package between the four products. `x` [hidden]
         is the residual stream, updated in place; `pending` [k, hidden] holds output vectors that have not been
         added to it yet (the previous block's down projection: one vector, or one partial vector per rank), as
-        the pair that `_pending_output` returns. Returns this block's own pending output."""
+        the pair that `_pending_output` returns. Returns this block's own pending output. `rows`: (page table, lengths) of the one
+        sequence where the cache is a paged one."""
         ops = torch.ops.macko_spmv
         qkv = self.qkv_proj(_add_norm(x, pending, self.input_norm))
-        attn = ops.rope_attention(qkv, cos_table, sin_table, pos, self.k_cache, self.v_cache)
+        if self.cache is None:
+            attn = ops.rope_attention(qkv, cos_table, sin_table, pos, self.k_cache, self.v_cache)
+        else:
+            attn = paged_attention(rope_append(qkv.view(1, -1), cos_table, sin_table, self.cache, *rows), self.cache, *rows).view(-1)
         gu = self.gate_up_proj(_add_norm(x, _pending_output(self.o_proj, attn), self.post_norm))
         return _pending_output(self.down_proj, ops.silu_mul(gu))
+
+    def extend(self, x, cos_table, sin_table, page_table, lengths, query_start):
+        """Rows x [N, hidden] of several sequences, the last ones of each (see `kv_cache`), with a paged cache."""
+        qkv = self.qkv_proj(self.input_norm(x))
+        q = rope_append(qkv, cos_table, sin_table, self.cache, page_table, lengths, query_start)
+        attn = paged_attention(q, self.cache, page_table, lengths, query_start)
+        x = x + self.o_proj(attn.view(x.shape[0], -1))
+        gu = self.gate_up_proj(self.post_norm(x))
+        return x + self.down_proj(torch.nn.functional.silu(gu[:, : self.ffn]) * gu[:, self.ffn :])
 
     def prefill(self, x, cos, sin):
         """All prompt positions at once: x [T, hidden], cos/sin [T, head_dim]. Fills cache rows 0..T-1."""
@@ -191,9 +215,14 @@ def _rope(t, cos, sin):
 
 class LlamaDecoder(nn.Module):
     def __init__(self, density: float, cfg=None, layers=None, device="cuda", max_len=384, seed=4000,
-                 prune_lm_head=True, peer=None, fused_glue=True):
+                 prune_lm_head=True, peer=None, fused_glue=True, cache_dtype=None, sequences=1, page_size=32):
         super().__init__()
+        if cache_dtype is None and sequences != 1:
+            raise ValueError("several sequences need a paged cache (cache_dtype)")
+        if cache_dtype is not None and not fused_glue:
+            raise ValueError("the step in plain PyTorch operators has an fp16 cache")
         self.fused_glue = fused_glue
+        self.cache_dtype, self.sequences = cache_dtype, sequences
         cfg = dict(LLAMA2_7B if cfg is None else cfg)
         if layers is not None:
             cfg["layers"] = layers
@@ -201,7 +230,10 @@ class LlamaDecoder(nn.Module):
         h = cfg["hidden"]
         g = torch.Generator(device=device).manual_seed(seed)
         self.embed = (0.02 * torch.randn(cfg["vocab"], h, generator=g, device=device)).to(torch.float16)
-        self.blocks = nn.ModuleList([Block(cfg, density, seed + 100 * (i + 1), device, max_len, peer) for i in range(cfg["layers"])])
+        pages = -(-max_len // page_size)   # of a sequence; sequence i has pages i * pages ... of every block's cache
+        self.blocks = nn.ModuleList([Block(cfg, density, seed + 100 * (i + 1), device, max_len, peer, sequences * pages, page_size, cache_dtype)
+                                     for i in range(cfg["layers"])])
+        self.page_table = torch.arange(sequences * pages, dtype=torch.int32, device=device).view(sequences, pages)
         self.norm = RMSNorm(h, cfg["eps"], device)
         # A decode step is two exchanges per block plus this one: an odd number. Replayed as one captured graph,
         # its last exchange would be followed by its first in the same slot; the LM head takes the spare slot.
@@ -209,7 +241,8 @@ class LlamaDecoder(nn.Module):
                                       peer if prune_lm_head else None, slot=2)
         half = (h // cfg["heads"]) // 2
         inv = 1.0 / (cfg["rope_theta"] ** (torch.arange(half, device=device, dtype=torch.float32) / half))
-        ang = torch.arange(max_len, device=device, dtype=torch.float32)[:, None] * inv[None, :]
+        positions = max_len if cache_dtype is None else pages * page_size
+        ang = torch.arange(positions, device=device, dtype=torch.float32)[:, None] * inv[None, :]
         ang = torch.cat((ang, ang), dim=-1)
         self.cos_table, self.sin_table = ang.cos().to(torch.float16), ang.sin().to(torch.float16)
         self.neg_inf = torch.tensor(float("-inf"), dtype=torch.float16, device=device)
@@ -226,6 +259,9 @@ class LlamaDecoder(nn.Module):
         """Runs the whole prompt (int64 [T]) in one pass (the linear layers see a [T, hidden] batch and route
         it through the multi-vector product or the dense-copy GEMM); returns the greedy next token [1]."""
         T = tokens.numel()
+        if self.cache_dtype is not None:
+            ends = torch.tensor([0, T], dtype=torch.int32, device=tokens.device)
+            return torch.argmax(self.extend(tokens, ends[1:], ends, self.page_table[:1])[0].float(), dim=-1, keepdim=True)
         x = self.embed.index_select(0, tokens)
         cos, sin = self.cos_table[:T], self.sin_table[:T]
         for blk in self.blocks:
@@ -233,13 +269,28 @@ class LlamaDecoder(nn.Module):
         logits = self.lm_head(self.norm(x[T - 1]))
         return torch.argmax(logits.float(), dim=-1, keepdim=True)
 
+    def extend(self, tokens, lengths, query_start=None, page_table=None):
+        """Rows of several sequences in one pass, with a paged cache: tokens int64 [N], of which query_start[i] .. query_start[i + 1] (int32 on
+        the device; None: one each) are the last of sequence i, which has lengths[i] (int32) with them. Returns fp16 logits
+        [sequences, vocab] of every sequence's last row. `page_table`: the model's own (sequence i in its own pages) if None."""
+        if self.cache_dtype is None:
+            raise RuntimeError("extend needs a paged cache (cache_dtype)")
+        table = self.page_table if page_table is None else page_table
+        x = self.embed.index_select(0, tokens)
+        for blk in self.blocks:
+            x = blk.extend(x, self.cos_table, self.sin_table, table, lengths, query_start)
+        if query_start is not None:
+            x = x.index_select(0, (query_start[1:] - 1).clamp(min=0))
+        return self.lm_head(self.norm(x))
+
     def logits(self, token, pos):
         """fp16 logits [vocab] of the token at position `pos`; updates the KV cache."""
         x = self.embed.index_select(0, token)[0]
         if self.fused_glue:
             pending = (x.new_empty((0, x.shape[0])), None)
+            rows = (self.page_table[:1], (pos + 1).to(torch.int32)) if self.cache_dtype is not None else None
             for blk in self.blocks:
-                pending = blk.step_fused(x, pending, pos, self.cos_table, self.sin_table)
+                pending = blk.step_fused(x, pending, pos, self.cos_table, self.sin_table, rows)
             return self.lm_head(_add_norm(x, pending, self.norm))
         cos = self.cos_table.index_select(0, pos)[0]
         sin = self.sin_table.index_select(0, pos)[0]
@@ -301,6 +352,57 @@ def generate(model: LlamaDecoder, prompt: torch.Tensor, new_tokens: int, use_gra
     return torch.cat(tokens), t2 - t1, t1 - t0
 
 
+@torch.no_grad()
+def generate_batch(model: LlamaDecoder, prompts, new_tokens: int, use_graph: bool = True):
+    """Greedy continuation of several prompts (int64 vectors of any lengths) side by side: one pass over all of them, then one captured
+    step per token. Returns (tokens [sequences, new_tokens], seconds for the generated part, seconds for the prompts)."""
+    dev, n = model.device, len(prompts)
+    if n != model.sequences:
+        raise ValueError(f"{n} prompts for a model of {model.sequences} sequences")
+    counts = [p.numel() for p in prompts]
+    if max(counts) + new_tokens > model.max_len or min(counts) < 1:
+        raise ValueError("every prompt needs a token, and room for it and the new ones")
+    ends = torch.tensor([sum(counts[:i]) for i in range(n + 1)], dtype=torch.int32, device=dev)
+    lengths = torch.tensor(counts, dtype=torch.int32, device=dev)
+    rows = torch.cat([p.to(dev) for p in prompts])
+
+    def first():
+        return torch.argmax(model.extend(rows, lengths, ends).float(), dim=-1)
+
+    first()   # untimed, as in `generate`
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    token = first()
+    torch.cuda.synchronize()
+    t1 = time.perf_counter()
+
+    def step():
+        lengths.add_(1)
+        token.copy_(torch.argmax(model.extend(token, lengths).float(), dim=-1))
+
+    graph = None
+    if use_graph and new_tokens > 1:
+        kept = lengths.clone(), token.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        lengths.copy_(kept[0])   # the warm-up's token is written again, at the same place
+        token.copy_(kept[1])
+    tokens = [token.clone()]
+    torch.cuda.synchronize()
+    t2 = time.perf_counter()
+    for _ in range(new_tokens - 1):
+        graph.replay() if graph is not None else step()
+        tokens.append(token.clone())
+    torch.cuda.synchronize()
+    return torch.stack(tokens, dim=1), time.perf_counter() - t2, t1 - t0
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--density", type=float, default=0.5, help="1.0 = dense nn.Linear (cuBLAS) baseline")
@@ -311,7 +413,12 @@ def main():
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--batched-prefill", action="store_true",
                     help="run the prompt in one pass (one GPU only): linear layers take the [tokens, hidden] batch")
+    ap.add_argument("--cache", choices=("fp16", "int8", "fp8"), default="fp16", help="keys and values: fp16, or paged in 8 bits")
+    ap.add_argument("--sequences", type=int, default=1, help="prompts continued side by side (one GPU, --cache int8 or fp8)")
     args = ap.parse_args()
+    cache_dtype = {"fp16": None, "int8": torch.int8, "fp8": torch.float8_e4m3fn}[args.cache]
+    if args.sequences < 1 or (args.sequences > 1 and (cache_dtype is None or int(os.environ.get("WORLD_SIZE", "1")) > 1)):
+        raise SystemExit("--sequences runs on one GPU with --cache int8 or fp8")
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
     local_rank = int(os.environ.get("LOCAL_RANK", "0"))
@@ -329,7 +436,7 @@ def main():
         peer = PeerGather(max(world * cfg["hidden"], cfg["vocab"]), device)   # N partial vectors of the column-sharded layers, or the logits
     t0 = time.perf_counter()
     model = LlamaDecoder(args.density, layers=args.layers, device=device, max_len=args.prompt + args.new_tokens,
-                         prune_lm_head=not args.dense_lm_head, peer=peer)
+                         prune_lm_head=not args.dense_lm_head, peer=peer, cache_dtype=cache_dtype, sequences=args.sequences)
     torch.cuda.synchronize()
     build_s = time.perf_counter() - t0
     g = torch.Generator(device=device).manual_seed(4001)
@@ -338,6 +445,17 @@ def main():
         dist.barrier()
     if args.batched_prefill and world > 1:
         raise SystemExit("--batched-prefill runs on one GPU: the row-sharded layers multiply one vector at a time")
+    if args.sequences > 1:
+        prompts = [torch.randint(0, model.cfg["vocab"], (args.prompt,), generator=g, device=device) for _ in range(args.sequences)]
+        tokens, gen_s, prompt_s = generate_batch(model, prompts, args.new_tokens, use_graph=not args.no_graph)
+        print(json.dumps({
+            "model": "llama-2-7b architecture, random init", "layers": args.layers, "density": args.density, "cache": args.cache,
+            "sequences": args.sequences, "prompt_tokens": args.prompt, "new_tokens": args.new_tokens,
+            "tokens_per_s": args.sequences * (args.new_tokens - 1) / max(gen_s, 1e-9),
+            "prompt_tokens_per_s": args.sequences * args.prompt / prompt_s, "build_seconds": build_s,
+            "memory_GB": torch.cuda.max_memory_allocated() / 1e9, "cuda_graph": not args.no_graph, "first_tokens": tokens[0, :8].tolist(),
+        }), flush=True)
+        return
     tokens, gen_s, prompt_s = generate(model, prompt, args.new_tokens, use_graph=not args.no_graph,
                                        batched_prefill=args.batched_prefill)
     same = True
@@ -354,7 +472,7 @@ def main():
         print(json.dumps({
             "model": "llama-2-7b architecture, random init", "layers": args.layers, "density": args.density,
             "tensor_parallel": world, "ranks_agree": same,
-            "lm_head": "dense" if args.dense_lm_head or args.density >= 1 else "pruned",
+            "cache": args.cache, "lm_head": "dense" if args.dense_lm_head or args.density >= 1 else "pruned",
             "prompt_tokens": args.prompt, "new_tokens": args.new_tokens,
             "tokens_per_s": args.new_tokens / gen_s, "prompt_tokens_per_s": args.prompt / prompt_s,
             "build_seconds": build_s, "memory_GB": torch.cuda.max_memory_allocated() / 1e9,

@@ -678,3 +678,75 @@ def test_refusals_of_the_c_entries():
     assert attend(cache(), rows(), q_head=68) == askew and attend(cache(), rows(), out=None) == bad
     for args in ((-1, 1, 1, 4, 2, 16, 64, 0), (1, 1, 1, 3, 2, 16, 64, 0), (1, 1, 1, 4, 2, 17, 64, 0), (1, 1 << 25, 1, 4, 2, 16, 64, 0)):
         assert lib.macko_cache_attention_workspace_bytes(*args) < 0
+
+
+def _model(cache_dtype=None, sequences=1, seed=31, max_len=70, **more):
+    from macko_spmv_b200 import llama_decode
+
+    cfg = dict(hidden=256, heads=4, ffn=512, vocab=1000, layers=3, eps=1e-5, rope_theta=10000.0)
+    return llama_decode.LlamaDecoder(0.5, cfg=cfg, max_len=max_len, seed=seed, cache_dtype=cache_dtype, sequences=sequences, page_size=16, **more)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code,far", [("int8", 0.03), ("fp8", 0.1)])
+def test_decoder_with_a_cache_in_8_bits(code, far):
+    """Logits of the decoder with a paged cache against those with an fp16 cache. Per layer, keys and values are off by at most half a
+    step: 2^-7 of a page's largest (int8, whose scale may be twice what is needed) or 2^-4 of themselves (e4m3), errors of random sign that an
+    average over tokens makes smaller; the residual stream carries them on. The bounds are those steps with their root mean square over
+    sqrt(3) and two for the three layers: 2 * 2^-6 and 2 * 2^-4 / sqrt(3), rounded up."""
+    with torch.no_grad():
+        a, b = _model(), _model(CODES[code])
+        tokens = [3, 999, 17, 0, 512, 44, 8, 250, 77, 1, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15]
+        for i, tok in enumerate(tokens):
+            token, pos = torch.tensor([tok], device="cuda"), torch.tensor([i], device="cuda")
+            la, lb = a.logits(token, pos).float(), b.logits(token, pos).float()
+            assert float((la - lb).norm() / la.norm()) < far, i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+def test_sequences_side_by_side(code):
+    """Prompts in one pass, in pieces, and mixed with single tokens: the caches are the same bits as far as the rows are, and logits agree with
+    the sequence alone to the rounding of fp16 activations (2^-11 a step, some ten steps a layer)."""
+    prompts = [torch.randint(0, 1000, (n,), generator=_gen(60 + n), device="cuda") for n in (5, 33, 1, 20)]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        m = _model(CODES[code], sequences=4)
+        whole = m.extend(torch.cat(prompts), i32([5, 33, 1, 20]), i32([0, 5, 38, 39, 59])).float()
+        alone = []
+        for p in prompts:
+            one = _model(CODES[code])
+            alone.append(one.extend(p, i32([p.numel()]), i32([0, p.numel()])).float()[0])
+        alone = torch.stack(alone)
+        assert float((whole - alone).norm() / alone.norm()) < 2e-2
+        m = _model(CODES[code], sequences=4)
+        # first 2, 30, 0 and 19 tokens, then the rest: 3, 3, 1 and 1
+        first = torch.cat([prompts[0][:2], prompts[1][:30], prompts[3][:19]])
+        m.extend(first, i32([2, 30, 0, 19]), i32([0, 2, 32, 32, 51]))
+        rest = torch.cat([prompts[0][2:], prompts[1][30:], prompts[2], prompts[3][19:]])
+        pieces = m.extend(rest, i32([5, 33, 1, 20]), i32([0, 3, 6, 7, 8])).float()
+        far = 0.03 if code == "int8" else 0.1      # a page that fills in two steps may be rounded twice
+        assert float((pieces - alone).norm() / alone.norm()) < far
+
+
+@pytest.mark.gpu
+def test_generate_batch():
+    from macko_spmv_b200 import llama_decode
+
+    prompts = [torch.randint(0, 1000, (n,), generator=_gen(70 + n), device="cuda") for n in (9, 30, 2)]
+    graph, _, _ = llama_decode.generate_batch(_model(torch.int8, sequences=3), prompts, 12)
+    eager, _, _ = llama_decode.generate_batch(_model(torch.int8, sequences=3), prompts, 12, use_graph=False)
+    assert graph.shape == (3, 12) and torch.equal(graph, eager)
+    with pytest.raises(ValueError):
+        llama_decode.generate_batch(_model(torch.int8, sequences=2), prompts, 12)
+    with pytest.raises(ValueError):
+        llama_decode.generate_batch(_model(torch.int8, sequences=3), prompts, 60)
+    single, _, _ = llama_decode.generate(_model(torch.float8_e4m3fn), prompts[0], 12)
+    again, _, _ = llama_decode.generate(_model(torch.float8_e4m3fn), prompts[0], 12, use_graph=False)
+    assert torch.equal(single, again)
+    assert llama_decode.generate(_model(torch.int8), prompts[1], 3, batched_prefill=True)[0].shape == (3,)
+    for bad in (dict(sequences=2), dict(cache_dtype=torch.int8, fused_glue=False)):
+        with pytest.raises(ValueError):
+            _model(**bad)
+    with pytest.raises(RuntimeError):
+        _model().extend(prompts[0], None)
