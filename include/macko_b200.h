@@ -455,7 +455,7 @@ int macko_decode_argmax(const void *values, int64_t n, int64_t *index, void *str
 typedef struct macko_kv_cache {
     void *k, *v;                             /* [pages][kv_heads][page_size][head_dim] codes, 16-byte aligned */
     float *k_scale, *v_scale;                /* [pages][kv_heads], greater than zero */
-    int64_t k_page_stride, v_page_stride;    /* bytes between pages, multiples of 16 */
+    int64_t k_page_stride, v_page_stride;    /* bytes between pages, multiples of 16; times pages at most 2^36 */
     int64_t k_scale_stride, v_scale_stride;  /* floats between pages */
     int64_t pages;
     int32_t kv_heads, page_size, head_dim, code; /* page_size 16, 32, 64 or 128; head_dim 64, 128 or 256; MACKO_KV_* */

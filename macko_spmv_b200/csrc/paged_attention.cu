@@ -178,68 +178,75 @@ few_rows_kernel(const AttentionArgs a)
         const int stop = min(end, (piece.first_tile + piece.tiles) * kTile);
         const int first = piece.first_tile * kTile + warp * 16 * MT;
         const long long head_at = ((long long)piece.kv_head << c.page_log2) * D;
-        int page_of_lane = -1;
-        float ks_of_lane = 0.f, vs_of_lane = 1.f;
+        // Of the warp's next 32 blocks of 16 tokens, one per lane: where their codes begin, in units of 16 bytes, and what the softmax
+        // needs of their page's scales.
+        bool there_of_lane = false;
+        uint32_t k_of_lane = 0u, v_of_lane = 0u;
+        float ks_of_lane = 0.f, shift_of_lane = 0.f, inverse_of_lane = 0.f;
         Codes<16> kc[MT][2][KC];
         Codes<VB> vc[MT][4];
-        // pages and scales of the warp's next 32 blocks of 16 tokens, one per lane
         auto fetch_pages = [&](int from) {
             const int token = from + (lane / MT) * kTile + (lane % MT) * 16;
-            page_of_lane = token < end ? page_at(c, r, piece.sequence, token) : -1;
-            ks_of_lane = 0.f;
-            vs_of_lane = 1.f;
-            if (page_of_lane >= 0) {
-                ks_of_lane = __ldcg(c.k_scale + page_of_lane * c.k_scale_stride + piece.kv_head);
-                vs_of_lane = value_scale(__ldcg(c.v_scale + page_of_lane * c.v_scale_stride + piece.kv_head));
+            const int page = token < end ? page_at(c, r, piece.sequence, token) : -1;
+            there_of_lane = page >= 0;
+            if (there_of_lane) {
+                const long long off = head_at + (long long)(token & page_mask) * D;
+                k_of_lane = (uint32_t)((page * c.k_stride + off) >> 4);
+                v_of_lane = (uint32_t)((page * c.v_stride + off) >> 4);
+                const float vs = value_scale(__ldcg(c.v_scale + page * c.v_scale_stride + piece.kv_head));
+                ks_of_lane = __ldcg(c.k_scale + page * c.k_scale_stride + piece.kv_head);
+                shift_of_lane = __log2f(vs);
+                inverse_of_lane = __fdividef(1.f, vs);
             }
         };
+        const uint8_t *const k_base = c.k + 16 * t + g * D, *const v_base = c.v + VB * g + 2 * t * D;
         // `whole`: all of the warp's tokens are there
         auto load_k = [&](int token, int index, int mt, bool whole) {
-            const int page = __shfl_sync(0xffffffffu, page_of_lane, index * MT + mt);
-            const uint8_t *base = c.k + page * c.k_stride + head_at + (long long)((token + mt * 16) & page_mask) * D + 16 * t + g * D;
+            const int from = index * MT + mt;
+            const uint8_t *base = k_base + 16ull * __shfl_sync(0xffffffffu, k_of_lane, from);
+            const bool there = whole || __shfl_sync(0xffffffffu, (int)there_of_lane, from);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int ch = 0; ch < KC; ++ch) {
-                    if (whole || (page >= 0 && token + mt * 16 + g + 8 * h < end)) kc[mt][h][ch] = load_codes<16>(base + 8 * h * D + 64 * ch);
+                    if (whole || (there && token + mt * 16 + g + 8 * h < end)) kc[mt][h][ch] = load_codes<16>(base + 8 * h * D + 64 * ch);
                     else kc[mt][h][ch] = no_codes<16>();
                 }
         };
         auto load_v = [&](int token, int index, int mt, bool whole) {
-            const int page = __shfl_sync(0xffffffffu, page_of_lane, index * MT + mt);
-            const uint8_t *base = c.v + page * c.v_stride + head_at + (long long)((token + mt * 16) & page_mask) * D + VB * g + 2 * t * D;
+            const int from = index * MT + mt;
+            const uint8_t *base = v_base + 16ull * __shfl_sync(0xffffffffu, v_of_lane, from);
+            const bool there = whole || __shfl_sync(0xffffffffu, (int)there_of_lane, from);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = (i & 1) + 8 * (i >> 1);
-                if (whole || (page >= 0 && token + mt * 16 + 2 * t + row < end)) vc[mt][i] = load_codes<VB>(base + row * D);
+                if (whole || (there && token + mt * 16 + 2 * t + row < end)) vc[mt][i] = load_codes<VB>(base + row * D);
                 else vc[mt][i] = no_codes<VB>();
             }
         };
         auto is_whole = [&](int token, int index) {
-            const bool there = __all_sync(0xffffffffu, page_of_lane >= 0 || lane / MT != index);
-            return there && token + 16 * MT <= end;
+            return __all_sync(0xffffffffu, there_of_lane || lane / MT != index) && token + 16 * MT <= end;
         };
-        // the warp's tokens `ahead` turns on, K and V, to the L2 cache: the registers hold no more than one turn, and a load from memory
-        // takes longer than a turn
-        auto ask = [&](int token, int index) {
-            const int mt = lane % MT, at = token + mt * 16;
-            const int page = __shfl_sync(0xffffffffu, page_of_lane, (index * MT + mt) & 31);
-            if (lane < 2 * MT && index * MT < 32 && page >= 0 && at < end) {
-                const long long off = head_at + (long long)(at & page_mask) * D;
-                prefetch(lane < MT ? c.k + page * c.k_stride + off : c.v + page * c.v_stride + off, 16 * D);
+        // the tokens of one of the warp's turns behind, K and V, to the L2 cache: the registers hold no more than one turn, and a load
+        // from memory takes longer than a turn
+        auto ask = [&](int index) {
+            if (lane / MT == index && there_of_lane) {
+                prefetch(c.k + 16ull * k_of_lane, 16 * D);
+                prefetch(c.v + 16ull * v_of_lane, 16 * D);
             }
         };
         constexpr int kPerFetch = 32 / MT;
         int index = 0;
+        bool whole = false;   // the current turn's tokens are all there
         if (first < stop) {
             fetch_pages(first);
-            const bool whole = is_whole(first, 0);
+            whole = is_whole(first, 0);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) load_k(first, 0, mt, whole);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) load_v(first, 0, mt, whole);
 #pragma unroll
-            for (int i = 1; i <= kAhead; ++i) ask(first + i * kTile, i);
+            for (int i = 1; i <= kAhead; ++i) ask(i);
         }
         for (int token = first; token < stop; token += kTile) {
             float x[MT][NB][4], inverse[MT];
@@ -263,11 +270,11 @@ few_rows_kernel(const AttentionArgs a)
             bool there[MT];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const float vs = __shfl_sync(0xffffffffu, vs_of_lane, index * MT + mt);
-                k_scale[mt] = __shfl_sync(0xffffffffu, ks_of_lane, index * MT + mt);
-                there[mt] = __shfl_sync(0xffffffffu, page_of_lane, index * MT + mt) >= 0;
-                shift[mt] = __log2f(vs);
-                inverse[mt] = 1.f / vs;
+                const int from = index * MT + mt;
+                k_scale[mt] = __shfl_sync(0xffffffffu, ks_of_lane, from);
+                shift[mt] = __shfl_sync(0xffffffffu, shift_of_lane, from);
+                inverse[mt] = __shfl_sync(0xffffffffu, inverse_of_lane, from);
+                there[mt] = whole || __shfl_sync(0xffffffffu, (int)there_of_lane, from);
             }
             const int next = token + kTile;
             const bool go_on = next < stop;
@@ -285,13 +292,13 @@ few_rows_kernel(const AttentionArgs a)
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) load_k(next, index, mt, false);
                 }
-                ask(next + kAhead * kTile, index + kAhead);
+                ask(index + kAhead);
             }
 
             float top[NB][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) top[nb][0] = top[nb][1] = -INFINITY;
-            const bool whole = token + 16 * MT <= all_see;
+            const bool all_seen = token + 16 * MT <= all_see;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -300,7 +307,7 @@ few_rows_kernel(const AttentionArgs a)
                     for (int i = 0; i < 4; ++i) {
                         float &v = x[mt][nb][i];
                         v = v * (k_scale[mt] * factor[nb][i & 1]) + shift[mt];
-                        if (!there[mt] || (!whole && token + mt * 16 + g + 8 * (i >> 1) >= limit[nb][i & 1])) v = -INFINITY;
+                        if (!there[mt] || (!all_seen && token + mt * 16 + g + 8 * (i >> 1) >= limit[nb][i & 1])) v = -INFINITY;
                         top[nb][i & 1] = fmaxf(top[nb][i & 1], v);
                     }
             }
@@ -367,6 +374,7 @@ few_rows_kernel(const AttentionArgs a)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) load_v(next, index, mt, false);
             }
+            whole = next_whole;
         }
 
         // the warps' results together: rows 2t, 2t + 1 of every block, dimensions g * D / 8 + 2 d + (0, 1)
@@ -690,7 +698,7 @@ int64_t macko_cache_attention_workspace_bytes(int64_t sequences, int64_t rows, i
 {
     // the refusals of macko_cache_attention, from the arguments that size it
     const macko_kv_cache cache = {reinterpret_cast<void *>(16), reinterpret_cast<void *>(16), reinterpret_cast<float *>(16), reinterpret_cast<float *>(16),
-                                  INT64_MAX / 16 * 16, INT64_MAX / 16 * 16, INT64_MAX, INT64_MAX, 1, kv_heads, page_size, head_dim, MACKO_KV_INT8};
+                                  1ll << 36, 1ll << 36, 1ll << 40, 1ll << 40, 1, kv_heads, page_size, head_dim, MACKO_KV_INT8};
     const macko_kv_rows batch = {reinterpret_cast<const int32_t *>(16), reinterpret_cast<const int32_t *>(16),
                                  one_row_each ? nullptr : reinterpret_cast<const int32_t *>(16), table_width, table_width, sequences, rows};
     AttentionArgs a = {};

@@ -306,6 +306,8 @@ int check_cache(const char *what, const macko_kv_cache *c, CacheView *view)
     const int64_t page_bytes = (int64_t)c->kv_heads * c->page_size * c->head_dim;
     if (c->k_page_stride < page_bytes || c->v_page_stride < page_bytes || c->k_scale_stride < c->kv_heads || c->v_scale_stride < c->kv_heads)
         return fail(MACKO_ERR_INVALID_ARGUMENT, "%s: a page stride is smaller than a page", what);
+    if (c->k_page_stride > (1ll << 36) / c->pages || c->v_page_stride > (1ll << 36) / c->pages || c->k_scale_stride > (1ll << 40) || c->v_scale_stride > (1ll << 40))
+        return fail(MACKO_ERR_SIZE_OVERFLOW, "%s: keys or values of more than 2^36 bytes", what);   // 32 bits count them by 16
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->k_page_stride % 16 || c->v_page_stride % 16 || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
         return fail(MACKO_ERR_MISALIGNED, "%s: codes and the strides of their pages must be multiples of 16 bytes, scales of 4", what);
     int log2 = 4;
