@@ -114,6 +114,14 @@ few_rows_kernel(const AttentionArgs a)
     while (more) {
         const UnitRows u = unit_rows(a, walk.s, piece);
         const int n_rows = u.rows();
+        // table entry of the lane's block of 16 tokens, of the 32 that begin at `from`; asked for before anybody knows how many tokens
+        // the sequence has
+        auto entry_of = [&](int from) {
+            const int token = from + (lane / MT) * kTile + (lane % MT) * 16;
+            return token < r.capacity ? __ldcg(r.table + (long long)piece.sequence * r.table_stride + (token >> c.page_log2)) : -1;
+        };
+        const int first = piece.first_tile * kTile + warp * 16 * MT;
+        const int first_entry = entry_of(first);
 
         // q as the B operand: row g of every block of 8, dimensions 64 c + 16 t + 4 i + 0..3 for step 4 c + i
         uint32_t q[NB][D / 16][2];
@@ -176,7 +184,6 @@ few_rows_kernel(const AttentionArgs a)
         }
 
         const int stop = min(end, (piece.first_tile + piece.tiles) * kTile);
-        const int first = piece.first_tile * kTile + warp * 16 * MT;
         const long long head_at = ((long long)piece.kv_head << c.page_log2) * D;
         // Of the warp's next 32 blocks of 16 tokens, one per lane: where their codes begin, in units of 16 bytes, and what the softmax
         // needs of their page's scales.
@@ -185,10 +192,9 @@ few_rows_kernel(const AttentionArgs a)
         float ks_of_lane = 0.f, shift_of_lane = 0.f, inverse_of_lane = 0.f;
         Codes<16> kc[MT][2][KC];
         Codes<VB> vc[MT][4];
-        auto fetch_pages = [&](int from) {
+        auto fetch_pages = [&](int from, int page) {
             const int token = from + (lane / MT) * kTile + (lane % MT) * 16;
-            const int page = token < end ? page_at(c, r, piece.sequence, token) : -1;
-            there_of_lane = page >= 0;
+            there_of_lane = token < end && (unsigned)page < (unsigned)c.pages;
             if (there_of_lane) {
                 const long long off = head_at + (long long)(token & page_mask) * D;
                 k_of_lane = (uint32_t)((page * c.k_stride + off) >> 4);
@@ -239,7 +245,7 @@ few_rows_kernel(const AttentionArgs a)
         int index = 0;
         bool whole = false;   // the current turn's tokens are all there
         if (first < stop) {
-            fetch_pages(first);
+            fetch_pages(first, first_entry);
             whole = is_whole(first, 0);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) load_k(first, 0, mt, whole);
@@ -280,7 +286,7 @@ few_rows_kernel(const AttentionArgs a)
             const bool go_on = next < stop;
             if (++index == kPerFetch && go_on) {
                 index = 0;
-                fetch_pages(next);
+                fetch_pages(next, entry_of(next));
             }
             bool next_whole = false;
             if (go_on) {
