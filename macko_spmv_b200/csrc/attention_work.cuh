@@ -66,18 +66,18 @@ struct SequenceWork {
     int begin, blocks;       // begin: first position, kept inside 0 .. capacity for counting
 };
 
-__device__ __forceinline__ SequenceWork sequence_work(const WorkShape &w, const RowsView &r, int i)
+__device__ __forceinline__ SequenceWork sequence_work(const WorkShape &w, const RowsView &r, const Sequence &rows)
 {
     SequenceWork s;
-    s.rows = sequence_at(r, i);
+    s.rows = rows;
     s.begin = min(max(s.rows.begin(), 0), r.capacity);
     s.blocks = (s.rows.count + w.queries - 1) / w.queries;
     return s;
 }
 
-__device__ __forceinline__ long long sequence_tiles(const WorkShape &w, const RowsView &r, int i)
+__device__ __forceinline__ long long sequence_tiles(const WorkShape &w, const RowsView &r, const Sequence &rows)
 {
-    const SequenceWork s = sequence_work(w, r, i);
+    const SequenceWork s = sequence_work(w, r, rows);
     return tiles_before(w, s.begin, s.blocks) * (w.kv_heads * w.parts);
 }
 
@@ -106,9 +106,14 @@ struct WorkWalk {
         cta = of_cta;
         // the total, then the sequence with this CTA's first tile
         long long total = 0, first_own = 0;
+        Sequence first_rows = {0, 0, 0};
         for (int i = lane; i < r.sequences; i += 32) {
-            const long long own = sequence_tiles(w, r, i);
-            if (i == lane) first_own = own;
+            const Sequence rows = sequence_at(r, i);
+            const long long own = sequence_tiles(w, r, rows);
+            if (i == lane) {
+                first_own = own;
+                first_rows = rows;
+            }
             total += own;
         }
 #pragma unroll
@@ -120,7 +125,7 @@ struct WorkWalk {
         if (at >= end) return;
         long long before = 0, base = 0;
         for (int first = 0; first < r.sequences; first += 32) {
-            const long long own = first == 0 ? first_own : first + lane < r.sequences ? sequence_tiles(w, r, first + lane) : 0;
+            const long long own = first == 0 ? first_own : first + lane < r.sequences ? sequence_tiles(w, r, sequence_at(r, first + lane)) : 0;
             long long sum = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -140,7 +145,15 @@ struct WorkWalk {
             at = end;
             return;
         }
-        s = sequence_work(w, r, sequence);
+        Sequence rows;
+        if (sequence < 32) {
+            rows.first = __shfl_sync(0xffffffffu, first_rows.first, sequence);
+            rows.count = __shfl_sync(0xffffffffu, first_rows.count, sequence);
+            rows.length = __shfl_sync(0xffffffffu, first_rows.length, sequence);
+        } else {
+            rows = sequence_at(r, sequence);
+        }
+        s = sequence_work(w, r, rows);
         const long long local = at - base, per_head = tiles_before(w, s.begin, s.blocks);
         head_part = (int)quotient(local, max(per_head, 1ll));
         const long long rest = local - head_part * per_head;
@@ -166,7 +179,7 @@ struct WorkWalk {
         if (at >= end) return false;
         while (s.blocks == 0 || head_part >= w.kv_heads * w.parts) {
             if (++sequence >= r.sequences) return false;
-            s = sequence_work(w, r, sequence);
+            s = sequence_work(w, r, sequence_at(r, sequence));
             head_part = block = tile = 0;
         }
         const int of_unit = (int)(((long long)s.begin + (long long)(block + 1) * w.queries + w.tile - 1) / w.tile);

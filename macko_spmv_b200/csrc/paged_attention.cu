@@ -443,72 +443,94 @@ few_rows_kernel(const AttentionArgs a)
     clear_other_rows(a);
 }
 
-// Units that lie in several CTAs: one block per CTA with whose share such a unit begins, and gridDim.y blocks for its rows. A
-// row's pieces are spread over the block's warps that are left for it.
+// Units that lie in several CTAs. Every block makes the list of them (the CTAs with whose share they begin); their rows are dealt out, to
+// warps where there are many, else to blocks, whose warps share a row's pieces.
+constexpr int kMostCtas = 1024;
+
 template <bool BF16, int D>
 __global__ void __launch_bounds__(256)
 join_kernel(const AttentionArgs a)
 {
     constexpr int V = D / 32;   // dimensions of a lane: 2, 4 or 8
     __shared__ float parts[8][D + 2];
+    __shared__ int list[kMostCtas], counts[9];
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 *at = reinterpret_cast<const int4 *>(a.split + blockIdx.x);
-    const int4 s = __ldcg(at);   // first row, rows, head, pieces
-    const int pieces = s.w;
-    if (pieces == 0) return;
-    const int unit_heads = __ldcg(at + 1).x;
-    const int rows_here = a.unit_rows / gridDim.y;                 // rows of this block: a power of two, or all of them
-    const int warps_of_row = rows_here >= 8 ? 1 : 8 / rows_here, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int stride = a.unit_rows * (D + 2);
-    for (int base = 0; base < rows_here; base += 8 / warps_of_row) {
-        const int row = blockIdx.y * rows_here + base + warp / warps_of_row, member = warp % warps_of_row;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ctas = a.work.ctas;
+    // in order, so that every block has the same list: each warp a range of CTAs
+    const int range = (ctas + 255) / 256;
+    uint32_t split = 0u;   // of this thread's CTAs
+    for (int i = 0; i < range; ++i) {
+        const int cta = (warp * 32 + lane) * range + i;
+        if (cta < ctas && __ldcg(&a.split[cta].pieces) > 0) split |= 1u << i;
+    }
+    int own = __popc(split), sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 31) counts[warp] = sum;
+    __syncthreads();
+    int at = sum - own, units = 0;
+    for (int w = 0; w < 8; ++w) {
+        if (w < warp) at += counts[w];
+        units += counts[w];
+    }
+    for (int i = 0; i < range; ++i)
+        if (split >> i & 1u) list[at++] = (warp * 32 + lane) * range + i;
+    __syncthreads();
+    const int rows = units * a.unit_rows, stride = a.unit_rows * (D + 2);
+    const bool shared = rows <= (int)gridDim.x * 2;   // a row for a block, not for a warp
+    for (int item = shared ? (int)blockIdx.x : (int)blockIdx.x * 8 + warp; item < rows; item += shared ? gridDim.x : gridDim.x * 8) {
+        const int cta = list[item / a.unit_rows], row = item % a.unit_rows;
+        const int4 s = __ldcg(reinterpret_cast<const int4 *>(a.split + cta));   // first row, rows, head, pieces
+        if (row >= s.y) continue;
+        const int unit_heads = __ldcg(&a.split[cta].heads);
+        const int member = shared ? warp : 0, members = shared ? 8 : 1, pieces = s.w;
         float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = 0.f;
-        if (row < s.y) {
-            constexpr int U = 4;
-            for (int p0 = member; p0 < pieces; p0 += U * warps_of_row) {
-                float pm[U], pl[U], po[U][V];
+        constexpr int U = 4;
+        for (int p0 = member; p0 < pieces; p0 += U * members) {
+            float pm[U], pl[U], po[U][V];
 #pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    const int p = p0 + i * warps_of_row;
-                    pm[i] = -INFINITY;
-                    pl[i] = 0.f;
-                    if (p < pieces) {
-                        // the first piece is the second result of its CTA, the others are the first of theirs
-                        const float *from = a.partial + ((long long)(blockIdx.x + p) * 2 + (p == 0)) * stride;
-                        pm[i] = __ldcg(from + a.unit_rows * D + row);
-                        pl[i] = __ldcg(from + a.unit_rows * D + a.unit_rows + row);
+            for (int i = 0; i < U; ++i) {
+                const int p = p0 + i * members;
+                pm[i] = -INFINITY;
+                pl[i] = 0.f;
 #pragma unroll
-                        for (int j = 0; j < V; j += 2) {
-                            const float2 x = __ldcg(reinterpret_cast<const float2 *>(from + row * D + lane * V + j));
-                            po[i][j] = x.x;
-                            po[i][j + 1] = x.y;
-                        }
-                    } else {
+                for (int j = 0; j < V; ++j) po[i][j] = 0.f;
+                if (p < pieces) {
+                    // the first piece is the second result of its CTA, the others are the first of theirs
+                    const float *from = a.partial + ((long long)(cta + p) * 2 + (p == 0)) * stride;
+                    pm[i] = __ldcg(from + a.unit_rows * D + row);
+                    pl[i] = __ldcg(from + a.unit_rows * D + a.unit_rows + row);
 #pragma unroll
-                        for (int j = 0; j < V; ++j) po[i][j] = 0.f;
+                    for (int j = 0; j < V; j += 2) {
+                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(from + row * D + lane * V + j));
+                        po[i][j] = x.x;
+                        po[i][j + 1] = x.y;
                     }
                 }
-                float most = m;
+            }
+            float most = m;
 #pragma unroll
-                for (int i = 0; i < U; ++i) most = fmaxf(most, pm[i]);
-                const float base2 = most == -INFINITY ? 0.f : most, keep = exp2_fast(m - base2);
-                m = most;
-                l *= keep;
+            for (int i = 0; i < U; ++i) most = fmaxf(most, pm[i]);
+            const float base = most == -INFINITY ? 0.f : most, keep = exp2_fast(m - base);
+            m = most;
+            l *= keep;
 #pragma unroll
-                for (int j = 0; j < V; ++j) o[j] *= keep;
+            for (int j = 0; j < V; ++j) o[j] *= keep;
 #pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    const float f = exp2_fast(pm[i] - base2);
-                    l += f * pl[i];
+            for (int i = 0; i < U; ++i) {
+                const float f = exp2_fast(pm[i] - base);
+                l += f * pl[i];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) o[j] += f * po[i][j];
-                }
+                for (int j = 0; j < V; ++j) o[j] += f * po[i][j];
             }
         }
-        if (warps_of_row > 1) {
+        if (shared) {
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < V; ++j) parts[warp][lane * V + j] = o[j];
@@ -517,27 +539,24 @@ join_kernel(const AttentionArgs a)
                 parts[warp][D + 1] = l;
             }
             __syncthreads();
-            if (member == 0) {
-                float most = m;
-                for (int w = 1; w < warps_of_row; ++w) most = fmaxf(most, parts[warp + w][D]);
-                const float base2 = most == -INFINITY ? 0.f : most, keep = exp2_fast(m - base2);
-                l *= keep;
+            if (warp != 0) continue;
+            float most = m;
+            for (int w = 1; w < 8; ++w) most = fmaxf(most, parts[w][D]);
+            const float base = most == -INFINITY ? 0.f : most, keep = exp2_fast(m - base);
+            l *= keep;
 #pragma unroll
-                for (int j = 0; j < V; ++j) o[j] *= keep;
-                for (int w = 1; w < warps_of_row; ++w) {
-                    const float f = exp2_fast(parts[warp + w][D] - base2);
-                    l += f * parts[warp + w][D + 1];
+            for (int j = 0; j < V; ++j) o[j] *= keep;
+            for (int w = 1; w < 8; ++w) {
+                const float f = exp2_fast(parts[w][D] - base);
+                l += f * parts[w][D + 1];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) o[j] += f * parts[warp + w][lane * V + j];
-                }
+                for (int j = 0; j < V; ++j) o[j] += f * parts[w][lane * V + j];
             }
         }
-        if (member == 0 && row < s.y) {
-            const float inverse = l == 0.f ? 0.f : 1.f / l;
-            uint16_t *to = a.out + ((long long)(s.x + row / unit_heads) * a.heads + s.z + row % unit_heads) * D + lane * V;
+        const float inverse = l == 0.f ? 0.f : 1.f / l;
+        uint16_t *to = a.out + ((long long)(s.x + row / unit_heads) * a.heads + s.z + row % unit_heads) * D + lane * V;
 #pragma unroll
-            for (int j = 0; j < V; j += 2) *reinterpret_cast<uint32_t *>(to + j) = pack2<BF16>(o[j] * inverse, o[j + 1] * inverse);
-        }
+        for (int j = 0; j < V; j += 2) *reinterpret_cast<uint32_t *>(to + j) = pack2<BF16>(o[j] * inverse, o[j + 1] * inverse);
     }
 }
 
@@ -614,9 +633,8 @@ int check_sizes(const macko_kv_cache *cache, const macko_kv_rows *batch, int hea
 struct Launch {
     WorkShape work;
     int unit_rows;      // 8 or 16; 128 or more: the kernel for many rows
-    int ctas, smem;
+    int ctas, smem, sm_count;
     bool split;
-    int join_rows;      // blocks per split unit
     int64_t split_bytes, partial_bytes;
 };
 
@@ -626,7 +644,11 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     const bool one_each = a.rows.start == nullptr;
     // rows that a head of the cache meets in a sequence, as far as the host knows: on average
     const int64_t mean = one_each ? group : ((int64_t)a.rows.rows * group + a.rows.sequences - 1) / (a.rows.sequences > 0 ? a.rows.sequences : 1);
-    const bool prompt = !one_each && mean > 16;
+    // The kernel for many rows takes 128 or 256 as long as one; the other reads and converts the cache once for 16. 16 sequences of 8000
+    // tokens, head_dim 128, 12 / 32 / 40 / 64 rows: 67 / 120 / 175 / 224 us against 135 / 141 / 139 / 142; 4 of 2000 tokens, 32 rows: 40 / 53; head_dim 64,
+    // 32 / 64 rows: 23 / 35 against 31 / 32; head_dim 256, 16 / 32 rows: 50 / 67 against 53 / 56.
+    const bool prompt = !one_each && mean > (d == 256 ? 24 : 32);
+    // Units of 8 rows where they suffice: 16 sequences of 8000 tokens, 8 rows 57 us against 66 with units of 16, 10 rows 96 against 67.
     const int rows = prompt ? prompt_rows(d) : mean <= 8 ? 8 : 16;
     l->unit_rows = rows;
     l->work.heads = group < rows ? group : rows;
@@ -635,26 +657,25 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     l->work.tile = prompt ? kPromptTile : kWarps * 16 * (d == 256 ? 1 : 2);
     l->work.group = group;
     l->work.kv_heads = a.cache.kv_heads;
-    l->work.least_share = 512 / l->work.tile;
+    // A CTA has at least so many tiles. One sequence of 32 heads: 1056 tokens 11.8 us with one tile of 128, 14.6 with two, 17.6 with four; many
+    // rows: 512 of a prompt 23.9 with four tiles of 64, 28.7 with two, 32.5 with eight, 8 pieces of 100 rows 30.3 / 27.9 / 47.4.
+    l->work.least_share = prompt ? 4 : 1;
     l->smem = (kWarps * rows * d + 2 * kWarps * rows) * 4;
+    l->sm_count = sm_count < kMostCtas / 3 ? sm_count : kMostCtas / 3;
     const int64_t units = (int64_t)a.rows.sequences * a.cache.kv_heads * l->work.parts;
-    l->split = !(one_each && a.rows.capacity <= 512);
-    l->ctas = l->split ? sm_count * (prompt ? 1 : rows == 8 && d <= 128 ? 3 : 2) : 0;
+    // One CTA per unit where the table has room for few tokens: shares and the second kernel take some microseconds. Tables of 200 / 512 /
+    // 1024 / 2048 tokens, one sequence of 32 heads: 6.0 / 8.7 / 14.2 / 25.1 us against 16.4 / 14.5 / 15.2 / 16.6; 16 sequences of 8 cache
+    // heads, 512 / 1024: 11.0 / 18.0 against 15.3 / 17.1.
+    l->split = !(one_each && a.rows.capacity <= 1024);
+    l->ctas = l->split ? l->sm_count * (prompt ? 1 : rows == 8 && d <= 128 ? 3 : 2) : 0;
     if (!l->split) {
         if (units > INT_MAX) return fail(MACKO_ERR_SIZE_OVERFLOW, "paged_attention: too many sequences and heads");
         l->ctas = (int)units;
     }
     l->work.ctas = l->ctas;
-    l->join_rows = units < l->ctas / 4 ? rows : rows / 8;
     l->split_bytes = l->split ? (int64_t)l->ctas * sizeof(SplitUnit) : 0;
     l->partial_bytes = l->split ? (int64_t)l->ctas * 2 * rows * (d + 2) * 4 : 0;
     return MACKO_OK;
-}
-
-template <bool BF16, int D>
-int launch_join(const AttentionArgs &a, const Launch &l, cudaStream_t s)
-{
-    return launch_pdl("paged_attention", join_kernel<BF16, D>, dim3(l.ctas, l.join_rows), dim3(256), 1, 0, s, a);
 }
 
 template <bool BF16, bool E4M3, int D, int RB>
@@ -669,7 +690,8 @@ int launch_few(const AttentionArgs &a, const Launch &l, cudaStream_t s)
     }
     if (e != cudaSuccess) return fail(MACKO_ERR_CUDA, "paged_attention: %s", cudaGetErrorString(e));
     if (int st = launch_pdl("paged_attention", few_rows_kernel<BF16, E4M3, D, RB>, dim3(l.ctas), dim3(kWarps * 32), 1, l.smem, s, a)) return st;
-    return l.split ? launch_join<BF16, D>(a, l, s) : MACKO_OK;
+    if (!l.split) return MACKO_OK;
+    return launch_pdl("paged_attention", join_kernel<BF16, D>, dim3(2 * l.sm_count), dim3(256), 1, 0, s, a);
 }
 
 template <bool BF16, bool E4M3, int D>

@@ -89,12 +89,12 @@ __device__ __forceinline__ void arrive(uint64_t *bar)
 }
 
 // Waits for the phase with parity `parity`; false (and from then on for every wait of the CTA) where it does not come. The thread
-// sleeps meanwhile, up to a millisecond at a time.
+// sleeps meanwhile, some microseconds at a time: the limit is a matter of seconds.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *given_up)
 {
     const uint32_t at = smem_address(bar);
 #pragma unroll 1
-    for (int i = 0; i < 4096; ++i) {
+    for (int i = 0; i < 1 << 20; ++i) {
         uint32_t done;
         asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(done) : "r"(at), "r"(parity), "r"(1000000u) : "memory");

@@ -449,6 +449,109 @@ def test_strided_q_and_qkv(rows, lengths):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 20, 90])
+def test_scales_of_the_softmax(d, n):
+    """Negative and zero ones: the largest weight may be that of the smallest product, and all weights may be the same."""
+    lengths = [n + 300, n + 1]
+    cache = Cache(lengths, 32, 2, d, torch.int8, seed=d + n)
+    for scale in (-0.25, 0.0, 1e-3):
+        _check_attend(cache, [n, n], lengths, 4, torch.float16, seed=1, scale=scale)
+        _check_attend(cache, [n, n], lengths, 4, torch.bfloat16, seed=2, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,hq", [(64, 300), (128, 257), (256, 130)])
+@pytest.mark.parametrize("n", [1, 3])
+def test_more_heads_than_a_unit_holds(d, hq, n):
+    lengths = [n + 70, n]
+    cache = Cache(lengths, 16, 1, d, torch.float8_e4m3fn, seed=d)
+    _check_attend(cache, [n, n], lengths, hq, torch.float16, seed=3, start="none" if n == 1 else "given")
+    _check_append(cache, [n, n], lengths, hq, torch.bfloat16, seed=4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_many_rows_of_no_sequence(d):
+    cache = Cache([40], 16, 2, d, torch.int8, seed=5)
+    out = _check_attend(cache, [40], [40], 4, torch.float16, seed=6, extra_rows=300)
+    assert bool((out[40:] == 0).all())
+    none, zero = torch.empty(0, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = torch.randn(500, 4, d, device="cuda").half()
+    assert bool((macko_spmv.paged_attention(q, cache.tensors, cache.table[:0], none, zero) == 0).all())
+    # rows in front of the first sequence's
+    lens, start = torch.tensor([40], dtype=torch.int32, device="cuda"), torch.tensor([460, 500], dtype=torch.int32, device="cuda")
+    late = macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start)
+    alone = macko_spmv.paged_attention(q[460:], cache.tensors, cache.table, lens, start - 460)
+    assert bool((late[:460] == 0).all()) and torch.allclose(late[460:].float(), alone.float(), rtol=2e-3, atol=2e-3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_many_sizes_of_prompts(d):
+    """Every number of tiles, of rows in the last unit and of pieces that a few hundred rows can have; twice, since what several warps hand one
+    another must not depend on who is first."""
+    for n in (41, 64, 65, 127, 128, 129, 190, 192, 255, 256, 257, 320, 385, 511, 700):
+        for before in (0, 1, 63, 64, 500):
+            lengths = [n + before, n]
+            cache = Cache(lengths, 64, 1, d, torch.int8, seed=n)
+            lens, start = torch.tensor(lengths, dtype=torch.int32, device="cuda"), _starts([n, n])
+            q = torch.randn(2 * n, 2, d, generator=_gen(n), device="cuda").half()
+            first = macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start)
+            assert torch.equal(first, macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start))
+            _check_attend(cache, [n, n], lengths, 2, torch.float16, seed=n, q=q)
+
+
+@pytest.mark.gpu
+def test_plain_calls_and_the_operators_agree():
+    lengths = [300, 17, 64]
+    a, b = (Cache(lengths, 16, 2, 64, torch.int8, seed=55) for _ in range(2))
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    cos, sin = _tables(a.table.shape[1] * 16, 64)
+    qkv = torch.randn(3, 8 * 64, generator=_gen(56), device="cuda").half()
+    versions = [t._version for t in a.tensors]
+    q = macko_spmv.rope_append(qkv, cos, sin, a.tensors, a.table, lens)
+    assert all(t._version > v for t, v in zip(a.tensors, versions))          # PyTorch knows that the cache was written
+    r = torch.ops.macko_spmv.rope_append(qkv, cos, sin, *b.tensors, b.table, lens)
+    assert torch.equal(q, r) and all(torch.equal(x, y) for x, y in zip(a.copy(), b.copy()))
+    out = macko_spmv.paged_attention(q, a.tensors, a.table, lens)
+    assert torch.equal(out, torch.ops.macko_spmv.paged_attention(q, *b.tensors, b.table, lens))
+    assert torch.equal(out, macko_spmv.paged_attention(q, macko_spmv.KVCache(*a.tensors), a.table, lens, None, 0.125))
+    assert torch.equal(out, macko_spmv.paged_attention(q, list(a.tensors), a.table, lens, scale=0.125))
+
+
+@pytest.mark.gpu
+def test_from_two_threads_at_once():
+    import threading
+
+    lengths = [2000, 900]
+    cache = Cache(lengths, 32, 4, 128, torch.int8, seed=57)
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    qs = [torch.randn(2, 8, 128, generator=_gen(58 + i), device="cuda").half() for i in range(2)]
+    many = torch.randn(400, 8, 128, generator=_gen(60), device="cuda").half()
+    start = torch.tensor([0, 300, 400], dtype=torch.int32, device="cuda")
+    expected = [macko_spmv.paged_attention(q, cache.tensors, cache.table, lens) for q in qs]
+    expected_many = macko_spmv.paged_attention(many, cache.tensors, cache.table, lens, start)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                out = macko_spmv.paged_attention(qs[i], cache.tensors, cache.table, lens)
+                all_rows = macko_spmv.paged_attention(many, cache.tensors, cache.table, lens, start)
+                stream.synchronize()
+                if not (torch.equal(out, expected[i]) and torch.equal(all_rows, expected_many)):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
+
+
+@pytest.mark.gpu
 def test_nothing_to_do():
     cache = Cache([16], 16, 2, 64, torch.int8, seed=42)
     cos, sin = _tables(16, 64)
@@ -664,7 +767,7 @@ def test_refusals_of_the_c_entries():
     for call in (append, attend):
         for change, status in ((dict(k=None), bad), (dict(v_scale=None), bad), (dict(page_size=8), bad), (dict(page_size=48), bad), (dict(head_dim=96), bad),
                                (dict(code=2), bad), (dict(pages=0), bad), (dict(kv_heads=0), bad), (dict(k_page_stride=2047), bad), (dict(v_scale_stride=1), bad),
-                               (dict(k=at + 8), askew), (dict(k_page_stride=2056), askew), (dict(v_scale=at + 2), askew), (dict(pages=1 << 31), large)):
+                               (dict(k=at + 8), askew), (dict(k_page_stride=2056), askew), (dict(v_scale=at + 2), askew), (dict(pages=1 << 31), large), (dict(k_page_stride=1 << 35), large)):
             assert call(cache(**change), rows()) == status, change
         for change, status in ((dict(rows=4), bad), (dict(rows=-1), bad), (dict(sequences=-1), bad), (dict(lengths=None), bad), (dict(page_table=None), bad),
                                (dict(table_stride=3), bad), (dict(lengths=at + 2), askew), (dict(query_start=at + 1), askew), (dict(table_width=1 << 27), large),
