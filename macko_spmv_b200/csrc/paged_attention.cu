@@ -11,7 +11,12 @@
 // layout that mma.m16n8k16 wants: tokens (for S^T = K Q^T) and dimensions (for O^T = V^T P^T) are its 16 rows, the call's rows its 8 columns, so that
 // one step costs half of what it would the other way round. Which dimensions are "k = 2t, 2t + 1" is free as long as K and Q agree, so a
 // lane loads 16 consecutive bytes of a token; bytes of two tokens are interleaved for V. The next K is asked for when this one has been
-// converted, and V alike, so a warp has its 8 KB in flight all the time.
+// converted, and V alike, so a warp has its 8 KB in flight all the time; the turn behind that is on its way to the L2 cache.
+//
+// 64 sequences of up to 4096 tokens, 32 heads of 128, e4m3: 274 us, 4.3 TB/s, 0.66 of what a copy moves; 131072 tokens, 8 cache heads: 60 us,
+// 4.5 TB/s. 32 tokens take a warp some 550 instructions, 160 of them conversions and byte interleaving, and 168 registers leave room for 12
+// warps of an SM, which issue 0.35 to 0.4 instructions a cycle and scheduler: more warps with 16 tokens each (16 warps: 260 and 66 us) or fewer
+// with all registers (299 and 62 us) are no faster on the whole.
 #include <climits>
 
 #include "attention_args.cuh"

@@ -17,6 +17,12 @@
 // the softmax of this one is done. (With one S of 128 columns a half waited for its P to go through the tensor core and for the next S,
 // 1900 of 5400 cycles for 128 tokens.)
 //
+// 4 pieces of up to 512 rows over up to 16384 tokens, 32/8 heads of 128, int8: 333 us, 805 TFLOP/s (0.48 of a cuBLAS product in a burst);
+// a 4096-token prompt, 32 heads, e4m3: 244 us, 563 TFLOP/s. The tensor pipe is active 40 % of the time, a scheduler issues 0.56 instructions
+// a cycle, 1430 for a tile. What bounds it is the chain from S through a half's softmax and P to the next S: with neither softmax
+// arithmetic nor conversions the first case still takes 279 us, without the products as well 182 (a wait for what is there already takes
+// 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other ways of waiting, P in 32-column pieces.
+//
 // Every wait has a limit: if one runs out, no further wait waits, and what the CTA writes from then on is NaN.
 #include "attention_args.cuh"
 #include "launch.cuh"
