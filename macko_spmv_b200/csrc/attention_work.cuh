@@ -94,7 +94,7 @@ __device__ __forceinline__ long long quotient(long long a, long long b)   // of 
     return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
 }
 
-// Walks the pieces of CTA `cta`. All lanes of a warp call start(); next() is each thread's own.
+// Walks the pieces of CTA `cta`. All lanes of a warp walk together.
 struct WorkWalk {
     long long at, end, share;
     int cta, sequence, head_part, block, tile;   // where the walk is; tile: of the unit
@@ -107,6 +107,7 @@ struct WorkWalk {
         // the total, then the sequence with this CTA's first tile
         long long total = 0, first_own = 0;
         Sequence first_rows = {0, 0, 0};
+#pragma unroll 4
         for (int i = lane; i < r.sequences; i += 32) {
             const Sequence rows = sequence_at(r, i);
             const long long own = sequence_tiles(w, r, rows);
@@ -173,12 +174,17 @@ struct WorkWalk {
         tile = (int)(rest - before);
     }
 
-    // The next piece, or false.
+    // The next piece, or false. All lanes of a warp call it together, like start().
     __device__ bool next(const WorkShape &w, const RowsView &r, Piece &p)
     {
         if (at >= end) return false;
         while (s.blocks == 0 || head_part >= w.kv_heads * w.parts) {
-            if (++sequence >= r.sequences) return false;
+            // the next sequence that has rows: a padded batch may have many without
+            const int other = sequence + 1 + (int)(threadIdx.x & 31);
+            const uint32_t with_rows = __ballot_sync(0xffffffffu, other < r.sequences && sequence_at(r, other).count > 0);
+            sequence += with_rows != 0 ? __ffs(with_rows) : 32;
+            if (sequence >= r.sequences) return false;
+            if (with_rows == 0) continue;
             s = sequence_work(w, r, sequence_at(r, sequence));
             head_part = block = tile = 0;
         }

@@ -15,8 +15,8 @@
 //
 // 64 sequences of up to 4096 tokens, 32 heads of 128, e4m3: 274 us, 4.3 TB/s, 0.66 of what a copy moves; 131072 tokens, 8 cache heads: 60 us,
 // 4.5 TB/s. 32 tokens take a warp some 550 instructions, 160 of them conversions and byte interleaving, and 168 registers leave room for 12
-// warps of an SM, which issue 0.35 to 0.4 instructions a cycle and scheduler: more warps with 16 tokens each (16 warps: 260 and 66 us) or fewer
-// with all registers (299 and 62 us) are no faster on the whole.
+// warps of an SM, which issue 0.35 to 0.4 instructions a cycle and scheduler: more warps with 16 tokens each (16 warps: 260 and 66 us, with 272 and
+// 63 then for these) or fewer with all registers (299 and 62 us) are no faster on the whole.
 #include <climits>
 
 #include "attention_args.cuh"

@@ -21,7 +21,7 @@
 // a 4096-token prompt, 32 heads, e4m3: 244 us, 563 TFLOP/s. The tensor pipe is active 40 % of the time, a scheduler issues 0.56 instructions
 // a cycle, 1430 for a tile. What bounds it is the chain from S through a half's softmax and P to the next S: with neither softmax
 // arithmetic nor conversions the first case still takes 279 us, without the products as well 182 (a wait for what is there already takes
-// 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other ways of waiting, P in 32-column pieces.
+// 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other ways of waiting.
 //
 // Every wait has a limit: if one runs out, no further wait waits, and what the CTA writes from then on is NaN.
 #include "attention_args.cuh"

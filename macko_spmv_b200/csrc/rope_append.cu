@@ -133,7 +133,9 @@ rope_append_kernel(const AppendArgs a)
         // way to memory; the others' rows are nearly always its own.
         const long long base = (long long)((int)blockIdx.x - a.page_blocks) * blockDim.x * a.query_items / kPerRow;   // row and head
         const int row0 = (int)(base / hq), head0 = (int)(base % hq);
+        int behind = r.rows;   // rows from here on belong to no sequence
         if (r.start != nullptr) {
+            behind = r.sequences > 0 ? __ldcg(r.start + r.sequences) : 0;
             if (tid == 0) found[0] = r.sequences;
             __syncthreads();
             for (int i = tid; i < r.sequences; i += blockDim.x) {
@@ -155,7 +157,7 @@ rope_append_kernel(const AppendArgs a)
             const int item = i * (int)blockDim.x + tid, part = item % kPerRow, row_head = head0 + item / kPerRow;
             const int row = row0 + row_head / hq, head = row_head % hq;
             int position = -1;
-            if (row < r.rows) {
+            if (row < min(r.rows, behind)) {
                 Sequence s = {0, 0, 0};
                 if (r.start == nullptr) {
                     s = sequence_at(r, row);

@@ -853,3 +853,15 @@ def test_generate_batch():
             _model(**bad)
     with pytest.raises(RuntimeError):
         _model().extend(prompts[0], None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 50])
+def test_padded_batches(n):
+    """Many sequences without rows, between others and at the end, and rows behind the last one's: what a batch of fixed size is padded with."""
+    rows = [0] * 40 + [n] + [0] * 70 + [n, 2, 0, 1] + [0] * 200
+    lengths = [(r + 20 if r else 0) for r in rows]
+    cache = Cache(lengths, 16, 2, 64, torch.int8, seed=61)
+    _check_append(cache, rows, lengths, 4, torch.float16, seed=62, extra_rows=77)
+    out = _check_attend(cache, rows, lengths, 4, torch.float16, seed=63, extra_rows=77)
+    assert bool((out[sum(rows):] == 0).all())
