@@ -3,10 +3,11 @@
 // A unit is one head of the cache and the rows of one sequence that meet it together: `queries` consecutive rows of the call with `heads`
 // heads each (a group of more heads than a unit holds is cut into `parts`). It walks the tokens in tiles of `tile`. Units of a sequence
 // are ordered by (head, part), then by rows; block b of the rows ends at position begin + (b + 1) * queries - 1 and takes
-// ceil((begin + (b + 1) * queries) / tile) tiles. All tiles of the call in this order are numbered; CTA c takes numbers
-// [c * share, (c + 1) * share). So every CTA has the same work whatever the lengths are, a unit lies in consecutive CTAs, and a
-// CTA has at most two units that are not its own alone: the one that began before it and the one that goes on after it. Their
-// partial results (maximum, sum, weighted values, fp32) go to scratch memory, and a second small kernel puts them together.
+// ceil((begin + (b + 1) * queries) / tile) tiles. All tiles of the call in this order are numbered, and in front of each unit's tiles
+// `extra` numbers stand for what a unit costs whatever its length is; CTA c takes numbers [c * share, (c + 1) * share). So every CTA has
+// the same work whatever the lengths are, a unit's tiles lie in consecutive CTAs, and a CTA has at most two units that are not its own
+// alone: the one that began before it and the one that goes on after it. Their partial results (maximum, sum, weighted values, fp32) go
+// to scratch memory, and a second small kernel puts them together.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -18,6 +19,7 @@ struct WorkShape {
     int tile;                    // tokens
     int group, kv_heads;         // heads per cache head, cache heads
     int ctas, least_share;
+    int extra;                   // numbers that a unit has in front of its tiles, for the time that it takes whatever its length is
 };
 
 // Rows of a unit that goes on in the CTAs behind: what the second kernel needs. pieces 0: nothing.
@@ -50,12 +52,13 @@ __host__ __device__ __noinline__ inline long long floor_sum(unsigned n, unsigned
     return (long long)sum;
 }
 
-// Tiles of the first `blocks` row blocks of a sequence whose rows begin at position `begin`, for one (head, part).
+// Numbers of the first `blocks` row blocks of a sequence whose rows begin at position `begin`, for one (head, part).
 __host__ __device__ inline long long tiles_before(const WorkShape &w, int begin, int blocks)
 {
     if (blocks == 0) return 0;
-    if (blocks == 1) return ((long long)begin + w.queries + w.tile - 1) / w.tile;
-    return floor_sum(blocks, w.tile, w.queries, (unsigned)begin + w.queries + w.tile - 1);
+    const long long extra = (long long)w.extra * blocks;
+    if (blocks == 1) return ((long long)begin + w.queries + w.tile - 1) / w.tile + extra;
+    return floor_sum(blocks, w.tile, w.queries, (unsigned)begin + w.queries + w.tile - 1) + extra;
 }
 
 #ifdef __CUDACC__
@@ -97,7 +100,7 @@ __device__ __forceinline__ long long quotient(long long a, long long b)   // of 
 // Walks the pieces of CTA `cta`. All lanes of a warp walk together.
 struct WorkWalk {
     long long at, end, share;
-    int cta, sequence, head_part, block, tile;   // where the walk is; tile: of the unit
+    int cta, sequence, head_part, block, tile;   // where the walk is; tile: of the unit's numbers, the extra ones first
     SequenceWork s;
 
     __device__ void start(const WorkShape &w, const RowsView &r, int of_cta)
@@ -188,18 +191,23 @@ struct WorkWalk {
             s = sequence_work(w, r, sequence_at(r, sequence));
             head_part = block = tile = 0;
         }
-        const int of_unit = (int)(((long long)s.begin + (long long)(block + 1) * w.queries + w.tile - 1) / w.tile);
+        const int of_unit = (int)(((long long)s.begin + (long long)(block + 1) * w.queries + w.tile - 1) / w.tile) + w.extra;
+        const int taken = (int)min((long long)max(of_unit - tile, 0), end - at);
+        if (tile + taken <= w.extra) {   // the unit's first tile is the next CTA's
+            at = end;
+            return false;
+        }
         p.sequence = sequence;
         p.block = block;
         p.kv_head = head_part / w.parts;
         p.part = head_part % w.parts;
-        p.first_tile = tile;
-        p.tiles = (int)min((long long)max(of_unit - tile, 0), end - at);
-        p.begins = tile == 0;
-        p.ends = tile + p.tiles >= of_unit;
-        p.pieces = p.begins ? p.ends ? 1 : (int)(quotient(at + of_unit - 1, share) - cta) + 1 : 0;
-        at += p.tiles;
-        tile += p.tiles;
+        p.first_tile = max(tile - w.extra, 0);
+        p.tiles = tile + taken - w.extra - p.first_tile;
+        p.begins = tile <= w.extra;
+        p.ends = tile + taken >= of_unit;
+        p.pieces = p.begins ? p.ends ? 1 : (int)(quotient(at + of_unit - tile - 1, share) - cta) + 1 : 0;
+        at += taken;
+        tile += taken;
         if (p.ends) {
             tile = 0;
             if (++block == s.blocks) {

@@ -665,6 +665,11 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     // A CTA has at least so many tiles. One sequence of 32 heads: 1056 tokens 11.8 us with one tile of 128, 14.6 with two, 17.6 with four; many
     // rows: 512 of a prompt 23.9 with four tiles of 64, 28.7 with two, 32.5 with eight, 8 pieces of 100 rows 30.3 / 27.9 / 47.4.
     l->work.least_share = prompt ? 4 : 1;
+    // What a unit costs by itself (its rows, the first loads, its epilogue) is that of some 256 tokens more. With 0 / 128 / 256 / 384 tokens,
+    // us: 64 sequences of 205 to 4096 tokens, 32 heads of 128, 273 / 223 / 201 / 202; of 8 heads of 64 up to 2048 tokens 45 / 32 / 29 / 29;
+    // of 8 heads of 256, 256 tokens 113, 384 109. Many rows, 0 / 128 / 256 / 512: a prompt of 4096, 237 / 222 / 213 / 215; 32 pieces of up to 40
+    // rows 69 / 51 / 50 / 54.
+    l->work.extra = 256 / l->work.tile;
     l->smem = (kWarps * rows * d + 2 * kWarps * rows) * 4;
     l->sm_count = sm_count < kMostCtas / 3 ? sm_count : kMostCtas / 3;
     const int64_t units = (int64_t)a.rows.sequences * a.cache.kv_heads * l->work.parts;
