@@ -13,10 +13,10 @@
 // lane loads 16 consecutive bytes of a token; bytes of two tokens are interleaved for V. The next K is asked for when this one has been
 // converted, and V alike, so a warp has its 8 KB in flight all the time; the turn behind that is on its way to the L2 cache.
 //
-// 64 sequences of up to 4096 tokens, 32 heads of 128, e4m3: 274 us, 4.3 TB/s, 0.66 of what a copy moves; 131072 tokens, 8 cache heads: 60 us,
+// 64 sequences of 205 to 4096 tokens, 32 heads of 128, e4m3: 226 us, 5.2 TB/s, 0.80 of what a copy moves; 131072 tokens, 8 cache heads: 60 us,
 // 4.5 TB/s. 32 tokens take a warp some 550 instructions, 160 of them conversions and byte interleaving, and 168 registers leave room for 12
-// warps of an SM, which issue 0.35 to 0.4 instructions a cycle and scheduler: more warps with 16 tokens each (16 warps: 260 and 66 us, with 272 and
-// 63 then for these) or fewer with all registers (299 and 62 us) are no faster on the whole.
+// warps of an SM. 16 warps with 16 tokens each and q in shared memory are no faster: sequences of equal length, 64 of 4096 tokens 348 against 343 us, 8192
+// tokens of one sequence 17.7 against 14.8.
 #include <climits>
 
 #include "attention_args.cuh"
@@ -650,10 +650,11 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     // rows that a head of the cache meets in a sequence, as far as the host knows: on average
     const int64_t mean = one_each ? group : ((int64_t)a.rows.rows * group + a.rows.sequences - 1) / (a.rows.sequences > 0 ? a.rows.sequences : 1);
     // The kernel for many rows takes 128 or 256 as long as one; the other reads and converts the cache once for 16. 16 sequences of 8000
-    // tokens, head_dim 128, 12 / 32 / 40 / 64 rows: 67 / 120 / 175 / 224 us against 135 / 141 / 139 / 142; 4 of 2000 tokens, 32 rows: 40 / 53; head_dim 64,
-    // 32 / 64 rows: 23 / 35 against 31 / 32; head_dim 256, 16 / 32 rows: 50 / 67 against 53 / 56.
+    // tokens, head_dim 128, 12 / 32 / 40 / 64 rows: 69 / 128 / 180 / 235 us against 134 / 141 / 142 / 142; 4 of 2000, 32 rows: 21 / 26; head_dim 64,
+    // 32 / 40 / 64 rows: 92 / 131 / 170 against 122 / 123 / 124; head_dim 256, 16 / 24 / 32 rows: 158 / 286 / 290 against 202 / 206 / 208, and 24 rows of
+    // 1 of 8000, 4 of 2000, 16 of 1000: 36 / 38 / 65 against 65 / 39 / 50.
     const bool prompt = !one_each && mean > (d == 256 ? 24 : 32);
-    // Units of 8 rows where they suffice: 16 sequences of 8000 tokens, 8 rows 57 us against 66 with units of 16, 10 rows 96 against 67.
+    // Units of 8 rows where they suffice: 16 sequences of 8000 tokens, 8 rows 58 us against 68 with units of 16, 10 rows 97 against 69.
     const int rows = prompt ? prompt_rows(d) : mean <= 8 ? 8 : 16;
     l->unit_rows = rows;
     l->work.heads = group < rows ? group : rows;
@@ -662,8 +663,8 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     l->work.tile = prompt ? kPromptTile : kWarps * 16 * (d == 256 ? 1 : 2);
     l->work.group = group;
     l->work.kv_heads = a.cache.kv_heads;
-    // A CTA has at least so many tiles. One sequence of 32 heads: 1056 tokens 11.8 us with one tile of 128, 14.6 with two, 17.6 with four; many
-    // rows: 512 of a prompt 23.9 with four tiles of 64, 28.7 with two, 32.5 with eight, 8 pieces of 100 rows 30.3 / 27.9 / 47.4.
+    // A CTA has at least so many numbers. One sequence of 32 heads: 1056 tokens 12.1 us with one (128 tokens), 13.6 with two, 16.7 with four; many
+    // rows: 512 of a prompt 25.4 with four (of 64 tokens) or two, 27.6 with eight, 8 pieces of 100 rows 17.9 / 18.2 / 23.6.
     l->work.least_share = prompt ? 4 : 1;
     // What a unit costs by itself (its rows, the first loads, its epilogue) is that of some 256 tokens more. With 0 / 128 / 256 / 384 tokens,
     // us: 64 sequences of 205 to 4096 tokens, 32 heads of 128, 273 / 223 / 201 / 202; of 8 heads of 64 up to 2048 tokens 45 / 32 / 29 / 29;
@@ -674,8 +675,8 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     l->sm_count = sm_count < kMostCtas / 3 ? sm_count : kMostCtas / 3;
     const int64_t units = (int64_t)a.rows.sequences * a.cache.kv_heads * l->work.parts;
     // One CTA per unit where the table has room for few tokens: shares and the second kernel take some microseconds. Tables of 200 / 512 /
-    // 1024 / 2048 tokens, one sequence of 32 heads: 6.0 / 8.7 / 14.2 / 25.1 us against 16.4 / 14.5 / 15.2 / 16.6; 16 sequences of 8 cache
-    // heads, 512 / 1024: 11.0 / 18.0 against 15.3 / 17.1.
+    // 1024 / 2048 tokens, one sequence of 32 heads: 6.0 / 8.7 / 14.2 / 25.1 us against 11.4 / 11.6 / 12.1 / 14.4; 16 sequences of 8 cache
+    // heads, 512 / 1024: 10.7 / 17.2 against 14.2 / 16.5; 64 such: 16.0 / 25.3 against 21.9 / 27.0.
     l->split = !(one_each && a.rows.capacity <= 1024);
     l->ctas = l->split ? l->sm_count * (prompt ? 1 : rows == 8 && d <= 128 ? 3 : 2) : 0;
     if (!l->split) {

@@ -18,7 +18,7 @@
 // 1900 of 5400 cycles for 128 tokens.)
 //
 // 4 pieces of up to 512 rows over up to 16384 tokens, 32/8 heads of 128, int8: 333 us, 805 TFLOP/s (0.48 of a cuBLAS product in a burst);
-// a 4096-token prompt, 32 heads, e4m3: 244 us, 563 TFLOP/s. The tensor pipe is active 40 % of the time, a scheduler issues 0.56 instructions
+// a 4096-token prompt, 32 heads, e4m3: 216 us, 636 TFLOP/s. The tensor pipe is active 40 % of the time, a scheduler issues 0.56 instructions
 // a cycle, 1430 for a tile. What bounds it is the chain from S through a half's softmax and P to the next S: with neither softmax
 // arithmetic nor conversions the first case still takes 279 us, without the products as well 182 (a wait for what is there already takes
 // 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other ways of waiting.

@@ -865,3 +865,14 @@ def test_padded_batches(n):
     _check_append(cache, rows, lengths, 4, torch.float16, seed=62, extra_rows=77)
     out = _check_attend(cache, rows, lengths, 4, torch.float16, seed=63, extra_rows=77)
     assert bool((out[sum(rows):] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 60])
+def test_short_sequences_next_to_long_ones(n, d):
+    """Shares of work that end in, before and behind a short unit's only tile, with long units between."""
+    rows = [n] * 25 + [1] + [n] * 12
+    lengths = [n + 1 + i % 3 for i in range(10)] + [5000, n] + [n + 130 * i for i in range(13)] + [1, 2100] + [n + i for i in range(11)]
+    cache = Cache(lengths, 32, 2, d, torch.float8_e4m3fn, seed=71)
+    _check_attend(cache, rows, lengths, 4, torch.float16, seed=72)
