@@ -24,6 +24,8 @@
 // 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other ways of waiting.
 //
 // Every wait has a limit: if one runs out, no further wait waits, and what the CTA writes from then on is NaN.
+#include <type_traits>
+
 #include "attention_args.cuh"
 #include "launch.cuh"
 
@@ -35,6 +37,7 @@ constexpr int kTile = kPromptTile;
 constexpr int kGroups = kTile / 16;     // blocks of 16 tokens: each lies on one page
 constexpr int kConstSlots = 16;         // scales are fetched at most 9 tiles ahead of the softmax (codes, K, S)
 constexpr float kLeastFactor = 1e-36f;  // a score times nothing is still minus infinity where it is masked
+constexpr float kFar = 1048576.f;       // 2^20, where steps of fp32 are an eighth
 constexpr int kWorkers = 19;            // warps that are given the CTA's pieces
 
 // Shared memory, from a 1024-byte boundary: Q of the halves, K and V stages, each as [64 dimensions][rows][128 bytes]; codes of K and V.
@@ -406,6 +409,7 @@ prompt_kernel(const AttentionArgs a)
                 const int limit = there ? min(u.begin + query + 1, r.capacity) : 0;           // tokens that this row sees
                 const int all_see = min(u.begin + 128 * half / u.heads + 1, r.capacity);      // that every row of this half sees
                 float m = -INFINITY, l = 0.f;
+                bool far = false;   // a row of the warp has a maximum from 2^20 on
 #pragma unroll 1
                 for (int j = h.first; j < h.end[half]; ++j) {
                     const int count = done + j - h.first, buffer = count & 1;
@@ -433,10 +437,11 @@ prompt_kernel(const AttentionArgs a)
                         top = max3(top, x[14], x[15]);
                         most = fmaxf(most, fmaf(fmaxf(top, top2), fmaxf(k.x * factor, kLeastFactor), k.y));
                     }
-                    const bool grown = most > m + 8.f || (m == -INFINITY && most > m);
+                    const bool grown = most - m > 8.f;   // the difference of numbers that are near one another is exact
                     if (__any_sync(0xffffffffu, grown)) {
                         const float keep = grown ? exp2_fast(m - most) : 1.f;
                         if (grown) m = most;
+                        far = __any_sync(0xffffffffu, m > kFar || (m < -kFar && m > -INFINITY));
                         l *= keep;
                         if (j > h.first) {
                             wait(bars + kODone + 2 * half + (buffer ^ 1), ((count - 1) >> 1) & 1, given_up);
@@ -454,29 +459,37 @@ prompt_kernel(const AttentionArgs a)
                         }
                     }
                     const float base = m == -INFINITY ? 0.f : m;
+                    // 2^x below takes the product's own rounding and that of k.y - base for nothing, which holds as long as fp32 has fractions of the
+                    // maximum. Beyond, x is what the maximum was found from, less the maximum: nothing is larger than 8 then either.
+                    auto weights = [&](auto is_far) {
+                        constexpr bool kIsFar = decltype(is_far)::value;
 #pragma unroll
-                    for (int two = 0; two < 2; ++two) {
-                        uint32_t p[16];
+                        for (int two = 0; two < 2; ++two) {
+                            uint32_t p[16];
 #pragma unroll
-                        for (int gg = 0; gg < 2; ++gg) {
-                            const int g = 2 * two + gg;
-                            const float4 k = of_tile[g];
-                            const float by = fmaxf(k.x * factor, kLeastFactor), plus = k.y - base;
-                            const uint64_t by2 = pair(by, by), plus2 = pair(plus, plus);
-                            uint64_t sum[2] = {0ull, 0ull};
+                            for (int gg = 0; gg < 2; ++gg) {
+                                const int g = 2 * two + gg;
+                                const float4 k = of_tile[g];
+                                const float by = fmaxf(k.x * factor, kLeastFactor), plus = k.y - base;
+                                const uint64_t by2 = pair(by, by), plus2 = kIsFar ? pair(k.y, k.y) : pair(plus, plus);
+                                uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                const float2 x = unpair(fma_pair(pair(s[16 * g + i], s[16 * g + i + 1]), by2, plus2));
-                                const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
-                                sum[(i >> 1) & 1] = add_pair(sum[(i >> 1) & 1], pair(e0, e1));
-                                p[8 * gg + i / 2] = pack2<false>(e0, e1);
+                                for (int i = 0; i < 16; i += 2) {
+                                    float2 x = unpair(fma_pair(pair(s[16 * g + i], s[16 * g + i + 1]), by2, plus2));
+                                    if (kIsFar) x = make_float2(x.x - base, x.y - base);
+                                    const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
+                                    sum[(i >> 1) & 1] = add_pair(sum[(i >> 1) & 1], pair(e0, e1));
+                                    p[8 * gg + i / 2] = pack2<false>(e0, e1);
+                                }
+                                const float2 both = unpair(add_pair(sum[0], sum[1]));
+                                const float all = both.x + both.y;
+                                l += all == 0.f ? 0.f : all * k.z;   // tokens that a row does not see may have any scale
                             }
-                            const float2 both = unpair(add_pair(sum[0], sum[1]));
-                            const float all = both.x + both.y;
-                            l += all == 0.f ? 0.f : all * k.z;   // tokens that a row does not see may have any scale
+                            tmem_store16(s_at + 16 * two, p);
                         }
-                        tmem_store16(s_at + 16 * two, p);
-                    }
+                    };
+                    if (far) weights(std::true_type());
+                    else weights(std::false_type());
                     tmem_store_wait();
                     fence_before();
                     arrive(bars + kPFull + 2 * half + buffer);
