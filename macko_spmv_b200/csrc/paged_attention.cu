@@ -1,11 +1,12 @@
 // Attention over the paged 8-bit cache, for a few rows per sequence and head of the cache: decoding and drafted tokens.
 //
 //   x(t) = scale * (q . k_t) * k_scale(page) * log2 e + log2 v_scale(page)        k_t, v_t: codes
-//   out  = sum 2^(x(t) - m) v_t  /  sum 2^(x(t) - m) / v_scale(page),             m = max x(t)
+//   out  = sum 2^(x(t) - m) v_t  /  sum 2^(x(t) - m) / v_scale(page),             m = max x(t) - 15
 //
-// The scale of the values is part of the exponent, so the weights that meet the codes are at most 1 whatever the scales are, and
-// rounding them to fp16 (2^-11 of themselves) is the one rounding on the way; sums, maxima and the accumulators are fp32. Products of
-// codes with fp16 are exact in the tensor core. bfloat16 rows of q become fp16 under a power of two of their own.
+// The scale of the values is part of the exponent, so the weights that meet the codes are at most 2^15 whatever the scales are. Rounding them to
+// fp16 is the one rounding on the way: 2^-11 of a weight down to 2^-29 of the row's largest, 2^-40 of the largest below (with the largest at 1 it
+// would be 2^-25 of it: of 30000 tokens that share a tenth of a row's weight, a hundredth was lost); sums, maxima and the accumulators are fp32. Products
+// of codes with fp16 are exact in the tensor core. bfloat16 rows of q become fp16 under a power of two of their own.
 //
 // Bound by HBM: a code is used for 2 to 16 rows. A warp takes 16 or 32 tokens at a time from the cache straight into registers, in the
 // layout that mma.m16n8k16 wants: tokens (for S^T = K Q^T) and dimensions (for O^T = V^T P^T) are its 16 rows, the call's rows its 8 columns, so that
@@ -28,6 +29,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kAhead = 1;   // turns of a warp between asking for its tokens and loading them
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kTop = 15.f;   // exponent of the largest weight: fp16 ends at 2^16
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
@@ -331,7 +333,7 @@ few_rows_kernel(const AttentionArgs a)
                     float &v = top[nb][i];
 #pragma unroll
                     for (int s = 4; s < 32; s <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, s));
-                    v = fmaxf(v, m[nb][i]);
+                    v = fmaxf(__fadd_ru(v, -kTop), m[nb][i]);   // up: a weight is at most 2^15 also where fp32 has no such difference
                     base[nb][i] = v == -INFINITY ? 0.f : v;
                     keep[nb][i] = exp2_fast(m[nb][i] - base[nb][i]);
                     grown |= v != m[nb][i];

@@ -7,7 +7,8 @@
 // of the call times heads of a group) in two halves of 128, tiles of 64 tokens. Five groups of warps:
 //
 //   0, 1   softmax of one half each, one row per thread: S from tensor memory, maximum, 2^x, P as fp16 over S in tensor memory; the
-//          accumulator is rescaled there when the maximum has grown by more than 8 (so weights are at most 2^8 and none is lost)
+//          accumulator is rescaled there when the maximum has grown by more than kLag, so that a row's largest weight is 2^11 to 2^15: fp16 rounds
+//          weights by 2^-11 of themselves down to 2^-25 of the largest, by 2^-36 of the largest below
 //   2, 3   keys and values: codes from shared memory to fp16 (exact) in shared memory, in the 128-byte swizzle, three stages each
 //   4      one warp for each half that issues its tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it
 //          lies (token by token: its "N" dimension is the contiguous one); two that fetch the codes of 16 tokens at a time with bulk
@@ -37,6 +38,7 @@ constexpr int kTile = kPromptTile;
 constexpr int kGroups = kTile / 16;     // blocks of 16 tokens: each lies on one page
 constexpr int kConstSlots = 16;         // scales are fetched at most 9 tiles ahead of the softmax (codes, K, S)
 constexpr float kLeastFactor = 1e-36f;  // a score times nothing is still minus infinity where it is masked
+constexpr float kTop = 15.f, kLag = 4.f;  // exponents of the largest weight, which fp16 ends behind, and of what a maximum may lag (8, 4 and 2: the same time)
 constexpr float kFar = 1048576.f;       // 2^20, where steps of fp32 are an eighth
 constexpr int kWorkers = 19;            // warps that are given the CTA's pieces
 
@@ -437,10 +439,10 @@ prompt_kernel(const AttentionArgs a)
                         top = max3(top, x[14], x[15]);
                         most = fmaxf(most, fmaf(fmaxf(top, top2), fmaxf(k.x * factor, kLeastFactor), k.y));
                     }
-                    const bool grown = most - m > 8.f;   // the difference of numbers that are near one another is exact
+                    const bool grown = most - m > kTop;   // the difference of numbers that are near one another is exact
                     if (__any_sync(0xffffffffu, grown)) {
-                        const float keep = grown ? exp2_fast(m - most) : 1.f;
-                        if (grown) m = most;
+                        const float to = grown ? __fadd_ru(most, kLag - kTop) : m, keep = grown ? exp2_fast(m - to) : 1.f;
+                        m = to;
                         far = __any_sync(0xffffffffu, m > kFar || (m < -kFar && m > -INFINITY));
                         l *= keep;
                         if (j > h.first) {
@@ -460,7 +462,7 @@ prompt_kernel(const AttentionArgs a)
                     }
                     const float base = m == -INFINITY ? 0.f : m;
                     // 2^x below takes the product's own rounding and that of k.y - base for nothing, which holds as long as fp32 has fractions of the
-                    // maximum. Beyond, x is what the maximum was found from, less the maximum: nothing is larger than 8 then either.
+                    // maximum. Beyond, x is what the maximum was found from, less m: nothing is above 2^15 then either.
                     auto weights = [&](auto is_far) {
                         constexpr bool kIsFar = decltype(is_far)::value;
 #pragma unroll
