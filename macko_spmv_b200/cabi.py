@@ -107,6 +107,7 @@ SIGNATURES = {
     "macko_cache_rope_append": (_int, [ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp]),
     "macko_cache_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32]),
     "macko_cache_attention": (_int, [ctypes.POINTER(KVCache), ctypes.POINTER(KVRows), _vp, _i64, _i64, _i32, _vp, _i32, _f, _vp, _i64, _vp]),
+    "macko_cache_attention_wait_limit": (_int, [_i64]),
 }
 
 

@@ -16,6 +16,7 @@ struct AttentionArgs {
     long long q_row_stride, q_head_stride;
     int heads, unit_rows;
     float scale;             // times log2 e
+    unsigned wait_limit;     // nanoseconds that a wait inside the kernel for many rows may take
 };
 
 // Rows per unit of the kernel for many rows, and its launch (no join): prompt_attention.cu.

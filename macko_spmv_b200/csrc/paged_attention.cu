@@ -18,6 +18,7 @@
 // 4.5 TB/s. 32 tokens take a warp some 550 instructions, 160 of them conversions and byte interleaving, and 168 registers leave room for 12
 // warps of an SM. 16 warps with 16 tokens each and q in shared memory are no faster: sequences of equal length, 64 of 4096 tokens 348 against 343 us, 8192
 // tokens of one sequence 17.7 against 14.8.
+#include <atomic>
 #include <climits>
 
 #include "attention_args.cuh"
@@ -626,6 +627,8 @@ join_many_kernel(const AttentionArgs a)
     }
 }
 
+std::atomic<unsigned> g_wait_limit{2000000000u};   // nanoseconds
+
 int check_sizes(const macko_kv_cache *cache, const macko_kv_rows *batch, int heads, AttentionArgs *a)
 {
     if (int st = check_cache("paged_attention", cache, &a->cache)) return st;
@@ -779,10 +782,19 @@ int macko_cache_attention(const macko_kv_cache *cache, const macko_kv_rows *batc
     a.heads = heads;
     a.unit_rows = l.unit_rows;
     a.scale = scale * kLog2e;
+    a.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e4m3 = cache->code == MACKO_KV_E4M3;
     if (type == MACKO_BF16) return e4m3 ? launch_attention<true, true>(a, l, s) : launch_attention<true, false>(a, l, s);
     return e4m3 ? launch_attention<false, true>(a, l, s) : launch_attention<false, false>(a, l, s);
+}
+
+int macko_cache_attention_wait_limit(int64_t nanoseconds)
+{
+    if (nanoseconds < 0 || nanoseconds > 2000000000)
+        return fail(MACKO_ERR_INVALID_ARGUMENT, "paged_attention: a limit of %lld nanoseconds (0 .. 2000000000)", (long long)nanoseconds);
+    g_wait_limit.store((unsigned)nanoseconds, std::memory_order_relaxed);
+    return MACKO_OK;
 }
 
 }  // extern "C"

@@ -99,21 +99,49 @@ __device__ __forceinline__ void arrive(uint64_t *bar)
         asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_address(bar)) : "memory");
 }
 
-// Waits for the phase with parity `parity`; false (and from then on for every wait of the CTA) where it does not come. The thread
-// sleeps meanwhile, some microseconds at a time: the limit is a matter of seconds.
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *given_up)
+// What a wait needs to give up: a word of the CTA that says whether one has, and the longest time in nanoseconds.
+struct Patience {
+    volatile int *given_up;
+    uint32_t limit;
+};
+
+__device__ __forceinline__ uint32_t nanoseconds()
 {
-    const uint32_t at = smem_address(bar);
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+    return t;
+}
+
+// One look for the phase with parity `parity`, sleeping until it comes or up to `sleep` nanoseconds.
+__device__ __forceinline__ bool has_come(uint32_t at, uint32_t parity, uint32_t sleep)
+{
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(at), "r"(parity), "r"(sleep) : "memory");
+    return done != 0;
+}
+
+// Waits for the phase with parity `parity`; false (and from then on for every wait of the CTA) where it does not come in time. The clock
+// is looked at from the second try on.
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, const Patience &p)
+{
+    const uint32_t at = smem_address(bar), sleep = min(p.limit, 20000u);
+    if (has_come(at, parity, sleep)) return true;
+    const uint32_t began = nanoseconds();
 #pragma unroll 1
-    for (int i = 0; i < 1 << 20; ++i) {
-        uint32_t done;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(done) : "r"(at), "r"(parity), "r"(1000000u) : "memory");
-        if (done) return true;
-        if (*given_up) return false;
+    while (!*p.given_up) {
+        if (has_come(at, parity, sleep)) return true;
+        if (nanoseconds() - began >= p.limit) *p.given_up = 1;
     }
-    *given_up = 1;
     return false;
+}
+
+// The same for what must not be left behind when the CTA ends: a second at most, whatever the others have given up.
+__device__ __forceinline__ void wait_for_own(uint64_t *bar, uint32_t parity)
+{
+    const uint32_t began = nanoseconds();
+#pragma unroll 1
+    while (!has_come(smem_address(bar), parity, 20000u) && nanoseconds() - began < 1000000000u) {}
 }
 
 // `bytes` of global memory to shared memory; their arrival counts for the barrier.
@@ -270,18 +298,18 @@ struct Job {
     bool begins, ends;
 };
 
-__device__ __forceinline__ bool next_job(Job &job, const Job *jobs, uint64_t *bars, int &count, volatile int *given_up)
+__device__ __forceinline__ bool next_job(Job &job, const Job *jobs, uint64_t *bars, int &count, const Patience &patience)
 {
     const int slot = count & 1;
-    wait(bars + kJobFull + slot, (count >> 1) & 1, given_up);
+    wait(bars + kJobFull + slot, (count >> 1) & 1, patience);
     job = jobs[slot];
     arrive(bars + kJobEmpty + slot);
     ++count;
-    return job.h.first >= 0 && !*given_up;
+    return job.h.first >= 0 && !*patience.given_up;
 }
 
 // Finds the next piece and gives it to the others, and to the caller.
-__device__ __forceinline__ bool publish_job(Job &job, Job *jobs, WorkWalk &walk, const AttentionArgs &a, uint64_t *bars, int &count, volatile int *given_up)
+__device__ __forceinline__ bool publish_job(Job &job, Job *jobs, WorkWalk &walk, const AttentionArgs &a, uint64_t *bars, int &count, const Patience &patience)
 {
     Piece piece;
     const bool more = walk.next(a.work, a.rows, piece);
@@ -296,11 +324,11 @@ __device__ __forceinline__ bool publish_job(Job &job, Job *jobs, WorkWalk &walk,
         job.ends = piece.ends;
     }
     const int slot = count & 1;
-    wait(bars + kJobEmpty + slot, ((count >> 1) & 1) ^ 1, given_up);
+    wait(bars + kJobEmpty + slot, ((count >> 1) & 1) ^ 1, patience);
     if ((threadIdx.x & 31) == 0) jobs[slot] = job;
     arrive(bars + kJobFull + slot);
     ++count;
-    return more && !*given_up;
+    return more && !*patience.given_up;
 }
 
 template <bool BF16, bool E4M3, int D>
@@ -319,7 +347,7 @@ prompt_kernel(const AttentionArgs a)
     __shared__ int present[2][kConstSlots];           // of a tile of keys and of values: which of its blocks of 16 tokens lie on a page
     __shared__ Job jobs[2];
     __shared__ int given_up_word;
-    volatile int *given_up = &given_up_word;
+    const Patience patience = {&given_up_word, a.wait_limit};
     uint8_t *smem = raw + ((1024u - (smem_address(raw) & 1023u)) & 1023u);
     const RowsView &r = a.rows;
     const CacheView &c = a.cache;
@@ -351,7 +379,7 @@ prompt_kernel(const AttentionArgs a)
         const uint32_t s_half = tmem + lanes + half * 128, o_at = tmem + lanes + 256 + half * D;
         int done = 0;                       // tiles of this half in the pieces before
         int slot0 = 0;                      // tiles of the pieces before: where this piece's scales begin
-        while (next_job(job, jobs, bars, job_count, given_up)) {
+        while (next_job(job, jobs, bars, job_count, patience)) {
             const UnitRows &u = job.u;
             const HalfTiles &h = job.h;
             if (h.rows[half] > 0) {
@@ -416,7 +444,7 @@ prompt_kernel(const AttentionArgs a)
                 for (int j = h.first; j < h.end[half]; ++j) {
                     const int count = done + j - h.first, buffer = count & 1;
                     const uint32_t s_at = s_half + 64 * buffer;
-                    wait(bars + kSFull + 2 * half + buffer, (count >> 1) & 1, given_up);
+                    wait(bars + kSFull + 2 * half + buffer, (count >> 1) & 1, patience);
                     __syncwarp();
                     fence_after();
                     const float4 *of_tile = scales[(slot0 + j - h.first) % kConstSlots];
@@ -446,7 +474,7 @@ prompt_kernel(const AttentionArgs a)
                         far = __any_sync(0xffffffffu, m > kFar || (m < -kFar && m > -INFINITY));
                         l *= keep;
                         if (j > h.first) {
-                            wait(bars + kODone + 2 * half + (buffer ^ 1), ((count - 1) >> 1) & 1, given_up);
+                            wait(bars + kODone + 2 * half + (buffer ^ 1), ((count - 1) >> 1) & 1, patience);
                             __syncwarp();
                             fence_after();
 #pragma unroll 1
@@ -499,14 +527,14 @@ prompt_kernel(const AttentionArgs a)
                 // the result of this half, divided or as a piece
                 if (h.first < h.end[half]) {
                     done += h.end[half] - h.first;
-                    wait(bars + kODone + 2 * half + ((done - 1) & 1), ((done - 1) >> 1) & 1, given_up);
+                    wait(bars + kODone + 2 * half + ((done - 1) & 1), ((done - 1) >> 1) & 1, patience);
                     __syncwarp();
                     fence_after();
                 }
                 const bool alone = job.begins && job.ends, empty = h.first >= h.end[half];
                 float *partial = a.partial + ((long long)blockIdx.x * 2 + (job.begins ? 1 : 0)) * L::kRows * (D + 2);
                 float by = alone ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-                if (*given_up) by = __uint_as_float(0x7fffffffu);
+                if (*patience.given_up) by = __uint_as_float(0x7fffffffu);
                 // through this half's place for Q, which the tensor core is done with, so that some lanes write a row: 16-bit values in
                 // one pass, fp32 in two
                 const long long own_to = alone ? ((long long)(u.first_row + query) * a.heads + head) * D : (long long)row * D;
@@ -584,13 +612,13 @@ prompt_kernel(const AttentionArgs a)
         int n = 0;                                       // tiles so far
         Ring<L::kStages> ring;
         Ring<L::kCodeStages> codes_ring;
-        while (next_job(job, jobs, bars, job_count, given_up)) {
+        while (next_job(job, jobs, bars, job_count, patience)) {
             const HalfTiles &h = job.h;
             const int end = max(0, min(job.u.begin + job.u.queries, r.capacity));   // no row sees anything from here on
 #pragma unroll 1
             for (int j = h.first; j < h.last; ++j, ++n) {
-                wait(codes_full + codes_ring.stage, codes_ring.phase, given_up);
-                wait(empty + ring.stage, ring.phase ^ 1u, given_up);
+                wait(codes_full + codes_ring.stage, codes_ring.phase, patience);
+                wait(empty + ring.stage, ring.phase ^ 1u, patience);
                 __syncwarp();
                 const int blocks = present[is_v][n % kConstSlots];
                 const int rows = blocks == (1 << kGroups) - 1 ? end - j * kTile : -1;   // that are there, if all pages are
@@ -627,7 +655,7 @@ prompt_kernel(const AttentionArgs a)
             const uint64_t q = descriptor(operands + L::kQ + w * L::kHalf, 16, 1024);
             int n = 0, done = 0;                  // tiles of the pieces before, and those of them that this half took part in
             uint32_t q_phase = 0;
-            while (next_job(job, jobs, bars, job_count, given_up)) {
+            while (next_job(job, jobs, bars, job_count, patience)) {
                 const int first = __shfl_sync(0xffffffffu, job.h.first, 0), end = __shfl_sync(0xffffffffu, w ? job.h.end[1] : job.h.end[0], 0);
                 const int last = __shfl_sync(0xffffffffu, job.h.last, 0);
                 // S of the first two tiles, then for every tile: O += P V, and S of the second tile behind it. Tiles that the other half
@@ -639,9 +667,9 @@ prompt_kernel(const AttentionArgs a)
                     if (j >= first) {
                         const unsigned use = (unsigned)tile / kStages;
                         const int stage = tile - use * kStages;
-                        wait(bars + kVFull + stage, use & 1, given_up);
+                        wait(bars + kVFull + stage, use & 1, patience);
                         if (j < end) {
-                            wait(bars + kPFull + 2 * w + (count & 1), (count >> 1) & 1, given_up);
+                            wait(bars + kPFull + 2 * w + (count & 1), (count >> 1) & 1, patience);
                             __syncwarp();
                             fence_after();
                             if (elected()) {
@@ -659,10 +687,10 @@ prompt_kernel(const AttentionArgs a)
                     if (j + 2 < last) {
                         const unsigned use = (unsigned)(tile + 2) / kStages;
                         const int stage = tile + 2 - use * kStages;
-                        wait(bars + kKFull + stage, use & 1, given_up);
+                        wait(bars + kKFull + stage, use & 1, patience);
                         if (j + 2 < end) {
                             if (j + 2 == first) {
-                                wait(bars + kQFull + w, q_phase, given_up);
+                                wait(bars + kQFull + w, q_phase, patience);
                                 q_phase ^= 1u;
                             }
                             __syncwarp();
@@ -686,10 +714,7 @@ prompt_kernel(const AttentionArgs a)
                 done += max(end - first, 0);
             }
             // all that was issued has arrived before shared and tensor memory are given back
-            if (n > 0) {
-                int never = 0;
-                wait(bars + kVEmpty + (n - 1) % kStages, ((n - 1) / kStages) & 1, &never);
-            }
+            if (n > 0) wait_for_own(bars + kVEmpty + (n - 1) % kStages, ((n - 1) / kStages) & 1);
             __syncwarp();
         } else {
             // codes of keys (warp 18, with the scales of both) or of values: one lane for each block of 16 tokens, eight tiles at a time
@@ -702,7 +727,7 @@ prompt_kernel(const AttentionArgs a)
             WorkWalk walk;
             if (!is_v) walk.start(a.work, r, blockIdx.x);
             asm volatile("fence.proxy.async.global;" ::: "memory");   // the cache may have been written by the kernel in front
-            while (is_v ? next_job(job, jobs, bars, job_count, given_up) : publish_job(job, jobs, walk, a, bars, job_count, given_up)) {
+            while (is_v ? next_job(job, jobs, bars, job_count, patience) : publish_job(job, jobs, walk, a, bars, job_count, patience)) {
                 const HalfTiles &h = job.h;
                 const int end = max(0, min(job.u.begin + job.u.queries, r.capacity));
                 const uint8_t *base = (is_v ? c.v : c.k) + ((long long)job.kv_head << c.page_log2) * D;
@@ -725,7 +750,7 @@ prompt_kernel(const AttentionArgs a)
                     const uint32_t all = __ballot_sync(0xffffffffu, page >= 0);
 #pragma unroll 1
                     for (int t = 0; t < 32 / kGroups && j0 + t < h.last; ++t, ++n) {
-                        wait(empty + ring.stage, ring.phase ^ 1u, given_up);
+                        wait(empty + ring.stage, ring.phase ^ 1u, patience);
                         __syncwarp();
                         const int blocks = (all >> (t * kGroups)) & ((1 << kGroups) - 1);
                         if (lane == 0) present[is_v][n % kConstSlots] = blocks;
@@ -739,10 +764,7 @@ prompt_kernel(const AttentionArgs a)
                 }
             }
             // no copy is in flight when the CTA's shared memory is given back
-            for (int k = max(n - L::kCodeStages, 0); k < n; ++k) {
-                int never = 0;
-                wait(full + k % L::kCodeStages, (k / L::kCodeStages) & 1, &never);
-            }
+            for (int k = max(n - L::kCodeStages, 0); k < n; ++k) wait_for_own(full + k % L::kCodeStages, (k / L::kCodeStages) & 1);
             __syncwarp();
         }
     }

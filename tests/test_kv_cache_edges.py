@@ -77,3 +77,13 @@ def test_scores_far_from_zero(code, dtype, d, n):
             q = torch.zeros(3 * n, 4, d, device="cuda")
             q[..., 0] = sign * torch.exp2(e.float()) * 1.5
             _check(cache, rows, lengths, q.to(TYPES[dtype]), FEW if n == 1 else MANY)
+
+
+def test_limit_of_waits():
+    from macko_spmv_b200 import cabi
+
+    lib = cabi.load()
+    for bad in (-1, 2 * 10 ** 9 + 1, 1 << 40):
+        assert lib.macko_cache_attention_wait_limit(bad) == cabi.ERR_INVALID_ARGUMENT
+    for good in (0, 10 ** 6, 2 * 10 ** 9):
+        assert lib.macko_cache_attention_wait_limit(good) == cabi.OK
