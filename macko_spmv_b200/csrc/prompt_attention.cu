@@ -24,7 +24,9 @@
 // arithmetic nor conversions the first case still takes 279 us, without the products as well 182 (a wait for what is there already takes
 // 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other ways of waiting.
 //
-// Every wait has a limit: if one runs out, no further wait waits, and what the CTA writes from then on is NaN.
+// The warps that fetch codes look at the clock when they wait, the last one until all others have left. Where one waits too long, no wait of the CTA
+// goes on: no copy is started any more, the working warps go through what is left of their piece with whatever is there (all addresses come
+// from the piece), and each leaves as a whole where no further piece has come; tensor memory is given back behind what was issued.
 #include <type_traits>
 
 #include "attention_args.cuh"
@@ -40,6 +42,7 @@ constexpr int kConstSlots = 16;         // scales are fetched at most 9 tiles ah
 constexpr float kLeastFactor = 1e-36f;  // a score times nothing is still minus infinity where it is masked
 constexpr float kTop = 15.f, kLag = 4.f;  // exponents of the largest weight, which fp16 ends behind, and of what a maximum may lag (8, 4 and 2: the same time)
 constexpr float kFar = 1048576.f;       // 2^20, where steps of fp32 are an eighth
+constexpr uint32_t kSleep = 20000u;     // nanoseconds that a warp sleeps at a time while it waits
 constexpr int kWorkers = 19;            // warps that are given the CTA's pieces
 
 // Shared memory, from a 1024-byte boundary: Q of the halves, K and V stages, each as [64 dimensions][rows][128 bytes]; codes of K and V.
@@ -70,7 +73,8 @@ template <int N> struct Ring {
 // barriers for each half as well: both of the last two products may be done before anybody asks.)
 enum Barrier {
     kQFull = 0, kSFull = 2, kPFull = 6, kODone = 10, kJobFull = 14, kJobEmpty = 16, kKFull = 18, kKEmpty = 21, kVFull = 24, kVEmpty = 27,
-    kKCodesFull = 30, kKCodesEmpty = 33, kVCodesFull = 36, kVCodesEmpty = 39, kBarriers = 42
+    kKCodesFull = 30, kKCodesEmpty = 33, kVCodesFull = 36, kVCodesEmpty = 39,
+    kHalfDone = 42, kClosed = 44, kAllLeft = 46, kBarriers = 47
 };
 
 __device__ __forceinline__ int arrivals(int bar)
@@ -86,7 +90,9 @@ __device__ __forceinline__ int arrivals(int bar)
     if (bar < kKCodesFull) return 2;
     if (bar < kKCodesEmpty) return 1;
     if (bar < kVCodesFull) return 4;
-    return bar < kVCodesEmpty ? 1 : 4;
+    if (bar < kVCodesEmpty) return 1;
+    if (bar < kClosed) return 4;                               // warps of a converting group, and of a half
+    return bar < kAllLeft ? 1 : kWorkers;
 }
 
 __device__ __forceinline__ uint32_t smem_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -121,27 +127,34 @@ __device__ __forceinline__ bool has_come(uint32_t at, uint32_t parity, uint32_t 
     return done != 0;
 }
 
-// Waits for the phase with parity `parity`; false (and from then on for every wait of the CTA) where it does not come in time. The clock
-// is looked at from the second try on.
+// Waits for the phase with parity `parity`; false where it has not come when the CTA gives up.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, const Patience &p)
 {
-    const uint32_t at = smem_address(bar), sleep = min(p.limit, 20000u);
-    if (has_come(at, parity, sleep)) return true;
-    const uint32_t began = nanoseconds();
 #pragma unroll 1
-    while (!*p.given_up) {
-        if (has_come(at, parity, sleep)) return true;
-        if (nanoseconds() - began >= p.limit) *p.given_up = 1;
-    }
-    return false;
+    while (!has_come(smem_address(bar), parity, kSleep))
+        if (*p.given_up) return false;
+    return true;
 }
 
-// The same for what must not be left behind when the CTA ends: a second at most, whatever the others have given up.
+// The same for a warp of the two that fetch codes, which looks at the clock meanwhile: where the phase does not come in time, the CTA gives up.
+// (In every wait the clock costs the working warps 3 % of the kernel's time.) Whatever stops, one of these two waits for it before long.
+__device__ __forceinline__ bool timed_wait(uint64_t *bar, uint32_t parity, const Patience &p)
+{
+    bool here = has_come(smem_address(bar), parity, 0u);
+    const uint32_t began = nanoseconds();
+    while (!here && !*p.given_up) {
+        here = has_come(smem_address(bar), parity, min(p.limit, kSleep));
+        if (!here && nanoseconds() - began >= p.limit) *p.given_up = 1;
+    }
+    return __all_sync(0xffffffffu, here);
+}
+
+// For what must not be left behind when the CTA ends: a second at most, whatever the others have given up.
 __device__ __forceinline__ void wait_for_own(uint64_t *bar, uint32_t parity)
 {
     const uint32_t began = nanoseconds();
 #pragma unroll 1
-    while (!has_come(smem_address(bar), parity, 20000u) && nanoseconds() - began < 1000000000u) {}
+    while (!has_come(smem_address(bar), parity, kSleep) && nanoseconds() - began < 1000000000u) {}
 }
 
 // `bytes` of global memory to shared memory; their arrival counts for the barrier.
@@ -301,11 +314,12 @@ struct Job {
 __device__ __forceinline__ bool next_job(Job &job, const Job *jobs, uint64_t *bars, int &count, const Patience &patience)
 {
     const int slot = count & 1;
-    wait(bars + kJobFull + slot, (count >> 1) & 1, patience);
+    // a warp goes on or leaves as a whole
+    if (!__all_sync(0xffffffffu, wait(bars + kJobFull + slot, (count >> 1) & 1, patience))) return false;
     job = jobs[slot];
     arrive(bars + kJobEmpty + slot);
     ++count;
-    return job.h.first >= 0 && !*patience.given_up;
+    return job.h.first >= 0;
 }
 
 // Finds the next piece and gives it to the others, and to the caller.
@@ -324,11 +338,11 @@ __device__ __forceinline__ bool publish_job(Job &job, Job *jobs, WorkWalk &walk,
         job.ends = piece.ends;
     }
     const int slot = count & 1;
-    wait(bars + kJobEmpty + slot, ((count >> 1) & 1) ^ 1, patience);
+    if (!timed_wait(bars + kJobEmpty + slot, ((count >> 1) & 1) ^ 1, patience)) return false;
     if ((threadIdx.x & 31) == 0) jobs[slot] = job;
     arrive(bars + kJobFull + slot);
     ++count;
-    return more && !*patience.given_up;
+    return more;
 }
 
 template <bool BF16, bool E4M3, int D>
@@ -591,7 +605,9 @@ prompt_kernel(const AttentionArgs a)
                 fence_before();   // O is read before this half arrives for the next piece's P
             }
             // nobody's part of Q is written while another warp still has results there
-            asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+            arrive(bars + kHalfDone + half);
+            wait(bars + kHalfDone + half, (job_count - 1) & 1, patience);
+            __syncwarp();
             slot0 += max(h.last - h.first, 0);
         }
     } else if (group < 4) {
@@ -714,7 +730,9 @@ prompt_kernel(const AttentionArgs a)
                 done += max(end - first, 0);
             }
             // all that was issued has arrived before shared and tensor memory are given back
-            if (n > 0) wait_for_own(bars + kVEmpty + (n - 1) % kStages, ((n - 1) / kStages) & 1);
+            if (elected()) commit(bars + kClosed + w);
+            __syncwarp();
+            wait_for_own(bars + kClosed + w, 0);
             __syncwarp();
         } else {
             // codes of keys (warp 18, with the scales of both) or of values: one lane for each block of 16 tokens, eight tiles at a time
@@ -725,15 +743,16 @@ prompt_kernel(const AttentionArgs a)
             int n = 0;
             Ring<L::kCodeStages> ring;
             WorkWalk walk;
+            bool came = true;
             if (!is_v) walk.start(a.work, r, blockIdx.x);
             asm volatile("fence.proxy.async.global;" ::: "memory");   // the cache may have been written by the kernel in front
-            while (is_v ? next_job(job, jobs, bars, job_count, patience) : publish_job(job, jobs, walk, a, bars, job_count, patience)) {
+            while (came && (is_v ? next_job(job, jobs, bars, job_count, patience) : publish_job(job, jobs, walk, a, bars, job_count, patience))) {
                 const HalfTiles &h = job.h;
                 const int end = max(0, min(job.u.begin + job.u.queries, r.capacity));
                 const uint8_t *base = (is_v ? c.v : c.k) + ((long long)job.kv_head << c.page_log2) * D;
                 const long long page_stride = is_v ? c.v_stride : c.k_stride;
 #pragma unroll 1
-                for (int j0 = h.first; j0 < h.last; j0 += 32 / kGroups) {
+                for (int j0 = h.first; j0 < h.last && came; j0 += 32 / kGroups) {
                     const int tile = j0 + own_tile, token = tile * kTile + 16 * block;
                     const int page = tile < h.last && token < end ? page_at(c, r, job.sequence, token) : -1;
                     const uint8_t *source = base + page * page_stride + (token & page_mask) * D;
@@ -750,8 +769,8 @@ prompt_kernel(const AttentionArgs a)
                     const uint32_t all = __ballot_sync(0xffffffffu, page >= 0);
 #pragma unroll 1
                     for (int t = 0; t < 32 / kGroups && j0 + t < h.last; ++t, ++n) {
-                        wait(empty + ring.stage, ring.phase ^ 1u, patience);
-                        __syncwarp();
+                        came = timed_wait(empty + ring.stage, ring.phase ^ 1u, patience);
+                        if (!came) break;
                         const int blocks = (all >> (t * kGroups)) & ((1 << kGroups) - 1);
                         if (lane == 0) present[is_v][n % kConstSlots] = blocks;
                         if (!is_v && own_tile == t) scales[n % kConstSlots][block] = of_lane;
@@ -768,6 +787,8 @@ prompt_kernel(const AttentionArgs a)
             __syncwarp();
         }
     }
+    if (warp < kWorkers) arrive(bars + kAllLeft);
+    else timed_wait(bars + kAllLeft, 0, patience);
     fence_before();
     __syncthreads();
     fence_after();

@@ -87,3 +87,28 @@ def test_limit_of_waits():
         assert lib.macko_cache_attention_wait_limit(bad) == cabi.ERR_INVALID_ARGUMENT
     for good in (0, 10 ** 6, 2 * 10 ** 9):
         assert lib.macko_cache_attention_wait_limit(good) == cabi.OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_waits_that_run_out_end_the_call(d):
+    """With limits of nothing, some and tens of microseconds every wait of the many-rows kernel ends, wherever the CTA is then, and the next call is
+    as if nothing had been."""
+    from macko_spmv_b200 import cabi
+
+    lib = cabi.load()
+    lengths, rows = [3000, 500, 64, 7], [700, 500, 64, 7]
+    cache = Cache(lengths, 32, 2, d, torch.int8, seed=d)
+    lens, start = torch.tensor(lengths, dtype=torch.int32, device="cuda"), _starts(rows)
+    q = torch.randn(sum(rows), 8, d, generator=_gen(d), device="cuda").half()
+    good = macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start)
+    torch.cuda.synchronize()
+    try:
+        for limit in (0, 1, 300, 1000, 3000, 10000, 30000):
+            assert lib.macko_cache_attention_wait_limit(limit) == cabi.OK
+            for _ in range(3):
+                macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start)
+            torch.cuda.synchronize()
+    finally:
+        assert lib.macko_cache_attention_wait_limit(2 * 10 ** 9) == cabi.OK
+    assert torch.equal(macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start), good)
