@@ -7,8 +7,8 @@
 // of the call times heads of a group) in two halves of 128, tiles of 64 tokens. Five groups of warps:
 //
 //   0, 1   softmax of one half each, one row per thread: S from tensor memory, maximum, 2^x, P as fp16 over S in tensor memory; the
-//          accumulator is rescaled there when the maximum has grown by more than kLag, so that a row's largest weight is 2^11 to 2^15: fp16 rounds
-//          weights by 2^-11 of themselves down to 2^-25 of the largest, by 2^-36 of the largest below
+//          accumulator is rescaled there when the maximum has grown by more than kLag, so that a row's largest weight is 2^7 to 2^15: fp16 rounds
+//          weights by 2^-11 of themselves down to 2^-21 of the largest, by 2^-32 of the largest below
 //   2, 3   keys and values: codes from shared memory to fp16 (exact) in shared memory, in the 128-byte swizzle, three stages each
 //   4      one warp for each half that issues its tcgen05.mma: S = Q K^T from shared memory, O += P V with P from tensor memory and V as it
 //          lies (token by token: its "N" dimension is the contiguous one); two that fetch the codes of 16 tokens at a time with bulk
@@ -27,8 +27,6 @@
 // The warps that fetch codes look at the clock when they wait, the last one until all others have left. Where one waits too long, no wait of the CTA
 // goes on: no copy is started any more, the working warps go through what is left of their piece with whatever is there (all addresses come
 // from the piece), and each leaves as a whole where no further piece has come; tensor memory is given back behind what was issued.
-#include <type_traits>
-
 #include "attention_args.cuh"
 #include "launch.cuh"
 
@@ -40,7 +38,8 @@ constexpr int kTile = kPromptTile;
 constexpr int kGroups = kTile / 16;     // blocks of 16 tokens: each lies on one page
 constexpr int kConstSlots = 16;         // scales are fetched at most 9 tiles ahead of the softmax (codes, K, S)
 constexpr float kLeastFactor = 1e-36f;  // a score times nothing is still minus infinity where it is masked
-constexpr float kTop = 15.f, kLag = 4.f;  // exponents of the largest weight, which fp16 ends behind, and of what a maximum may lag (8, 4 and 2: the same time)
+constexpr float kTop = 15.f, kLag = 8.f;  // exponents of the largest weight, which fp16 ends behind, and of what a maximum may lag
+                                          // (by 4: pieces 340 instead of 333 us)
 constexpr float kFar = 1048576.f;       // 2^20, where steps of fp32 are an eighth
 constexpr uint32_t kSleep = 20000u;     // nanoseconds that a warp sleeps at a time while it waits
 constexpr int kWorkers = 19;            // warps that are given the CTA's pieces
@@ -505,35 +504,36 @@ prompt_kernel(const AttentionArgs a)
                     const float base = m == -INFINITY ? 0.f : m;
                     // 2^x below takes the product's own rounding and that of k.y - base for nothing, which holds as long as fp32 has fractions of the
                     // maximum. Beyond, x is what the maximum was found from, less m: nothing is above 2^15 then either.
-                    auto weights = [&](auto is_far) {
-                        constexpr bool kIsFar = decltype(is_far)::value;
+                    if (__builtin_expect(far, 0)) {
 #pragma unroll
-                        for (int two = 0; two < 2; ++two) {
-                            uint32_t p[16];
-#pragma unroll
-                            for (int gg = 0; gg < 2; ++gg) {
-                                const int g = 2 * two + gg;
-                                const float4 k = of_tile[g];
-                                const float by = fmaxf(k.x * factor, kLeastFactor), plus = k.y - base;
-                                const uint64_t by2 = pair(by, by), plus2 = kIsFar ? pair(k.y, k.y) : pair(plus, plus);
-                                uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-                                for (int i = 0; i < 16; i += 2) {
-                                    float2 x = unpair(fma_pair(pair(s[16 * g + i], s[16 * g + i + 1]), by2, plus2));
-                                    if (kIsFar) x = make_float2(x.x - base, x.y - base);
-                                    const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
-                                    sum[(i >> 1) & 1] = add_pair(sum[(i >> 1) & 1], pair(e0, e1));
-                                    p[8 * gg + i / 2] = pack2<false>(e0, e1);
-                                }
-                                const float2 both = unpair(add_pair(sum[0], sum[1]));
-                                const float all = both.x + both.y;
-                                l += all == 0.f ? 0.f : all * k.z;   // tokens that a row does not see may have any scale
-                            }
-                            tmem_store16(s_at + 16 * two, p);
+                        for (int i = 0; i < kTile; ++i) {
+                            const float4 k = of_tile[i / 16];
+                            s[i] = fmaf(s[i], fmaxf(k.x * factor, kLeastFactor), k.y) - base;
                         }
-                    };
-                    if (far) weights(std::true_type());
-                    else weights(std::false_type());
+                    }
+#pragma unroll
+                    for (int two = 0; two < 2; ++two) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int gg = 0; gg < 2; ++gg) {
+                            const int g = 2 * two + gg;
+                            const float4 k = of_tile[g];
+                            const float by = far ? 1.f : fmaxf(k.x * factor, kLeastFactor), plus = far ? 0.f : k.y - base;
+                            const uint64_t by2 = pair(by, by), plus2 = pair(plus, plus);
+                            uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const float2 x = unpair(fma_pair(pair(s[16 * g + i], s[16 * g + i + 1]), by2, plus2));
+                                const float e0 = exp2_fast(x.x), e1 = exp2_fast(x.y);
+                                sum[(i >> 1) & 1] = add_pair(sum[(i >> 1) & 1], pair(e0, e1));
+                                p[8 * gg + i / 2] = pack2<false>(e0, e1);
+                            }
+                            const float2 both = unpair(add_pair(sum[0], sum[1]));
+                            const float all = both.x + both.y;
+                            l += all == 0.f ? 0.f : all * k.z;   // tokens that a row does not see may have any scale
+                        }
+                        tmem_store16(s_at + 16 * two, p);
+                    }
                     tmem_store_wait();
                     fence_before();
                     arrive(bars + kPFull + 2 * half + buffer);
