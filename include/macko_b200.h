@@ -491,7 +491,8 @@ int64_t macko_cache_attention_workspace_bytes(int64_t sequences, int64_t rows, i
 int macko_cache_attention(const macko_kv_cache *cache, const macko_kv_rows *batch, const void *q, int64_t q_row_stride,
                           int64_t q_head_stride, int32_t type, void *out, int32_t heads, float scale, void *workspace,
                           int64_t workspace_bytes, void *stream);
-/* The longest time that a warp of the kernel for many rows waits for another one, 2000000000 ns unless set: for all calls of the process from now on. */
+/* The longest time that a warp of the kernel for many rows waits for another one, 2000000000 ns unless set: for all calls of the process from now on.
+ * Where a wait runs out, the rows that are lost with it are NaN; nothing else is known to make one run out than a smaller limit. */
 int macko_cache_attention_wait_limit(int64_t nanoseconds);
 
 #ifdef __cplusplus

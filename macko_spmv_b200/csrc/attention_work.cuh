@@ -25,7 +25,9 @@ struct WorkShape {
 // Rows of a unit that goes on in the CTAs behind: what the second kernel needs. pieces 0: nothing.
 struct SplitUnit {
     int first_row, rows, head, pieces;   // rows = queries * heads, packed query by query
-    int heads, unused[3];
+    int heads;
+    int lost;                            // 1: the CTA has given up; NaN is in all rows that it has a part in
+    int unused[2];
 };
 
 // sum of floor((a * i + b) / m) for i = 0 .. n - 1; a * n + b, once a and b are below m, fits 32 bits

@@ -443,7 +443,7 @@ few_rows_kernel(const AttentionArgs a)
             }
         }
         if (!alone && piece.begins && tid == 0)
-            a.split[blockIdx.x] = SplitUnit{u.first_row, n_rows, u.head, piece.pieces, u.heads, {0, 0, 0}};
+            a.split[blockIdx.x] = SplitUnit{u.first_row, n_rows, u.head, piece.pieces, u.heads, 0, {0, 0}};
         __syncthreads();
         more = walk.next(a.work, r, piece);
     }
@@ -578,9 +578,10 @@ join_many_kernel(const AttentionArgs a)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int4 *at = reinterpret_cast<const int4 *>(a.split + blockIdx.x);
     const int4 s = __ldcg(at);   // first row, rows, head, pieces
-    const int unit_heads = __ldcg(at + 1).x, lane = threadIdx.x & 31;
+    const int2 more = __ldcg(reinterpret_cast<const int2 *>(at + 1));   // heads, lost
+    const int unit_heads = more.x, lane = threadIdx.x & 31;
     const int row0 = (blockIdx.y * 16 + (threadIdx.x >> 5)) * R;
-    if (s.w == 0 || row0 >= s.y) return;
+    if (s.w == 0 || row0 >= s.y || more.y != 0) return;   // lost: NaN is there already
     const int stride = a.unit_rows * (D + 2);
     float m[R], l[R], o[R][V];
 #pragma unroll
@@ -590,10 +591,12 @@ join_many_kernel(const AttentionArgs a)
 #pragma unroll
         for (int j = 0; j < V; ++j) o[i][j] = 0.f;
     }
+    int lost = 0;
     for (int p = 0; p < s.w; ++p) {
         // the first piece is the second result of its CTA, the others are the first of theirs; rows behind the unit's have whatever
         // was there: they are not written
         const float *from = a.partial + ((long long)(blockIdx.x + p) * 2 + (p == 0)) * stride;
+        lost |= __ldcg(&a.split[blockIdx.x + p].lost);
         float pm[R], pl[R], po[R][V];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -620,7 +623,7 @@ join_many_kernel(const AttentionArgs a)
     for (int i = 0; i < R; ++i) {
         const int row = row0 + i;
         if (row >= s.y) break;
-        const float inverse = l[i] == 0.f ? 0.f : 1.f / l[i];
+        const float inverse = lost != 0 ? __uint_as_float(0x7fffffffu) : l[i] == 0.f ? 0.f : 1.f / l[i];
         uint16_t *to = a.out + ((long long)(s.x + row / unit_heads) * a.heads + s.z + row % unit_heads) * D + lane * V;
 #pragma unroll
         for (int j = 0; j < V; j += 2) *reinterpret_cast<uint32_t *>(to + j) = pack2<BF16>(o[i][j] * inverse, o[i][j + 1] * inverse);

@@ -24,9 +24,10 @@
 // arithmetic nor conversions the first case still takes 279 us, without the products as well 182 (a wait for what is there already takes
 // 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other ways of waiting.
 //
-// The warps that fetch codes look at the clock when they wait, the last one until all others have left. Where one waits too long, no wait of the CTA
+// The warps that fetch codes look at the clock when they wait, one of them until all others have left. Where one waits too long, no wait of the CTA
 // goes on: no copy is started any more, the working warps go through what is left of their piece with whatever is there (all addresses come
-// from the piece), and each leaves as a whole where no further piece has come; tensor memory is given back behind what was issued.
+// from the piece), and each leaves as a whole where no further piece has come; tensor memory is given back behind what was issued. The
+// rows that the CTA has a part in are filled with NaN, and the kernel that joins pieces leaves them so.
 #include "attention_args.cuh"
 #include "launch.cuh"
 
@@ -42,7 +43,7 @@ constexpr float kTop = 15.f, kLag = 8.f;  // exponents of the largest weight, wh
                                           // (by 4: pieces 340 instead of 333 us)
 constexpr float kFar = 1048576.f;       // 2^20, where steps of fp32 are an eighth
 constexpr uint32_t kSleep = 20000u;     // nanoseconds that a warp sleeps at a time while it waits
-constexpr int kWorkers = 19;            // warps that are given the CTA's pieces
+constexpr int kWorkers = 19;            // warps that are given the CTA's pieces by the one that finds them
 
 // Shared memory, from a 1024-byte boundary: Q of the halves, K and V stages, each as [64 dimensions][rows][128 bytes]; codes of K and V.
 // At head_dim 256 O takes 256 columns of tensor memory: units have one half, and there is room for two stages and for one of codes.
@@ -139,11 +140,14 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, const Patie
 // (In every wait the clock costs the working warps 3 % of the kernel's time.) Whatever stops, one of these two waits for it before long.
 __device__ __forceinline__ bool timed_wait(uint64_t *bar, uint32_t parity, const Patience &p)
 {
-    bool here = has_come(smem_address(bar), parity, 0u);
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(smem_address(bar)), "r"(parity) : "memory");
+    bool here = done != 0;
     const uint32_t began = nanoseconds();
     while (!here && !*p.given_up) {
-        here = has_come(smem_address(bar), parity, min(p.limit, kSleep));
-        if (!here && nanoseconds() - began >= p.limit) *p.given_up = 1;
+        if (nanoseconds() - began >= p.limit) *p.given_up = 1;
+        else here = has_come(smem_address(bar), parity, min(p.limit, kSleep));
     }
     return __all_sync(0xffffffffu, here);
 }
@@ -377,7 +381,7 @@ prompt_kernel(const AttentionArgs a)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (tid == 0) a.split[blockIdx.x].pieces = 0;
+    if (tid == 0) a.split[blockIdx.x].pieces = a.split[blockIdx.x].lost = 0;
     fence_before();
     __syncthreads();
     fence_after();
@@ -547,8 +551,7 @@ prompt_kernel(const AttentionArgs a)
                 }
                 const bool alone = job.begins && job.ends, empty = h.first >= h.end[half];
                 float *partial = a.partial + ((long long)blockIdx.x * 2 + (job.begins ? 1 : 0)) * L::kRows * (D + 2);
-                float by = alone ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-                if (*patience.given_up) by = __uint_as_float(0x7fffffffu);
+                const float by = alone ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 // through this half's place for Q, which the tensor core is done with, so that some lanes write a row: 16-bit values in
                 // one pass, fp32 in two
                 const long long own_to = alone ? ((long long)(u.first_row + query) * a.heads + head) * D : (long long)row * D;
@@ -601,7 +604,7 @@ prompt_kernel(const AttentionArgs a)
                     partial[L::kRows * D + L::kRows + row] = l;
                 }
                 if (!alone && job.begins && row == 0)
-                    a.split[blockIdx.x] = SplitUnit{u.first_row, u.rows(), u.head, job.pieces, u.heads, {0, 0, 0}};
+                    a.split[blockIdx.x] = SplitUnit{u.first_row, u.rows(), u.head, job.pieces, u.heads, 0, {0, 0}};
                 fence_before();   // O is read before this half arrives for the next piece's P
             }
             // nobody's part of Q is written while another warp still has results there
@@ -785,10 +788,24 @@ prompt_kernel(const AttentionArgs a)
             // no copy is in flight when the CTA's shared memory is given back
             for (int k = max(n - L::kCodeStages, 0); k < n; ++k) wait_for_own(full + k % L::kCodeStages, (k / L::kCodeStages) & 1);
             __syncwarp();
+            const bool all_left = is_v || timed_wait(bars + kAllLeft, 0, patience);
+            if (!is_v && __any_sync(0xffffffffu, !all_left || *patience.given_up)) {
+                // given up: NaN for all rows that the CTA has a part in, when nobody else writes any more
+                wait_for_own(bars + kAllLeft, 0);
+                Piece piece;
+                walk.start(a.work, r, blockIdx.x);
+                while (walk.next(a.work, r, piece)) {
+                    const UnitRows u = unit_rows(a, walk.s, piece);
+                    for (int row = 0; row < u.rows(); ++row) {
+                        uint32_t *to = reinterpret_cast<uint32_t *>(a.out + ((long long)(u.first_row + row / u.heads) * a.heads + u.head + row % u.heads) * D);
+                        for (int i = lane; i < D / 2; i += 32) to[i] = 0x7fff7fffu;
+                    }
+                }
+                if (lane == 0) a.split[blockIdx.x].lost = 1;
+            }
         }
     }
-    if (warp < kWorkers) arrive(bars + kAllLeft);
-    else timed_wait(bars + kAllLeft, 0, patience);
+    if (warp != 18) arrive(bars + kAllLeft);
     fence_before();
     __syncthreads();
     fence_after();

@@ -112,3 +112,30 @@ def test_waits_that_run_out_end_the_call(d):
     finally:
         assert lib.macko_cache_attention_wait_limit(2 * 10 ** 9) == cabi.OK
     assert torch.equal(macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start), good)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows,lengths", [([700, 500, 64, 7], [3000, 500, 64, 7]), ([100] * 40, [100 + 37 * i for i in range(40)]), ([300], [20000])])
+def test_rows_lost_with_a_wait_are_nan(rows, lengths, d):
+    """Every row of a call whose waits run out is right or NaN in all of a head, whatever was in its place before."""
+    from macko_spmv_b200 import cabi
+
+    lib = cabi.load()
+    cache = Cache(lengths, 32, 2, d, torch.int8, seed=d)
+    lens, start = torch.tensor(lengths, dtype=torch.int32, device="cuda"), _starts(rows)
+    q = torch.randn(sum(rows), 8, d, generator=_gen(d), device="cuda").bfloat16()
+    good = macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start)
+    try:
+        for limit, least in ((0, 0.9), (1, 0.9), (300, 0.0), (2000, 0.0), (8000, 0.0), (30000, 0.0)):
+            assert lib.macko_cache_attention_wait_limit(limit) == cabi.OK
+            for _ in range(3):
+                filled = torch.full_like(q, 7.0)                       # memory that the next result is likely to get
+                del filled
+                out = macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start)
+                lost = out.isnan().all(-1)
+                assert bool((lost[..., None] | (out == good)).all())
+                assert float(lost.float().mean()) >= least, limit
+    finally:
+        assert lib.macko_cache_attention_wait_limit(2 * 10 ** 9) == cabi.OK
+    assert torch.equal(macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start), good)
