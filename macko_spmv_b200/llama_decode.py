@@ -260,6 +260,8 @@ class LlamaDecoder(nn.Module):
         it through the multi-vector product or the dense-copy GEMM); returns the greedy next token [1]."""
         T = tokens.numel()
         if self.cache_dtype is not None:
+            if not 1 <= T <= self.max_len:
+                raise ValueError(f"a prompt of {T} tokens, room for 1 to {self.max_len}")
             ends = torch.tensor([0, T], dtype=torch.int32, device=tokens.device)
             return torch.argmax(self.extend(tokens, ends[1:], ends, self.page_table[:1])[0].float(), dim=-1, keepdim=True)
         x = self.embed.index_select(0, tokens)
@@ -272,16 +274,22 @@ class LlamaDecoder(nn.Module):
     def extend(self, tokens, lengths, query_start=None, page_table=None):
         """Rows of several sequences in one pass, with a paged cache: tokens int64 [N], of which query_start[i] .. query_start[i + 1] (int32 on
         the device; None: one each) are the last of sequence i, which has lengths[i] (int32) with them. Returns fp16 logits
-        [sequences, vocab] of every sequence's last row. `page_table`: the model's own (sequence i in its own pages) if None."""
+        [sequences, vocab] of every sequence's last row, NaN for a sequence that has no rows here or no tokens. `page_table`: the model's own
+        (sequence i in its own pages) if None."""
         if self.cache_dtype is None:
             raise RuntimeError("extend needs a paged cache (cache_dtype)")
-        table = self.page_table if page_table is None else page_table
+        table, n = self.page_table if page_table is None else page_table, tokens.numel()
+        if n == 0:
+            return self.embed.new_full((lengths.numel(), self.embed.shape[0]), float("nan"))
         x = self.embed.index_select(0, tokens)
         for blk in self.blocks:
             x = blk.extend(x, self.cos_table, self.sin_table, table, lengths, query_start)
+        none = lengths <= 0
         if query_start is not None:
-            x = x.index_select(0, (query_start[1:] - 1).clamp(min=0))
-        return self.lm_head(self.norm(x))
+            starts = query_start.clamp(0, n)   # as the kernels take it
+            none = none | (starts[1:] <= starts[:-1])
+            x = x.index_select(0, (starts[1:] - 1).clamp(min=0))
+        return self.lm_head(self.norm(x)).masked_fill(none[:, None], float("nan"))
 
     def logits(self, token, pos):
         """fp16 logits [vocab] of the token at position `pos`; updates the KV cache."""

@@ -15,7 +15,7 @@ import pytest
 import torch
 
 import macko_spmv_b200 as macko_spmv
-from test_kv_cache import CODES, TYPES, Cache, _attend_plain, _gen, _starts
+from test_kv_cache import CODES, TYPES, Cache, _attend_plain, _gen, _model, _starts
 
 FEW, MANY = 2.0 ** -40, 2.0 ** -32
 
@@ -139,3 +139,27 @@ def test_rows_lost_with_a_wait_are_nan(rows, lengths, d):
     finally:
         assert lib.macko_cache_attention_wait_limit(2 * 10 ** 9) == cabi.OK
     assert torch.equal(macko_spmv.paged_attention(q, cache.tensors, cache.table, lens, start), good)
+
+
+@pytest.mark.gpu
+def test_logits_of_sequences_without_rows():
+    """A padded call gives every sequence its own logits, or NaN; rows that query_start names beyond the call's are no rows. The products round
+    fp16 activations in another order for another number of sequences: 2^-11 a step, some ten steps in each of three layers, 2e-2 in all."""
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    prompts = [torch.randint(0, 1000, (n,), generator=_gen(80 + n), device="cuda") for n in (5, 9)]
+    with torch.no_grad():
+        model = _model(torch.int8, sequences=4)
+        logits = model.extend(torch.cat(prompts), i32(0, 5, 0, 9), i32(0, 0, 5, 5, 14))
+        alone = _model(torch.int8, sequences=4)
+        both = alone.extend(torch.cat(prompts), i32(5, 9), i32(0, 5, 14), alone.page_table[[1, 3]])
+        assert bool(logits[[0, 2]].isnan().all())
+        assert float((logits[[1, 3]] - both).float().norm() / both.float().norm()) < 2e-2
+        token = torch.tensor([1, 2, 3, 4], device="cuda")
+        step = model.extend(token, i32(0, 6, 0, 10))
+        assert step[[0, 2]].isnan().all() and not step[[1, 3]].isnan().any()
+        assert bool(model.extend(token[:0], i32(0, 6, 0, 10), i32(0, 0, 0, 0, 0)).isnan().all())
+        far = model.extend(token, i32(4, 0, 0, 0), i32(0, 4, 9, 9, 9))
+        assert bool(far[1:].isnan().all()) and not far[0].isnan().any()
+        for tokens in (token[:0], torch.zeros(71, dtype=torch.int64, device="cuda")):
+            with pytest.raises(ValueError):
+                model.prefill(tokens)
