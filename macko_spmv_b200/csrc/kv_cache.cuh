@@ -101,6 +101,9 @@ __device__ __forceinline__ void load_if(uint4 &x, const void *p, bool there)
 // The scale of a page's values as the softmax counts it: NaN stays NaN.
 __device__ __forceinline__ float value_scale(float scale) { return scale < kLowestScale ? kLowestScale : scale; }
 
+// 1 / scale; the quick division by more than 2^126 would be zero.
+__device__ __forceinline__ float inverse_scale(float scale) { return __fdividef(0.25f, 0.25f * scale); }
+
 // Four codes, as they lie in memory, as two pairs of fp16 values, exactly. int8: the byte with its sign bit flipped, put under
 // the exponent of 1024, is 1024 + 128 + code; 1152 is taken off again.
 template <bool E4M3>

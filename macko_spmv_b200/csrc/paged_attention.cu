@@ -210,7 +210,7 @@ few_rows_kernel(const AttentionArgs a)
                 const float vs = value_scale(__ldcg(c.v_scale + page * c.v_scale_stride + piece.kv_head));
                 ks_of_lane = __ldcg(c.k_scale + page * c.k_scale_stride + piece.kv_head);
                 shift_of_lane = __log2f(vs);
-                inverse_of_lane = __fdividef(1.f, vs);
+                inverse_of_lane = inverse_scale(vs);
             }
         };
         const uint8_t *const k_base = c.k + 16 * t + g * D, *const v_base = c.v + VB * g + 2 * t * D;

@@ -763,7 +763,7 @@ prompt_kernel(const AttentionArgs a)
                     if (!is_v && page >= 0) {
                         const float ks = __ldcg(c.k_scale + page * c.k_scale_stride + job.kv_head);
                         const float vs = value_scale(__ldcg(c.v_scale + page * c.v_scale_stride + job.kv_head));
-                        of_lane = ks < INFINITY && vs < INFINITY ? make_float4(ks, __log2f(vs), __fdividef(1.f, vs), 0.f)
+                        of_lane = ks < INFINITY && vs < INFINITY ? make_float4(ks, __log2f(vs), inverse_scale(vs), 0.f)
                                                                  : make_float4(0.f, 1e30f, __uint_as_float(0x7fffffffu), 0.f);
                     }
                     // with one stage of codes the way from memory would be a part of every tile: from the L2 cache it is a short one

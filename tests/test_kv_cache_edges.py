@@ -163,3 +163,15 @@ def test_logits_of_sequences_without_rows():
         for tokens in (token[:0], torch.zeros(71, dtype=torch.int64, device="cuda")):
             with pytest.raises(ValueError):
                 model.prefill(tokens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("n", [1, 60])
+def test_the_largest_scales_of_values(d, n):
+    """Scales of a user's own up to 2^127, with codes that keep the values inside bfloat16."""
+    lengths = [n + 70, n]
+    cache = Cache(lengths, 16, 2, d, torch.int8, seed=d)
+    cache.v.clamp_(-1, 1)
+    cache.vs.copy_(torch.exp2(torch.randint(122, 128, cache.vs.shape, generator=_gen(d), device="cuda").float()))
+    _check(cache, [n, n], lengths, (torch.randn(2 * n, 4, d, generator=_gen(n), device="cuda")).bfloat16(), FEW if n == 1 else MANY)
