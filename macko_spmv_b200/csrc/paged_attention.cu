@@ -20,6 +20,7 @@
 // tokens of one sequence 17.7 against 14.8.
 #include <atomic>
 #include <climits>
+#include <cmath>
 
 #include "attention_args.cuh"
 #include "launch.cuh"
@@ -764,6 +765,7 @@ int macko_cache_attention(const macko_kv_cache *cache, const macko_kv_rows *batc
     AttentionArgs a = {};
     if (int st = check_sizes(cache, batch, heads, &a)) return st;
     if (type != MACKO_FP16 && type != MACKO_BF16) return fail(MACKO_ERR_INVALID_ARGUMENT, "paged_attention: unknown type %d", type);
+    if (!std::isfinite(scale * kLog2e)) return fail(MACKO_ERR_INVALID_ARGUMENT, "paged_attention: scale %g", (double)scale);
     if (a.rows.rows == 0) return MACKO_OK;
     if (!q || !out) return fail(MACKO_ERR_INVALID_ARGUMENT, "paged_attention: null pointer");
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16) || q_row_stride % 8 || q_head_stride % 8)

@@ -89,6 +89,21 @@ def test_limit_of_waits():
         assert lib.macko_cache_attention_wait_limit(good) == cabi.OK
 
 
+def test_softmax_scales_that_are_not_finite_are_refused():
+    """(Many rows of a NaN scale gave the mean of the values, a few rows NaN.) No device is needed."""
+    import ctypes
+
+    from macko_spmv_b200 import cabi
+
+    lib, at = cabi.load(), 0x10000
+    cache = cabi.KVCache(k=at, v=at, k_scale=at, v_scale=at, k_page_stride=2 * 16 * 64, v_page_stride=2 * 16 * 64, k_scale_stride=2, v_scale_stride=2,
+                         pages=5, kv_heads=2, page_size=16, head_dim=64, code=0)
+    for rows in (3, 0):
+        batch = cabi.KVRows(page_table=at, lengths=at, query_start=at, table_stride=4, table_width=4, sequences=3, rows=rows)
+        for scale in (math.nan, math.inf, -math.inf, 3e38):
+            assert lib.macko_cache_attention(ctypes.byref(cache), ctypes.byref(batch), at, 4 * 64, 64, 0, at, 4, scale, at, 1 << 40, None) == cabi.ERR_INVALID_ARGUMENT
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_waits_that_run_out_end_the_call(d):
