@@ -15,7 +15,7 @@ import pytest
 import torch
 
 import macko_spmv_b200 as macko_spmv
-from test_kv_cache import CODES, TYPES, Cache, _attend_plain, _gen, _model, _starts
+from test_kv_cache import CODES, TYPES, Cache, _attend_plain, _check_append, _check_attend, _gen, _model, _starts
 
 FEW, MANY = 2.0 ** -40, 2.0 ** -32
 
@@ -190,3 +190,59 @@ def test_the_largest_scales_of_values(d, n):
     cache.v.clamp_(-1, 1)
     cache.vs.copy_(torch.exp2(torch.randint(122, 128, cache.vs.shape, generator=_gen(d), device="cuda").float()))
     _check(cache, [n, n], lengths, (torch.randn(2 * n, 4, d, generator=_gen(n), device="cuda")).bfloat16(), FEW if n == 1 else MANY)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("d,page,hq,hkv", [(64, 16, 6, 2), (128, 32, 4, 4), (128, 64, 16, 1), (256, 128, 4, 2), (64, 128, 3, 3), (256, 16, 24, 1), (128, 16, 7, 1), (256, 64, 9, 3)])
+@pytest.mark.parametrize("longest", [33, 500, 1000, 2300])
+def test_one_row_each_without_query_start(code, dtype, d, page, hq, hkv, longest):
+    """Decoding as it is called most: tables of up to 1024 tokens, where every unit has a CTA of its own, and longer ones. Empty sequences, ones that are
+    longer than their table, and pages that are none."""
+    lengths = [1, longest, 0, 2, longest // 2 + 1, longest + 5000, 16, 17, longest - 1, 0]
+    cache = Cache([min(n, longest) for n in lengths], page, hkv, d, CODES[code], seed=d + page, strided=page == 32)
+    cache.table[4, 0] = -3
+    cache.table[8, cache.table.shape[1] // 2] = 1 << 30
+    for start in ("none", "given"):
+        _check_attend(cache, [1] * len(lengths), lengths, hq, TYPES[dtype], seed=hq, start=start)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("longest", [100, 3000])
+def test_one_row_each_on_pages_that_are_not_finite(longest):
+    lengths = [longest, 100, 90]
+    cache = Cache(lengths, 16, 2, 64, torch.int8, seed=36)
+    q = torch.randn(3, 4, 64, generator=_gen(37), device="cuda").half()
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    clean = macko_spmv.paged_attention(q, cache.tensors, cache.table, lens)
+    cache.vs[int(cache.table[0, 1]), 1] = float("nan")
+    cache.ks[int(cache.table[1, 0]), 0] = float("nan")
+    out = macko_spmv.paged_attention(q, cache.tensors, cache.table, lens)
+    assert bool(out[0, 2:].isnan().all()) and torch.equal(out[0, :2], clean[0, :2])
+    assert bool(out[1, :2].isnan().all()) and torch.equal(out[1, 2:], clean[1, 2:])
+    assert torch.equal(out[2], clean[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_padded_batches_of_many_rows(d):
+    """Long runs of sequences without rows in front of, between and behind prompts, through the kernel for many rows (20 heads a cache head: 38 rows
+    a sequence on average)."""
+    rows = [0] * 40 + [300] + [0] * 70 + [300, 2, 0, 1] + [0] * 200
+    lengths = [(r + 20 if r else 0) for r in rows]
+    cache = Cache(lengths, 16, 2, d, torch.int8, seed=61)
+    out = _check_attend(cache, rows, lengths, 40, torch.float16, seed=63, extra_rows=77)
+    assert bool((out[sum(rows):] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("single,prompt", [(200, 2048), (60, 4096), (300, 700)])
+def test_a_prompt_next_to_single_tokens(code, single, prompt):
+    """Single tokens of many sequences and a prompt in one call, through either kernel, appended and attended to."""
+    rows = [1] * (single // 2) + [prompt] + [1] * (single - single // 2)
+    lengths = [prompt + 5 if r > 1 else 1 + (37 * i) % 900 for i, r in enumerate(rows)]
+    cache = Cache(lengths, 32, 2, 64, CODES[code], seed=single)
+    _check_append(cache, rows, lengths, 2, torch.bfloat16, seed=1)
+    _check_attend(cache, rows, lengths, 2, torch.bfloat16, seed=2)
