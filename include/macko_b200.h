@@ -454,7 +454,7 @@ int macko_decode_argmax(const void *values, int64_t n, int64_t *index, void *str
 
 typedef struct macko_kv_cache {
     void *k, *v;                             /* [pages][kv_heads][page_size][head_dim] codes, 16-byte aligned */
-    float *k_scale, *v_scale;                /* [pages][kv_heads], greater than zero */
+    float *k_scale, *v_scale;                /* [pages][kv_heads], greater than zero; those of values below 2^-64 count as 2^-64 */
     int64_t k_page_stride, v_page_stride;    /* bytes between pages, multiples of 16; times pages at most 2^36 */
     int64_t k_scale_stride, v_scale_stride;  /* floats between pages */
     int64_t pages;
@@ -476,9 +476,9 @@ typedef struct macko_kv_rows {
  *   rows on that page fit the codes, or the scale that the page has if that is larger and the page held tokens of the sequence
  *   before; those are moved to the new scale where it grows. A value that is not finite makes the scale of its page and head NaN,
  *   for good: whoever attends to that page gets NaN. Slots behind the last token keep their bytes. A page must be written for
- *   one sequence only in one call, and calls that write one page must not overlap.
+ *   one place of one sequence only in one call, and calls that write one page must not overlap.
  * macko_cache_attention: out[row][head] = sum over the tokens t at or before the row's position of softmax(scale * q . k_t) v_t, in
- *   out [rows][heads][head_dim]; head h reads key head h / (heads / kv_heads). A row that sees nothing gives zeros. q: rows
+ *   out [rows][heads][head_dim]; head h reads key head h / (heads / kv_heads). A row that sees nothing gives zeros; `scale` is finite. q: rows
  *   q_row_stride and heads q_head_stride elements apart, both multiples of 8, 16-byte aligned. `workspace`: scratch of this call
  *   alone of macko_cache_attention_workspace_bytes(...) bytes, 16-byte aligned (the size depends on the arguments that it
  *   takes and on the current device; negative: they are out of range).

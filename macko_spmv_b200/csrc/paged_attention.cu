@@ -14,9 +14,9 @@
 // lane loads 16 consecutive bytes of a token; bytes of two tokens are interleaved for V. The next K is asked for when this one has been
 // converted, and V alike, so a warp has its 8 KB in flight all the time; the turn behind that is on its way to the L2 cache.
 //
-// 64 sequences of 205 to 4096 tokens, 32 heads of 128, e4m3: 226 us, 5.2 TB/s, 0.80 of what a copy moves; 131072 tokens, 8 cache heads: 60 us,
-// 4.5 TB/s. 32 tokens take a warp some 550 instructions, 160 of them conversions and byte interleaving, and 168 registers leave room for 12
-// warps of an SM. 16 warps with 16 tokens each and q in shared memory are no faster: sequences of equal length, 64 of 4096 tokens 348 against 343 us, 8192
+// 64 sequences of 205 to 4096 tokens, 32 heads of 128, e4m3: 229 us, 5.1 TB/s, 0.79 of what a copy moves; 131072 tokens, 8 cache heads: 61 us,
+// 4.4 TB/s. 32 tokens take a warp some 550 instructions, 160 of them conversions and byte interleaving, and 168 registers leave room for 12
+// warps of an SM (with 310 bytes of a thread spilled at head_dim 128; units of 16 rows, 255 registers and 8 warps: 30 to 90 at 128, 740 to 840 at 256). 16 warps with 16 tokens each and q in shared memory are no faster: sequences of equal length, 64 of 4096 tokens 348 against 343 us, 8192
 // tokens of one sequence 17.7 against 14.8.
 #include <atomic>
 #include <climits>
@@ -661,7 +661,9 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     // The kernel for many rows takes 128 or 256 as long as one; the other reads and converts the cache once for 16. 16 sequences of 8000
     // tokens, head_dim 128, 12 / 32 / 40 / 64 rows: 69 / 128 / 180 / 235 us against 134 / 141 / 142 / 142; 4 of 2000, 32 rows: 21 / 26; head_dim 64,
     // 32 / 40 / 64 rows: 92 / 131 / 170 against 122 / 123 / 124; head_dim 256, 16 / 24 / 32 rows: 158 / 286 / 290 against 202 / 206 / 208, and 24 rows of
-    // 1 of 8000, 4 of 2000, 16 of 1000: 36 / 38 / 65 against 65 / 39 / 50.
+    // 1 of 8000, 4 of 2000, 16 of 1000: 36 / 38 / 65 against 65 / 39 / 50. (So at 256 a few sequences would have a higher limit, many a lower one.)
+    // The mean takes in sequences without rows and single tokens, and one kernel serves the call: 8 heads of 128, a prompt of 4096 tokens with 300 sequences
+    // without rows 261 us, bare 90; with 200 single tokens over 4000 each 621 together, 269 and 91 in two calls; with 60 of them 367, 93 and 90.
     const bool prompt = !one_each && mean > (d == 256 ? 24 : 32);
     // Units of 8 rows where they suffice: 16 sequences of 8000 tokens, 8 rows 58 us against 68 with units of 16, 10 rows 97 against 69.
     const int rows = prompt ? prompt_rows(d) : mean <= 8 ? 8 : 16;
@@ -685,7 +687,8 @@ int plan_launch(const AttentionArgs &a, int heads, int sm_count, Launch *l)
     const int64_t units = (int64_t)a.rows.sequences * a.cache.kv_heads * l->work.parts;
     // One CTA per unit where the table has room for few tokens: shares and the second kernel take some microseconds. Tables of 200 / 512 /
     // 1024 / 2048 tokens, one sequence of 32 heads: 6.0 / 8.7 / 14.2 / 25.1 us against 11.4 / 11.6 / 12.1 / 14.4; 16 sequences of 8 cache
-    // heads, 512 / 1024: 10.7 / 17.2 against 14.2 / 16.5; 64 such: 16.0 / 25.3 against 21.9 / 27.0.
+    // heads, 512 / 1024: 10.7 / 17.2 against 14.2 / 16.5; 64 such: 16.0 / 25.3 against 21.9 / 27.0. (The two meet between 512 and 1024: at the limit itself
+    // shares are the faster ones of the first two.)
     l->split = !(one_each && a.rows.capacity <= 1024);
     l->ctas = l->split ? l->sm_count * (prompt ? 1 : rows == 8 && d <= 128 ? 3 : 2) : 0;
     if (!l->split) {

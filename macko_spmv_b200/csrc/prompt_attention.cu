@@ -18,11 +18,11 @@
 // the softmax of this one is done. (With one S of 128 columns a half waited for its P to go through the tensor core and for the next S,
 // 1900 of 5400 cycles for 128 tokens.)
 //
-// 4 pieces of up to 512 rows over up to 16384 tokens, 32/8 heads of 128, int8: 333 us, 805 TFLOP/s (0.48 of a cuBLAS product in a burst);
-// a 4096-token prompt, 32 heads, e4m3: 216 us, 636 TFLOP/s. The tensor pipe is active 40 % of the time, a scheduler issues 0.56 instructions
-// a cycle, 1430 for a tile. What bounds it is the chain from S through a half's softmax and P to the next S: with neither softmax
-// arithmetic nor conversions the first case still takes 279 us, without the products as well 182 (a wait for what is there already takes
-// 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other ways of waiting.
+// 4 pieces of up to 512 rows over up to 16384 tokens, 32/8 heads of 128, int8: 339 us, 790 TFLOP/s (0.47 of a cuBLAS product in a burst);
+// a 4096-token prompt, 32 heads, e4m3: 213 us, 644 TFLOP/s. The tensor pipe is active 42 % of the time, a scheduler issues 0.56 instructions
+// a cycle, 1360 for a tile. What bounds it is the chain from S through a half's softmax and P to the next S: with neither softmax
+// arithmetic nor conversions the first case took 279 of 333 us, without the products as well 182 (a wait for what is there already takes
+// 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other lengths of sleep while waiting.
 //
 // The warps that fetch codes look at the clock when they wait, one of them until all others have left. Where one waits too long, no wait of the CTA
 // goes on: no copy is started any more, the working warps go through what is left of their piece with whatever is there (all addresses come

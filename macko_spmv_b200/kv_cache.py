@@ -1,7 +1,8 @@
 """A key/value cache in 8 bits, in pages, for several sequences, and the two operators that a model runs on it.
 
 A cache is four tensors (`KVCache`): k and v [pages, kv_heads, page_size, head_dim] of torch.int8 or torch.float8_e4m3fn, and
-k_scale, v_scale [pages, kv_heads] of torch.float32; a value is its code times the scale of its page and head. Next to weights
+k_scale, v_scale [pages, kv_heads] of torch.float32; a value is its code times the scale of its page and head (scales are greater than zero, and those of
+values below 2^-64 count as 2^-64). Next to weights
 that are pruned and compressed the cache is what a decode step reads most of: half the bytes of an fp16 cache.
 
 Which tokens belong to which sequence is said by three int32 tensors on the device, read when the kernels run (so a captured call
@@ -58,7 +59,7 @@ def rope_append(qkv, cos_table, sin_table, cache, page_table, lengths, query_sta
     """Rotates q and k of the call's rows at their positions and puts k and v into the cache; returns q [rows, heads, head_dim].
 
     qkv [rows, (heads + 2 * kv_heads) * head_dim], fp16 or bfloat16: q, k and v of every row, not yet rotated (what a stacked
-    q/k/v projection returns; rows may be strided). cos_table, sin_table: fp16 [positions, head_dim] with both halves equal, rows for every
+    q/k/v projection returns; rows may be strided, each 16-byte aligned). cos_table, sin_table: fp16 [positions, head_dim] with both halves equal, rows for every
     position that the page table can name (rotate-half, as in `rope_attention`).
 
     The scale of a page and head is the smallest power of two (2^-64 or more) with which the call's rows on that page fit the type; it
@@ -68,7 +69,7 @@ def rope_append(qkv, cos_table, sin_table, cache, page_table, lengths, query_sta
     rows of no sequence get a q of zeros, and slots behind the last token are left as they were.
 
     A page may be read by many sequences but written for one: calls that write the same page must not overlap on the GPU, and the
-    rows of one call must not share a page between sequences."""
+    rows of one call must not share a page between sequences, or between two places of one."""
     if not _is_compiling():
         q = _direct_append(qkv, cos_table, sin_table, cache, page_table, lengths, query_start)   # None: not a plain call
         if q is not None:
@@ -80,9 +81,13 @@ def rope_append(qkv, cos_table, sin_table, cache, page_table, lengths, query_sta
 def paged_attention(q, cache, page_table, lengths, query_start=None, scale=None):
     """softmax(scale * q K^T) V over the cached tokens at or before each row's position; returns [rows, heads, head_dim] of q's type.
 
-    q [rows, heads, head_dim], fp16 or bfloat16, rotated (heads and rows may be strided); heads must be a multiple of the cache's, and head h reads
-    the cache's head h // (heads // kv_heads). scale: 1 / sqrt(head_dim) if None. A row that sees no token (an empty sequence, rows of no
-    sequence) gives zeros. Sums and the softmax are kept in fp32; the weights of the values are rounded to fp16 on the way."""
+    q [rows, heads, head_dim], fp16 or bfloat16, rotated (heads and rows may be strided, all 16-byte aligned); heads must be a multiple of the cache's, and head h reads
+    the cache's head h // (heads // kv_heads). scale: 1 / sqrt(head_dim) if None, else a finite number. A row that sees no token (an empty sequence, rows of no
+    sequence) gives zeros. Sums and the softmax are kept in fp32; the weights of the values are rounded to fp16 on the way, by half a step or by 2^-32 of
+    the row's largest product of a weight and its value's scale.
+
+    One kernel serves the whole call, chosen by the mean number of rows of a sequence, those without rows among them: a call takes longer than its parts
+    where a long prompt stands next to many single tokens or empty sequences, and is better made as two."""
     if not _is_compiling():
         out = _direct_attention(q, cache, page_table, lengths, query_start, scale)   # None: not a plain call
         if out is not None:
