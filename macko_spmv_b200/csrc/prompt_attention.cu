@@ -25,8 +25,8 @@
 // 100 to 150 cycles). Tried without gain: 2^x of a part of the scores on the FMA pipe, other lengths of sleep while waiting.
 //
 // The warps that fetch codes look at the clock when they wait, one of them until all others have left. Where one waits too long, no wait of the CTA
-// goes on: no copy is started any more, the working warps go through what is left of their piece with whatever is there (all addresses come
-// from the piece), and each leaves as a whole where no further piece has come; tensor memory is given back behind what was issued. The
+// goes on: no copy is started any more, and the working warps leave their piece and then their loop, each as a whole, after a tile at most of whatever
+// is there (all addresses come from the piece); tensor memory is given back behind what was issued. The
 // rows that the CTA has a part in are filled with NaN, and the kernel that joins pieces leaves them so.
 #include "attention_args.cuh"
 #include "launch.cuh"
@@ -149,7 +149,8 @@ __device__ __forceinline__ bool timed_wait(uint64_t *bar, uint32_t parity, const
         if (nanoseconds() - began >= p.limit) *p.given_up = 1;
         else here = has_come(smem_address(bar), parity, min(p.limit, kSleep));
     }
-    return __all_sync(0xffffffffu, here);
+    // (also where the phase has come: what is given back after giving up may not have arrived yet)
+    return __all_sync(0xffffffffu, here && !*p.given_up);
 }
 
 // For what must not be left behind when the CTA ends: a second at most, whatever the others have given up.
@@ -461,7 +462,7 @@ prompt_kernel(const AttentionArgs a)
                 for (int j = h.first; j < h.end[half]; ++j) {
                     const int count = done + j - h.first, buffer = count & 1;
                     const uint32_t s_at = s_half + 64 * buffer;
-                    wait(bars + kSFull + 2 * half + buffer, (count >> 1) & 1, patience);
+                    const bool late = !wait(bars + kSFull + 2 * half + buffer, (count >> 1) & 1, patience);
                     __syncwarp();
                     fence_after();
                     const float4 *of_tile = scales[(slot0 + j - h.first) % kConstSlots];
@@ -485,7 +486,8 @@ prompt_kernel(const AttentionArgs a)
                         most = fmaxf(most, fmaf(fmaxf(top, top2), fmaxf(k.x * factor, kLeastFactor), k.y));
                     }
                     const bool grown = most - m > kTop;   // the difference of numbers that are near one another is exact
-                    if (__any_sync(0xffffffffu, grown)) {
+                    if (__any_sync(0xffffffffu, grown || late)) {
+                        if (__any_sync(0xffffffffu, late)) break;   // given up
                         const float to = grown ? __fadd_ru(most, kLag - kTop) : m, keep = grown ? exp2_fast(m - to) : 1.f;
                         m = to;
                         far = __any_sync(0xffffffffu, m > kFar || (m < -kFar && m > -INFINITY));
@@ -636,9 +638,8 @@ prompt_kernel(const AttentionArgs a)
             const int end = max(0, min(job.u.begin + job.u.queries, r.capacity));   // no row sees anything from here on
 #pragma unroll 1
             for (int j = h.first; j < h.last; ++j, ++n) {
-                wait(codes_full + codes_ring.stage, codes_ring.phase, patience);
-                wait(empty + ring.stage, ring.phase ^ 1u, patience);
-                __syncwarp();
+                if (!__all_sync(0xffffffffu, wait(codes_full + codes_ring.stage, codes_ring.phase, patience) && wait(empty + ring.stage, ring.phase ^ 1u, patience)))
+                    break;
                 const int blocks = present[is_v][n % kConstSlots];
                 const int rows = blocks == (1 << kGroups) - 1 ? end - j * kTile : -1;   // that are there, if all pages are
 #pragma unroll
@@ -688,8 +689,7 @@ prompt_kernel(const AttentionArgs a)
                         const int stage = tile - use * kStages;
                         wait(bars + kVFull + stage, use & 1, patience);
                         if (j < end) {
-                            wait(bars + kPFull + 2 * w + (count & 1), (count >> 1) & 1, patience);
-                            __syncwarp();
+                            if (!__all_sync(0xffffffffu, wait(bars + kPFull + 2 * w + (count & 1), (count >> 1) & 1, patience))) break;
                             fence_after();
                             if (elected()) {
                                 const uint64_t v = descriptor(operands + L::kV + stage * L::kStage, kBlock, 1024);
