@@ -16,8 +16,9 @@
 //
 // 64 sequences of 205 to 4096 tokens, 32 heads of 128, e4m3: 229 us, 5.1 TB/s, 0.79 of what a copy moves; 131072 tokens, 8 cache heads: 61 us,
 // 4.4 TB/s. 32 tokens take a warp some 550 instructions, 160 of them conversions and byte interleaving, and 168 registers leave room for 12
-// warps of an SM (with 310 bytes of a thread spilled at head_dim 128; units of 16 rows, 255 registers and 8 warps: 30 to 90 at 128, 740 to 840 at 256). 16 warps with 16 tokens each and q in shared memory are no faster: sequences of equal length, 64 of 4096 tokens 348 against 343 us, 8192
-// tokens of one sequence 17.7 against 14.8.
+// warps of an SM (with 310 bytes of a thread spilled at head_dim 128; units of 16 rows, 255 registers and 8 warps: 30 to 90 at 128, 740 to 840 at 256).
+// 16 warps with 16 tokens each and q in shared memory are no faster: sequences of equal length, 64 of 4096 tokens 348 against 343 us, 8192 tokens of
+// one sequence 17.7 against 14.8.
 #include <atomic>
 #include <climits>
 #include <cmath>

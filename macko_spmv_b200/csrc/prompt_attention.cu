@@ -26,8 +26,8 @@
 //
 // The warps that fetch codes look at the clock when they wait, one of them until all others have left. Where one waits too long, no wait of the CTA
 // goes on: no copy is started any more, and the working warps leave their piece and then their loop, each as a whole, after a tile at most of whatever
-// is there (all addresses come from the piece); tensor memory is given back behind what was issued. The
-// rows that the CTA has a part in are filled with NaN, and the kernel that joins pieces leaves them so.
+// is there (all addresses come from the piece); tensor memory is given back behind what was issued. The rows that the CTA has a part in are filled with
+// NaN, and the kernel that joins pieces leaves them so.
 #include "attention_args.cuh"
 #include "launch.cuh"
 
